@@ -162,6 +162,106 @@ int mq_linear_ragged(const mq_weight *w, const float *x, const int *offsets, int
 int mq_linear_noalloc(const mq_weight *w, const float *x, int m, int ldx, const float *bias, float *y, int ldy,
                       void *stream);
 
+/* ---- Paged 4-bit key/value cache for serving: what a forward over ragged
+ * requests needs between its projections (mq_linear_ragged). A cache holds,
+ * for each layer, `pages` pages of `page_size` consecutive tokens of one
+ * request; page ids are shared by the layers. Every 32 elements of a key or
+ * value row are a Q4_0 block, c * d with c in [-8, 7]: for the block's first
+ * element s of largest |x|, d = fp16(bf16(s / -8)), and c = x / d rounded to
+ * nearest even and clamped. (d has 8 significant bits, so that every c * d is
+ * an fp16 number.) A block with a non-finite element, or whose |d| would pass
+ * 8160, is stored as NaN, and attention that sees it answers NaN. 4.5 bits an
+ * element. No counterpart in the reference, whose forward keeps one
+ * max_seq_len F32 cache per context (src/forward.cc).
+ *
+ * A step: mq_pages_plan once, then for each layer mq_kv4_store and
+ * mq_kv4_attention on the same stream. All lengths, offsets and tables are
+ * int32 device arrays, read by the kernels when they run: a captured graph
+ * serves every step of its buffers' sizes. No call allocates or synchronises,
+ * except a creation without memory of its own and its destruction. */
+typedef struct mq_kv4 mq_kv4;
+
+/* Device bytes of a cache: layers * pages * page_size * kv_heads * head_dim *
+ * 9 / 8; 0 (and mq_last_error) for a shape that mq_kv4_create refuses. */
+size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head_dim);
+
+/* A cache of zeros on `device`. page_size: a multiple of 16 up to 1024;
+ * head_dim: 32, 64, 96 or 128; pages * page_size < 2^31. `memory` is the
+ * caller's device memory for it (at least mq_kv4_bytes(), 16-byte aligned),
+ * which must outlive the handle and is cleared on `stream`; NULL allocates
+ * it, which synchronizes `stream`. */
+int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads, int head_dim, void *memory,
+                  size_t memory_bytes, void *stream, mq_kv4 **out);
+void mq_kv4_destroy(mq_kv4 *c);
+
+/* Shape, device and device bytes of a handle (any out-pointer may be NULL). */
+int mq_kv4_info(const mq_kv4 *c, int *device, int *layers, int *pages, int *page_size, int *kv_heads, int *head_dim,
+                size_t *device_bytes);
+
+/* Packs key and value rows into `layer` at `slots` (slot = page id *
+ * page_size + place in the page; a row whose slot is negative or past the
+ * cache is skipped). Head h of row i: device F32 k + i * ld_k + h * hs_k,
+ * head_dim elements (the rows of a fused [q | k | v] projection: ld its row
+ * length, hs = head_dim); any alignment to 4 bytes works, 16-byte pointers
+ * and strides run faster. The slots of one call must differ: of two rows for
+ * one slot, either may win each block. */
+int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64_t hs_k, const float *v, int64_t ld_v,
+                 int64_t hs_v, const int *slots, int rows, void *stream);
+
+/* The values that `layer` holds at `slots`, into k and v [rows][kv_heads]
+ * [head_dim]; rows of a negative slot or one past the cache are 0. */
+int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k, float *v, void *stream);
+
+/* Workspace bytes of mq_kv4_attention for this cache, head count and
+ * max_new, whatever the batch; 0 for a NULL handle. */
+size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new);
+
+/* Causal attention over the cache: row i of request r (rows offsets[r] ..
+ * offsets[r + 1] - 1 of q and out; offsets[0] = 0, non-decreasing) stands at
+ * position seq_lens[r] - (offsets[r + 1] - offsets[r]) + i of its request and
+ * sees positions 0 up to its own, at most seq_lens[r] of them:
+ *   out = softmax(scale * q . k) v, query head h with KV head h / (heads / kv_heads).
+ * seq_lens counts the step's own rows, which mq_kv4_store has written.
+ * block_tables [n_seqs][max_pages] page ids; lengths past max_pages *
+ * page_size count as that, and tokens of a page id outside the cache are not
+ * seen. A row that sees nothing is 0; rows past offsets[n_seqs] stay as they
+ * are, and no row past `rows` is touched. max_new: the most rows that a
+ * request brings, as far as the caller knows; it selects kernels and a lower
+ * or higher value costs time only. q and out as in mq_kv4_store; out may be q
+ * only if it has q's strides. F32 softmax and sums; q and the softmax weights
+ * enter the tensor cores as fp16 hi + lo pairs (22 bits). workspace: device
+ * memory of at least mq_kv4_attention_workspace() bytes, 16-byte aligned,
+ * not shared with a call that may run at the same time; its contents do not
+ * matter. The summation order is fixed: equal inputs give equal bits. */
+int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
+                     const int *offsets, const int *seq_lens, const int *block_tables, int n_seqs, int max_pages,
+                     int max_new, float scale, float *out, int64_t ld_out, int64_t hs_out, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Block tables and slot map of a step, from the lengths of its requests
+ * (n_seqs <= 8192). Request r holds ctx_lens[r] tokens, in the pages of its
+ * row of block_tables [n_seqs][max_pages], and brings new_lens[r] rows. The
+ * further pages that it needs are taken from the top of the stack free_pages
+ * (capacity n_pages, *n_free of them valid) in request order and entered in
+ * its row. Out: offsets [n_seqs + 1], the rows before each request;
+ * seq_lens [n_seqs] = ctx + new (may be ctx_lens); slots and positions
+ * [rows], -1 behind the last request; *n_free_out (may be n_free).
+ * A request is refused when a length is negative, when ctx + new passes
+ * max_pages * page_size, when its rows pass `rows`, or when it needs pages
+ * and it and the requests before it need more than *n_free: its table,
+ * length and the stack stay as they were, and its rows get slot -1.
+ * *refused counts them. */
+int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_seqs, int page_size, int *block_tables,
+                  int max_pages, const int *free_pages, int n_pages, const int *n_free, int rows, int *offsets,
+                  int *seq_lens, int *slots, int *positions, int *n_free_out, int *refused, void *stream);
+
+/* Ends requests: pushes the pages of requests[0..n) (indices of the rows of
+ * block_tables; those outside [0, n_seqs) are skipped, one named twice counts
+ * once) onto the stack and sets their seq_lens to 0. The stack never passes
+ * its capacity n_pages. */
+int mq_pages_release(int device, const int *requests, int n, int n_seqs, int page_size, int *seq_lens,
+                     const int *block_tables, int max_pages, int *free_pages, int n_pages, int *n_free, void *stream);
+
 /* ---- Row-sharded linear across GPUs (one process or host thread per GPU).
  * A weight of N = G*R rows is split into G equal output-row shards
  * (mq_weight_shard_create with rows [r*R, (r+1)*R) on rank r). Each rank

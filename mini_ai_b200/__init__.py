@@ -4,6 +4,7 @@ The engine is the shared library ``libmq_b200.so`` (C ABI, include/mq_b200.h);
 this package is the host-side mirror of the reference operator surface over it.
 """
 from ._lib import LIB_PATH, MQError, lib
+from .kv_cache import Kv4Cache, PagePlan, PlanPages, ReleasePages
 from .quantized_tensor import (BlockBytes, CudaDeviceInfo, CudaWeight, DequantizeTensor, Linear, LinearDispatch,
                                LinearSwiGlu, QuantizedStorage, QuantizeTensor, QuantType, TensorFromQuantized,
                                set_path)
@@ -12,5 +13,6 @@ from .sharded import CudaComm, ShardedLinear, assemble, shard_rows
 __all__ = [
     "LIB_PATH", "MQError", "lib", "BlockBytes", "CudaDeviceInfo", "CudaWeight", "DequantizeTensor", "Linear",
     "LinearDispatch", "LinearSwiGlu", "QuantizedStorage", "QuantizeTensor", "QuantType", "TensorFromQuantized", "set_path",
+    "Kv4Cache", "PagePlan", "PlanPages", "ReleasePages",
     "CudaComm", "ShardedLinear", "assemble", "shard_rows",
 ]

@@ -22,7 +22,7 @@ MQ_ERR_TIMEOUT = -6
 MQ_ERR_UNSUPPORTED = -7
 
 # Every symbol include/mq_b200.h declares, with (restype, argtypes).
-_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_vp, _i, _sz, _f, _i64 = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_int64
 SIGNATURES = {
     "mq_last_error": (C.c_char_p, []),
     "mq_version": (C.c_char_p, []),
@@ -40,6 +40,17 @@ SIGNATURES = {
     "mq_linear_noalloc": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i, _vp]),
     "mq_linear_swiglu": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _vp]),
     "mq_linear_residual": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
+    "mq_kv4_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "mq_kv4_create": (_i, [_i, _i, _i, _i, _i, _i, _vp, _sz, _vp, C.POINTER(_vp)]),
+    "mq_kv4_destroy": (None, [_vp]),
+    "mq_kv4_info": (_i, [_vp] + [C.POINTER(_i)] * 6 + [C.POINTER(_sz)]),
+    "mq_kv4_store": (_i, [_vp, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp]),
+    "mq_kv4_load": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "mq_kv4_attention_workspace": (_sz, [_vp, _i, _i]),
+    "mq_kv4_attention": (_i, [_vp, _i, _vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _i64, _i64, _vp,
+                              _sz, _vp]),
+    "mq_pages_plan": (_i, [_i, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mq_pages_release": (_i, [_i, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _vp]),
     "mq_comm_unique_id": (_i, [_vp, _sz]),
     "mq_comm_create": (_i, [_i, _i, _i, _vp, _sz, C.POINTER(_vp)]),
     "mq_comm_destroy": (None, [_vp]),

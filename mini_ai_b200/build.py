@@ -14,7 +14,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmq_b200.so"
-SOURCES = [CSRC / "mq_abi.cu", CSRC / "mq_noalloc.cu", CSRC / "mq_comm.cu"]
+SOURCES = [CSRC / "mq_abi.cu", CSRC / "mq_noalloc.cu", CSRC / "mq_comm.cu", CSRC / "mq_kv4.cu"]
 DEPS = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [ROOT / "include" / "mq_b200.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,302 @@
+// C-ABI entry points of the paged 4-bit key/value cache and of the block
+// tables that address it (declared in include/mq_b200.h).
+//
+// No call here allocates or synchronises except creation and destruction of a
+// cache: all of them may be captured in a CUDA graph, and what a call needs
+// beside its arguments is the caller's workspace, so graphs share nothing.
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "mq_kv4.cuh"
+#include "mq_kv4_attn.cuh"
+#include "mq_pages.cuh"
+#include "mq_tcdec_api.h"
+
+using namespace mq;
+
+namespace {
+
+// Switches the calling thread to `device` for the scope and restores it.
+struct OnDevice {
+  int prev = -1;
+  cudaError_t err = cudaSuccess;
+  explicit OnDevice(int device) {
+    err = cudaGetDevice(&prev);
+    if (err == cudaSuccess && prev != device) err = cudaSetDevice(device);
+    else if (err == cudaSuccess) prev = -1;
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+int check_device(int device) {
+  int count = 0;
+  const cudaError_t e = cudaGetDeviceCount(&count);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDeviceCount");
+  if (device < 0 || device >= count) return fail(MQ_ERR_INVALID, "CUDA device id %d out of range", device);
+  if (!gemm_supported(device)) return fail(MQ_ERR_UNSUPPORTED, "the kernels need an sm_100 device (device %d)", device);
+  return MQ_OK;
+}
+
+bool valid_page(int page) { return page >= kKv4Unit && page <= 1024 && page % kKv4Unit == 0; }
+
+// Rows [rows][heads][hd] of floats, heads of one row not overlapping.
+int check_rows(const char *what, const float *p, int64_t ld, int64_t hs, int heads, int hd) {
+  if (!p) return fail(MQ_ERR_INVALID, "null %s pointer", what);
+  if (reinterpret_cast<uintptr_t>(p) % sizeof(float)) return fail(MQ_ERR_INVALID, "%s is not aligned to a float", what);
+  if (ld < 0 || hs < 0 || (heads > 1 && hs < hd))
+    return fail(MQ_ERR_INVALID, "%s strides (%lld, %lld) do not hold heads of %d", what, (long long)ld, (long long)hs,
+                hd);
+  return MQ_OK;
+}
+
+bool vector16(const void *p, int64_t ld, int64_t hs) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0 && hs % 4 == 0;
+}
+
+int check_cache(const mq_kv4 *c, int layer) {
+  if (!c) return fail(MQ_ERR_INVALID, "null cache handle");
+  if (layer < 0 || layer >= c->v.layers) return fail(MQ_ERR_INVALID, "layer %d of %d", layer, c->v.layers);
+  return MQ_OK;
+}
+
+int cache_shape(int layers, int pages, int page_size, int kv_heads, int head_dim, Kv4View &v, size_t &bytes) {
+  if (layers < 1 || pages < 1 || kv_heads < 1)
+    return fail(MQ_ERR_INVALID, "invalid cache shape: %d layers, %d pages, %d heads", layers, pages, kv_heads);
+  if (!valid_page(page_size))
+    return fail(MQ_ERR_INVALID, "page size %d: a multiple of %d up to 1024 is needed", page_size, kKv4Unit);
+  if (head_dim < 32 || head_dim > 128 || head_dim % 32)
+    return fail(MQ_ERR_INVALID, "head size %d: 32, 64, 96 or 128 is needed", head_dim);
+  if ((int64_t)pages * page_size > INT_MAX)
+    return fail(MQ_ERR_INVALID, "%d pages of %d tokens: slots must stay below 2^31", pages, page_size);
+  const int nb = head_dim / 32;
+  const int64_t page_head = (int64_t)(page_size / kKv4Unit) * kv4_unit_bytes(nb);
+  const int64_t slices = (int64_t)layers * pages;  // both below 2^31
+  if (slices > INT64_MAX / page_head / kv_heads) return fail(MQ_ERR_INVALID, "cache size overflow");
+  v = Kv4View{nullptr, layers, pages, page_size, kv_heads, head_dim, nb, page_head};
+  bytes = (size_t)(slices * kv_heads * page_head);
+  return MQ_OK;
+}
+
+int launched(const char *what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  count_launch();
+  return MQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head_dim) {
+  Kv4View v;
+  size_t bytes = 0;
+  last_error().clear();
+  return cache_shape(layers, pages, page_size, kv_heads, head_dim, v, bytes) == MQ_OK ? bytes : 0;
+}
+
+int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads, int head_dim, void *memory,
+                  size_t memory_bytes, void *stream, mq_kv4 **out) {
+  last_error().clear();
+  if (!out) return fail(MQ_ERR_INVALID, "null output handle");
+  *out = nullptr;
+  Kv4View v;
+  size_t bytes = 0;
+  if (int rc = cache_shape(layers, pages, page_size, kv_heads, head_dim, v, bytes)) return rc;
+  if (memory && memory_bytes < bytes)
+    return fail(MQ_ERR_SIZE, "cache memory: %zu bytes, %zu are needed", memory_bytes, bytes);
+  if (reinterpret_cast<uintptr_t>(memory) % 16) return fail(MQ_ERR_INVALID, "cache memory is not aligned to 16 bytes");
+  if (int rc = check_device(device)) return rc;
+  OnDevice g(device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  auto *c = new (std::nothrow) mq_kv4;
+  if (!c) return fail(MQ_ERR_INVALID, "out of host memory");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  void *base = memory;
+  if (!base) e = cudaMalloc(&base, bytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // an allocation that does not fit is no fault of later calls
+    delete c;
+    return cuda_fail(e, "cudaMalloc cache");
+  }
+  e = cudaMemsetAsync(base, 0, bytes, s);
+  if (e == cudaSuccess && !memory) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) {
+    if (!memory) cudaFree(base);
+    delete c;
+    return cuda_fail(e, "clear cache");
+  }
+  v.base = static_cast<uint8_t *>(base);
+  c->device = device;
+  c->v = v;
+  c->bytes = bytes;
+  c->owned = memory ? nullptr : base;
+  *out = c;
+  return MQ_OK;
+}
+
+void mq_kv4_destroy(mq_kv4 *c) {
+  if (!c) return;
+  if (c->owned) {
+    OnDevice g(c->device);
+    cudaFree(c->owned);
+  }
+  delete c;
+}
+
+int mq_kv4_info(const mq_kv4 *c, int *device, int *layers, int *pages, int *page_size, int *kv_heads, int *head_dim,
+                size_t *device_bytes) {
+  last_error().clear();
+  if (!c) return fail(MQ_ERR_INVALID, "null cache handle");
+  if (device) *device = c->device;
+  if (layers) *layers = c->v.layers;
+  if (pages) *pages = c->v.pages;
+  if (page_size) *page_size = c->v.page;
+  if (kv_heads) *kv_heads = c->v.kv;
+  if (head_dim) *head_dim = c->v.hd;
+  if (device_bytes) *device_bytes = c->bytes;
+  return MQ_OK;
+}
+
+int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64_t hs_k, const float *v, int64_t ld_v,
+                 int64_t hs_v, const int *slots, int rows, void *stream) {
+  last_error().clear();
+  if (int rc = check_cache(c, layer)) return rc;
+  if (rows < 0) return fail(MQ_ERR_INVALID, "negative row count %d", rows);
+  if (rows == 0) return MQ_OK;
+  if (int rc = check_rows("key", k, ld_k, hs_k, c->v.kv, c->v.hd)) return rc;
+  if (int rc = check_rows("value", v, ld_v, hs_v, c->v.kv, c->v.hd)) return rc;
+  if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
+  const int64_t blocks = ((int64_t)rows * 8 * c->v.kv * c->v.nb + kKv4Threads - 1) / kKv4Threads;
+  if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
+  OnDevice g(c->device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Kv4Rows kr{k, ld_k, hs_k}, vr{v, ld_v, hs_v};
+  if (vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v))
+    kv4_store_kernel<true><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
+  else
+    kv4_store_kernel<false><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
+  return launched("cache store");
+}
+
+int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k, float *v, void *stream) {
+  last_error().clear();
+  if (int rc = check_cache(c, layer)) return rc;
+  if (rows < 0) return fail(MQ_ERR_INVALID, "negative row count %d", rows);
+  if (rows == 0) return MQ_OK;
+  const int64_t ld = (int64_t)c->v.kv * c->v.hd;
+  if (int rc = check_rows("key", k, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
+  if (int rc = check_rows("value", v, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
+  if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
+  const int64_t blocks = ((int64_t)rows * 8 * c->v.kv * c->v.nb + kKv4Threads - 1) / kKv4Threads;
+  if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
+  OnDevice g(c->device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (vector16(k, 0, 0) && vector16(v, 0, 0))
+    kv4_load_kernel<true><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
+  else
+    kv4_load_kernel<false><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
+  return launched("cache load");
+}
+
+size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new) {
+  (void)heads, (void)max_new;
+  return c ? 16 : 0;
+}
+
+int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
+                     const int *offsets, const int *seq_lens, const int *block_tables, int n_seqs, int max_pages,
+                     int max_new, float scale, float *out, int64_t ld_out, int64_t hs_out, void *workspace,
+                     size_t workspace_bytes, void *stream) {
+  last_error().clear();
+  if (int rc = check_cache(c, layer)) return rc;
+  if (rows < 0 || n_seqs < 0) return fail(MQ_ERR_INVALID, "negative count: %d rows, %d requests", rows, n_seqs);
+  if (heads < 1 || heads % c->v.kv)
+    return fail(MQ_ERR_INVALID, "%d query heads do not share %d key/value heads evenly", heads, c->v.kv);
+  if (max_pages < 1 || max_new < 0) return fail(MQ_ERR_INVALID, "%d pages a request, %d new rows", max_pages, max_new);
+  if (!std::isfinite(scale)) return fail(MQ_ERR_INVALID, "the score scale is not finite");
+  if (rows == 0 || n_seqs == 0) return MQ_OK;
+  if (int rc = check_rows("query", q, ld_q, hs_q, heads, c->v.hd)) return rc;
+  if (int rc = check_rows("output", out, ld_out, hs_out, heads, c->v.hd)) return rc;
+  if (!offsets || !seq_lens || !block_tables) return fail(MQ_ERR_INVALID, "null offsets, lengths or block tables");
+  const size_t need = mq_kv4_attention_workspace(c, heads, max_new);
+  if (!workspace || workspace_bytes < need)
+    return fail(MQ_ERR_SIZE, "attention workspace: %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(MQ_ERR_INVALID, "the attention workspace is not aligned to 16 bytes");
+  OnDevice g(c->device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Kv4AttnArgs a{c->v, layer, q, ld_q, hs_q, out, ld_out, hs_out, offsets, seq_lens, block_tables,
+                      n_seqs, max_pages, rows, heads, scale};
+  kv4_attention_kernel<<<dim3(rows, heads), 32, 0, s>>>(a);
+  return launched("cache attention");
+}
+
+int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_seqs, int page_size, int *block_tables,
+                  int max_pages, const int *free_pages, int n_pages, const int *n_free, int rows, int *offsets,
+                  int *seq_lens, int *slots, int *positions, int *n_free_out, int *refused, void *stream) {
+  last_error().clear();
+  if (n_seqs < 0 || n_seqs > kPagesMaxSeqs)
+    return fail(MQ_ERR_INVALID, "%d requests: at most %d are planned in one call", n_seqs, kPagesMaxSeqs);
+  if (rows < 0) return fail(MQ_ERR_INVALID, "negative row count %d", rows);
+  if (!valid_page(page_size))
+    return fail(MQ_ERR_INVALID, "page size %d: a multiple of %d up to 1024 is needed", page_size, kKv4Unit);
+  if (max_pages < 1 || n_pages < 0 || (int64_t)max_pages * page_size > INT_MAX)
+    return fail(MQ_ERR_INVALID, "%d pages a request, %d free pages", max_pages, n_pages);
+  if ((n_seqs && (!ctx_lens || !new_lens || !block_tables || !seq_lens)) || (rows && (!slots || !positions)) ||
+      (n_pages && !free_pages) || !n_free || !offsets || !n_free_out || !refused)
+    return fail(MQ_ERR_INVALID, "null pointer");
+  if (seq_lens == new_lens && n_seqs) return fail(MQ_ERR_INVALID, "the lengths may not replace the new row counts");
+  if (int rc = check_device(device)) return rc;
+  OnDevice g(device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  const PagesArgs a{ctx_lens, new_lens, n_seqs, page_size, block_tables, max_pages, free_pages, n_pages,
+                    n_free, rows, offsets, seq_lens, slots, positions, n_free_out, refused};
+  const size_t smem = pages_smem(n_seqs);
+  if (smem > 48 * 1024)
+    MQ_CUDA(cudaFuncSetAttribute(pages_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)pages_smem(kPagesMaxSeqs)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows > 4 * kPagesThreads ? kPagesCluster : 1);
+  cfg.blockDim = dim3(kPagesThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cfg.gridDim.x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MQ_CUDA(cudaLaunchKernelEx(&cfg, pages_plan_kernel, a));
+  count_launch();
+  return MQ_OK;
+}
+
+int mq_pages_release(int device, const int *requests, int n, int n_seqs, int page_size, int *seq_lens,
+                     const int *block_tables, int max_pages, int *free_pages, int n_pages, int *n_free, void *stream) {
+  last_error().clear();
+  if (n < 0 || n_seqs < 0) return fail(MQ_ERR_INVALID, "negative count: %d of %d requests", n, n_seqs);
+  if (!valid_page(page_size))
+    return fail(MQ_ERR_INVALID, "page size %d: a multiple of %d up to 1024 is needed", page_size, kKv4Unit);
+  if (max_pages < 1 || n_pages < 0 || (int64_t)max_pages * page_size > INT_MAX)
+    return fail(MQ_ERR_INVALID, "%d pages a request, %d free pages", max_pages, n_pages);
+  if (n == 0 || n_seqs == 0) return MQ_OK;
+  if (!requests || !seq_lens || !block_tables || (n_pages && !free_pages) || !n_free)
+    return fail(MQ_ERR_INVALID, "null pointer");
+  if (int rc = check_device(device)) return rc;
+  OnDevice g(device);
+  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  pages_release_kernel<<<1, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      requests, n, n_seqs, page_size, seq_lens, block_tables, max_pages, free_pages, n_pages, n_free);
+  return launched("release pages");
+}
+
+}  // extern "C"

@@ -1,0 +1,183 @@
+// Block tables and slot maps of a ragged batch, built on the GPU.
+//
+// A cache page holds `page` consecutive tokens of one request; a request's
+// block table lists its pages, and token p of it lives in slot
+// table[p / page] * page + p % page. A step brings new_r rows to request r,
+// which holds ctx_r tokens: the plan appends the pages that they need, taken
+// from the top of a stack of free pages in request order, and writes every
+// row's slot and position.
+//
+//   held_r = ceil(ctx_r / page), need_r = ceil((ctx_r + new_r) / page)
+//   offset_r = sum of new over the requests before r, first_r = sum of
+//   need - held over them; page i >= held_r of request r is
+//   free[n_free - 1 - (first_r + i - held_r)].
+//
+// The bytes are few (a thousand requests with 64k rows: 0.5 MB), so latency
+// bounds it: one launch, in which every CTA of one cluster computes the two
+// prefix sums itself (R loads, no exchange), waits once for the others to have
+// read the inputs that the outputs may overwrite, and writes its share of the
+// rows.
+#pragma once
+
+#include "mq_common.cuh"
+#include "mq_sm100.cuh"
+
+namespace mq {
+
+constexpr int kPagesThreads = 1024;
+constexpr int kPagesMaxSeqs = 8192;  // shared memory: 12 bytes a request
+constexpr int kPagesCluster = 8;     // CTAs of a large batch
+
+struct PagesArgs {
+  const int *ctx, *fresh;  // tokens held and tokens brought, per request
+  int n, page;
+  int *tables;
+  int width;  // pages per table row
+  const int *stack;
+  int capacity;
+  const int *n_free;
+  int rows;
+  int *offsets, *lens, *slots, *positions, *n_free_out, *refused;
+};
+
+__host__ __device__ constexpr size_t pages_smem(int n) { return (size_t)(3 * n + 1) * sizeof(int); }
+
+// Inclusive sum over the CTA's threads; `total` the CTA's sum. Two barriers.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int w = 0; w < nwarps; ++w) {
+    const int64_t s = warp_sums[w];
+    if (w < warp) before += s;
+    all += s;
+  }
+  total = all;
+  __syncthreads();
+  return v + before;
+}
+
+__global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesArgs a) {
+  extern __shared__ int pages_sm[];
+  __shared__ int64_t warp_sums[kPagesThreads / 32];
+  int *off = pages_sm, *ctx = off + a.n + 1, *first = ctx + a.n;  // first: -1 of a refused request
+  const int ncta = gridDim.x, cta = blockIdx.x;
+  const int n_free = min(max(*a.n_free, 0), a.capacity);
+  const int64_t room = (int64_t)a.width * a.page;
+  int64_t rows_before = 0, pages_before = 0;  // over earlier chunks of requests
+  int refused = 0, taken = 0;                 // this thread's
+  for (int r0 = 0; r0 < a.n; r0 += blockDim.x) {
+    const int r = r0 + threadIdx.x;
+    const bool real = r < a.n;
+    const int c = real ? a.ctx[r] : 0, m = real ? a.fresh[r] : 0;
+    int64_t sum;
+    const int64_t end = rows_before + block_scan(max(m, 0), warp_sums, sum);
+    rows_before += sum;
+    const bool fits = real && c >= 0 && m >= 0 && (int64_t)c + m <= room && end <= a.rows;
+    const int more = fits ? (int)(((int64_t)c + m + a.page - 1) / a.page - ((int64_t)c + a.page - 1) / a.page) : 0;
+    const int64_t upto = pages_before + block_scan(more, warp_sums, sum);
+    pages_before += sum;
+    if (real) {
+      const bool served = fits && (more == 0 || upto <= n_free);
+      off[r + 1] = (int)min(end, (int64_t)INT_MAX);
+      ctx[r] = c;
+      first[r] = served ? (int)min(upto - more, (int64_t)INT_MAX) : -1;
+      refused += !served;
+      taken += served ? more : 0;
+    }
+  }
+  if (threadIdx.x == 0) off[0] = 0;
+  int64_t all_refused, all_taken;
+  block_scan(refused, warp_sums, all_refused);
+  block_scan(taken, warp_sums, all_taken);  // its barriers order the writes of off, ctx and first
+  // seq_lens may be ctx_lens, and n_free_out may be n_free: every CTA has read them.
+  if (ncta > 1) sm100::cluster_sync();
+  if (cta == 0) {
+    for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
+      a.offsets[r + 1] = off[r + 1];
+      a.lens[r] = first[r] < 0 ? ctx[r] : ctx[r] + off[r + 1] - off[r];
+    }
+    if (threadIdx.x == 0) {
+      a.offsets[0] = 0;
+      *a.n_free_out = n_free - (int)all_taken;
+      *a.refused = (int)all_refused;
+    }
+  }
+  for (int64_t row = (int64_t)cta * blockDim.x + threadIdx.x; row < a.rows; row += (int64_t)ncta * blockDim.x) {
+    int slot = -1, pos = -1;
+    if (row < off[a.n]) {
+      int lo = 0, hi = a.n - 1;  // the first request that ends behind the row
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid + 1] > row) hi = mid;
+        else lo = mid + 1;
+      }
+      if (first[lo] >= 0) {
+        pos = ctx[lo] + (int)row - off[lo];
+        const int held = (int)(((int64_t)ctx[lo] + a.page - 1) / a.page), i = pos / a.page;
+        int *entry = a.tables + (int64_t)lo * a.width + i;
+        int id;
+        if (i < held) {
+          id = *entry;
+        } else {
+          id = a.stack[n_free - 1 - (first[lo] + i - held)];
+          if (pos % a.page == 0) *entry = id;  // a new page's first token is one of the new rows
+        }
+        const int64_t s = (int64_t)id * a.page + pos % a.page;
+        slot = id >= 0 && s <= INT_MAX ? (int)s : -1;
+      }
+    }
+    a.slots[row] = slot;
+    a.positions[row] = pos;
+  }
+}
+
+// Returns the pages of `requests` to the stack, in the order given (a request
+// named twice counts once), and sets their lengths to 0.
+__global__ void __launch_bounds__(kPagesThreads)
+    pages_release_kernel(const int *requests, int n, int n_seqs, int page, int *lens, const int *tables, int width,
+                         int *stack, int capacity, int *n_free) {
+  __shared__ int64_t warp_sums[kPagesThreads / 32];
+  __shared__ int s_first[kPagesThreads + 1], s_req[kPagesThreads];
+  int64_t top = min(max(*n_free, 0), capacity);
+  __syncthreads();
+  for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x;
+    int r = i < n ? requests[i] : -1;
+    if (r < 0 || r >= n_seqs) r = -1;
+    s_req[threadIdx.x] = r;
+    __syncthreads();
+    for (int j = 0; j < (int)threadIdx.x && r >= 0; ++j)
+      if (s_req[j] == r) r = -1;  // of earlier chunks' requests the lengths are 0 already
+    const int64_t len = r >= 0 ? min((int64_t)max(lens[r], 0), (int64_t)width * page) : 0;
+    const int pages = (int)((len + page - 1) / page);
+    int64_t sum;
+    const int64_t upto = block_scan(pages, warp_sums, sum);
+    s_first[threadIdx.x + 1] = (int)min(upto, (int64_t)INT_MAX);
+    s_req[threadIdx.x] = r;
+    if (threadIdx.x == 0) s_first[0] = 0;
+    __syncthreads();
+    const int64_t fit = min(sum, (int64_t)capacity - top);  // a full stack keeps its size: lengths were not the tables'
+    for (int64_t p = threadIdx.x; p < fit; p += blockDim.x) {
+      int lo = 0, hi = (int)blockDim.x - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid + 1] > p) hi = mid;
+        else lo = mid + 1;
+      }
+      stack[top + p] = tables[(int64_t)s_req[lo] * width + (p - s_first[lo])];
+    }
+    if (r >= 0) lens[r] = 0;
+    top += fit;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *n_free = (int)top;
+}
+
+}  // namespace mq
