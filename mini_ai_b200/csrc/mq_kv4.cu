@@ -5,6 +5,7 @@
 // cache: all of them may be captured in a CUDA graph, and what a call needs
 // beside its arguments is the caller's workspace, so graphs share nothing.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <new>
 
@@ -87,6 +88,49 @@ int launched(const char *what) {
   return MQ_OK;
 }
 
+// Launched behind the previous kernel of the stream with programmatic
+// serialization: it may start early and waits where it depends on that one.
+template <typename... KArgs, typename... Args>
+int launch_after(const char *what, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                 const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  count_launch();
+  return MQ_OK;
+}
+
+int dec_grid(int sms) { return 3 * sms; }
+
+size_t attention_bytes(int hd, int sms) {
+  return (size_t)dec_grid(sms) * 2 * (sizeof(int4) + sizeof(float) * kv4_part_floats(kDecRowTile, hd));
+}
+
+template <int NB>
+int launch_decode(const Kv4AttnArgs &a, int device, int sms, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};  // devices whose kernel may use this much shared memory
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    MQ_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 DecSmem<NB>::kBytes));
+    if (device < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (int rc = launch_after("cache attention", kv4_decode_kernel<NB>, dim3(dec_grid(sms)), kDecWarps * 32,
+                            DecSmem<NB>::kBytes, s, a))
+    return rc;
+  return launch_after("join attention parts", kv4_join_kernel, dim3(dec_grid(sms), kDecRowTile), 32 * NB, 0, s, a,
+                      kDecRowTile);
+}
+
 }  // namespace
 
 extern "C" {
@@ -135,6 +179,7 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   c->v = v;
   c->bytes = bytes;
   c->owned = memory ? nullptr : base;
+  cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, device);
   *out = c;
   return MQ_OK;
 }
@@ -207,7 +252,7 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
 
 size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new) {
   (void)heads, (void)max_new;
-  return c ? 16 : 0;
+  return c ? attention_bytes(c->v.hd, c->sms) : 0;
 }
 
 int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
@@ -233,10 +278,25 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Kv4AttnArgs a{c->v, layer, q, ld_q, hs_q, out, ld_out, hs_out, offsets, seq_lens, block_tables,
-                      n_seqs, max_pages, rows, heads, scale};
-  kv4_attention_kernel<<<dim3(rows, heads), 32, 0, s>>>(a);
-  return launched("cache attention");
+  Kv4AttnArgs a{};
+  a.c = c->v;
+  a.layer = layer;
+  a.q = q, a.ld_q = ld_q, a.hs_q = hs_q;
+  a.out = out, a.ld_o = ld_out, a.hs_o = hs_out;
+  a.offsets = offsets, a.lens = seq_lens, a.tables = block_tables;
+  a.n = n_seqs, a.width = max_pages, a.rows = rows, a.group = heads / c->v.kv;
+  a.min_rows = 1, a.max_rows = INT_MAX;
+  a.scale = scale * 1.44269504088896341f;
+  a.meta = static_cast<int4 *>(workspace);
+  a.parts = reinterpret_cast<float *>(a.meta + 2 * dec_grid(c->sms));
+  a.vec_q = vector16(q, ld_q, hs_q);
+  a.vec_o = vector16(out, ld_out, hs_out);
+  switch (c->v.nb) {
+  case 1: return launch_decode<1>(a, c->device, c->sms, s);
+  case 2: return launch_decode<2>(a, c->device, c->sms, s);
+  case 3: return launch_decode<3>(a, c->device, c->sms, s);
+  default: return launch_decode<4>(a, c->device, c->sms, s);
+  }
 }
 
 int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_seqs, int page_size, int *block_tables,

@@ -189,5 +189,6 @@ struct mq_kv4 {
   int device = 0;
   mq::Kv4View v{};
   size_t bytes = 0;
+  int sms = 0;
   void *owned = nullptr;  // the allocation, where the caller gave no memory
 };

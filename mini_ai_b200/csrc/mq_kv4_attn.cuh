@@ -1,12 +1,26 @@
-// Causal attention of a ragged batch's query rows over the paged 4-bit cache.
+// Causal attention of a ragged batch's query rows over the paged 4-bit cache:
+// the work's division over CTAs, and the kernel for few rows a request.
 //
 // Row i of request r (new_r rows, len_r cached tokens, its own among them)
 // stands at position len_r - new_r + i and sees the tokens 0..position:
 //   out = sum_s p_s v_s / sum_s p_s, p_s = exp(scale q . k_s - max).
-// A row that sees nothing is 0.
+// A row that sees nothing is 0. The G = heads / kv query heads that share a KV
+// head are rows of one matrix: "flat row" f = i G + g of (request, KV head).
+//
+// Division (stream-K). An item is a tile of RT flat rows of one (request, KV
+// head); its work is the number of BN-token tiles that its last row sees. All
+// items in order (request, KV head, row tile) form one line of work, cut into
+// equal pieces, one a CTA, whatever the lengths. A CTA thus has at most one
+// item that began in an earlier CTA and one that it leaves unfinished; the
+// partial results of those (reference, sum and unscaled output per row) go to
+// its two workspace slots, and a second kernel joins them in order. The
+// kernels read all lengths from device memory, so that a captured launch
+// serves any batch.
 #pragma once
 
 #include "mq_kv4.cuh"
+#include "mq_pages.cuh"
+#include "mq_sm100.cuh"
 
 namespace mq {
 
@@ -18,49 +32,600 @@ struct Kv4AttnArgs {
   float *out;
   int64_t ld_o, hs_o;
   const int *offsets, *lens, *tables;
-  int n, width, rows, heads;
-  float scale;
+  int n, width, rows, group;
+  int min_rows, max_rows;  // requests of min_rows..max_rows flat rows are this kernel's
+  float scale;             // times log2(e): the softmax is in powers of two
+  float *parts;            // [grid][2] partial items
+  int4 *meta;              // [grid][2]: the item that a CTA leaves unfinished
+  bool vec_q, vec_o;
 };
 
-// One warp per (row, head): lanes along the elements of a block.
-__global__ void __launch_bounds__(32) kv4_attention_kernel(const Kv4AttnArgs a) {
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, nb = a.c.nb;
-  int lo = 0, hi = a.n;
+// ------------------------------------------------------------ division of the work
+struct Kv4Request {
+  int row0;      // first row in q and out
+  int flat;      // flat rows
+  int base;      // position of the first row (negative: it sees nothing)
+  int len;       // cached tokens
+  int tiles;     // row tiles
+  int64_t work;  // of one KV head
+};
+
+// sum of floor((a i + b) / m) for i in [0, n); a, b >= 0, m > 0 (the Euclid-like recursion).
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t s = 0;
+  for (;;) {
+    s += (n - 1) * n / 2 * (a / m) + n * (b / m);
+    a %= m, b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) return s;
+    n = y / m, b = y % m;
+    const int64_t t = m;
+    m = a, a = t;
+  }
+}
+
+// Work of the first `tiles` row tiles: tile i costs floor((base G + RT (i + 1) - 1) / (G BN)) + 1,
+// the BN-token tiles up to its last row (a tile cut short by the request's end may see fewer).
+template <int RT, int BN>
+__device__ __forceinline__ int64_t kv4_work(int base, int group, int tiles) {
+  const int64_t b = (int64_t)max(base, 0) * group + RT - 1, m = (int64_t)group * BN;
+  if (tiles == 1) return b / m + 1;
+  return tiles ? floor_sum(tiles, m, RT, b) + tiles : 0;
+}
+
+template <int RT, int BN>
+__device__ __forceinline__ Kv4Request kv4_request(const Kv4AttnArgs &a, int r) {
+  Kv4Request q;
+  const int first = __ldg(a.offsets + r), end = __ldg(a.offsets + r + 1);
+  const int64_t fresh = (int64_t)end - first;
+  q.row0 = first;
+  q.len = (int)min((int64_t)max(__ldg(a.lens + r), 0), (int64_t)a.width * a.c.page);
+  q.base = (int)max((int64_t)q.len - fresh, (int64_t)INT_MIN);
+  const int n = first >= 0 ? max(min(end, a.rows) - first, 0) : 0;
+  q.flat = n * a.group;
+  if (q.flat < a.min_rows || q.flat > a.max_rows) q.flat = 0;
+  q.tiles = (q.flat + RT - 1) / RT;
+  q.work = kv4_work<RT, BN>(q.base, a.group, q.tiles);
+  return q;
+}
+
+// A walk along this CTA's piece of the line.
+struct Kv4Walk {
+  int r;               // request at the current place
+  int64_t at;          // place within it
+  int64_t left;        // work left to this CTA
+  int64_t line, place;  // the whole line, and the current place on it
+  int ctas;            // pieces
+};
+
+// All threads; two block-wide scans. false: no work for this CTA.
+template <int RT, int BN>
+__device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
+  __shared__ int64_t sums[32], s_at;
+  __shared__ int s_r;
+  const int per = (a.n + blockDim.x - 1) / blockDim.x;
+  const int r0 = threadIdx.x * per, r1 = min(r0 + per, a.n);
+  int64_t mine = 0;
+  for (int r = r0; r < r1; ++r) mine += a.c.kv * kv4_request<RT, BN>(a, r).work;
+  const int64_t upto = block_scan(mine, sums, w.line);
+  if (w.line == 0) return false;
+  w.ctas = (int)min((int64_t)gridDim.x, w.line);
+  if ((int)blockIdx.x >= w.ctas) return false;
+  w.place = blockIdx.x * w.line / w.ctas;
+  w.left = (blockIdx.x + 1) * w.line / w.ctas - w.place;
+  if (w.place >= upto - mine && w.place < upto) {
+    int64_t at = w.place - (upto - mine);
+    int r = r0;
+    for (;; ++r) {
+      const int64_t here = a.c.kv * kv4_request<RT, BN>(a, r).work;
+      if (at < here) break;
+      at -= here;
+    }
+    s_r = r, s_at = at;
+  }
+  __syncthreads();
+  w.r = s_r, w.at = s_at;
+  return true;
+}
+
+struct Kv4Segment {
+  Kv4Request q;
+  int r, head, tile;  // request, KV head, row tile
+  int t0, t1;         // BN-token tiles of this CTA
+  int whole;          // of the item
+};
+
+// The next item's part of this CTA; advances the walk. false: done.
+template <int RT, int BN>
+__device__ __forceinline__ bool kv4_next(const Kv4AttnArgs &a, Kv4Walk &w, Kv4Segment &s) {
+  if (w.left == 0) return false;
+  for (;; ++w.r) {
+    s.q = kv4_request<RT, BN>(a, w.r);
+    if (w.at < a.c.kv * s.q.work) break;
+    w.at -= a.c.kv * s.q.work;
+  }
+  s.r = w.r;
+  s.head = (int)(w.at / s.q.work);
+  const int64_t in_head = w.at % s.q.work;
+  int lo = 0, hi = s.q.tiles - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (a.offsets[mid + 1] > row) hi = mid;
+    if (kv4_work<RT, BN>(s.q.base, a.group, mid + 1) > in_head) hi = mid;
     else lo = mid + 1;
   }
-  if (lo >= a.n || row < a.offsets[lo]) return;
-  const int len = (int)min((int64_t)max(a.lens[lo], 0), (int64_t)a.width * a.c.page);
-  const int last = min(len - (a.offsets[lo + 1] - a.offsets[lo]) + row - a.offsets[lo], len - 1);
-  const int kh = h / (a.heads / a.c.kv);
-  float q[4], acc[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-  for (int j = 0; j < nb; ++j) q[j] = a.q[row * a.ld_q + h * a.hs_q + 32 * j + lane];
-  for (int s = 0; s <= last; ++s) {
-    const int id = a.tables[(int64_t)lo * a.width + s / a.c.page];
-    if (id < 0 || id >= a.c.pages) continue;
-    const int in_page = s % a.c.page, tok = in_page % kKv4Unit;
-    const uint8_t *u = kv4_unit(a.c, a.layer, id, kh, in_page / kKv4Unit);
-    float dot = 0.0f, v[4];
-    for (int j = 0; j < nb; ++j) {
-      const uint32_t kw = *reinterpret_cast<const uint32_t *>(u + tok * 16 * nb + (lane >> 3) * 4 * nb + 4 * j);
-      const uint16_t vw =
-          *reinterpret_cast<const uint16_t *>(u + kv4_v_off(nb) + tok * 16 * nb + (lane >> 2) * 2 * nb + 2 * j);
-      const float dk = __half2float(*reinterpret_cast<const __half *>(u + kv4_k_scale_off(nb) + 2 * (tok * nb + j)));
-      const float dv = __half2float(*reinterpret_cast<const __half *>(u + kv4_v_scale_off(nb) + 2 * (tok * nb + j)));
-      dot += q[j] * (dk * (float)((int)((kw >> (4 * (lane & 7))) & 15u) - 8));
-      v[j] = dv * (float)((int)((vw >> (4 * (lane & 3))) & 15u) - 8);
-    }
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    dot *= a.scale;
-    const float m2 = fmaxf(m, dot), shift = m2 == -INFINITY ? 0.0f : m2;
-    const float old = expf(m - shift), p = expf(dot - shift);
-    l = l * old + p;
-    for (int j = 0; j < nb; ++j) acc[j] = acc[j] * old + p * v[j];
-    m = m2;
+  s.tile = lo;
+  const int64_t before = kv4_work<RT, BN>(s.q.base, a.group, lo);
+  s.whole = (int)(kv4_work<RT, BN>(s.q.base, a.group, lo + 1) - before);
+  s.t0 = (int)(in_head - before);
+  s.t1 = (int)min((int64_t)s.whole, s.t0 + w.left);
+  const int n = s.t1 - s.t0;
+  w.at += n, w.left -= n, w.place += n;
+  return true;
+}
+
+// The CTAs from this one on that an item which ends at place `end` is spread over.
+__device__ __forceinline__ int kv4_spread(const Kv4Walk &w, int64_t end) {
+  return (int)((end * w.ctas - 1) / w.line) - (int)blockIdx.x + 1;
+}
+
+// ------------------------------------------------------------ fragments
+__device__ __forceinline__ float ex2(float x) {  // 2^x, off by at most 2^-22 of it
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<const __half2 *>(&u); }
+
+// (x, y) as fp16 hi + lo pairs: 22 bits of each.
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_bits(h);
+  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// D = A B + D: A 16 x 16 row-major, B 16 x 8 column-major, fp16; D fp32.
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 2 nibbles of each half-word as codes c = q - 8: 1024 + q and 64 + q are fp16
+// numbers that hold q in their low and in their next four bits.
+__device__ __forceinline__ __half2 code_lo(uint32_t x) {
+  return __hsub2(bits_h2((x & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f));
+}
+__device__ __forceinline__ __half2 code_hi(uint32_t x) {
+  return __hsub2(bits_h2((x & 0x00F000F0u) | 0x54005400u), __float2half2_rn(72.0f));
+}
+
+// N consecutive half-words of shared memory (aligned to the whole where N is even).
+template <int N>
+__device__ __forceinline__ void lds_halves(const uint8_t *p, uint32_t (&w)[(N + 1) / 2]) {
+  if constexpr (N == 4) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else if constexpr (N == 2) {
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
+  } else {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+    w[0] = h[0];
+    if constexpr (N == 3) w[0] |= (uint32_t)h[1] << 16, w[1] = h[2];
   }
-  for (int j = 0; j < nb; ++j) a.out[row * a.ld_o + h * a.hs_o + 32 * j + lane] = l == 0.0f ? 0.0f : acc[j] / l;
+}
+
+// Half-word j of a and of b side by side.
+template <int W>
+__device__ __forceinline__ uint32_t pair_halves(const uint32_t (&a)[W], const uint32_t (&b)[W], int j) {
+  return __byte_perm(a[j >> 1], b[j >> 1], j & 1 ? 0x7632 : 0x5410);
+}
+template <int W>
+__device__ __forceinline__ float half_at(const uint32_t (&a)[W], int j) {
+  return __half2float(__ushort_as_half((uint16_t)(a[j >> 1] >> (j & 1 ? 16 : 0))));
+}
+
+// ------------------------------------------------------------ few rows
+// One CTA, 4 warps, 8 flat rows an item. Every warp streams its own 16-token
+// units through a ring of bulk copies in shared memory, without a barrier to
+// the other warps, and keeps a softmax of its own; the four are joined at the
+// item's end.
+//
+// m16n8k16 products with the query side as A: its 16 rows are the 8 rows' hi
+// parts and their lo parts, so that both halves of a score land in one
+// thread's accumulators. The weights of a score fragment are, in place, the A
+// fragment of the product with V, again as hi and lo rows.
+//   Scores: K codes are fed as the integers q = c + 8 in fp16's subnormals
+//   (nibble i of a half-word: one AND; odd nibbles count 16-fold, and the query
+//   elements that meet them are divided by 16), starting the accumulator at
+//   -8 sum(query), and the block's scale is applied to its 32-element sum.
+//   Output: V is c d, exact in fp16.
+// Tokens of a unit are taken in the order that keeps shared memory free of
+// bank conflicts: column n of score tile i is token (n >> 1) + 4 (n & 1) + 8 i.
+//
+// Bound: the cache's bytes, 1152 a token of 8 heads of 128, against ~300 issue
+// slots a unit and warp for decoding and weights.
+constexpr int kDecWarps = 4;
+constexpr int kDecRowTile = 8;
+constexpr int kDecUnits = 2;   // per warp and step
+constexpr int kDecTokens = kDecWarps * kDecUnits * kKv4Unit;  // BN
+constexpr int kDecStages = 3;
+constexpr uint64_t kKv4WaitNs = 1000000000ull;
+
+template <int NB>
+struct DecSmem {
+  static constexpr int kUnit = kv4_unit_bytes(NB);
+  static constexpr int kRing = kDecStages * kDecUnits * kUnit;  // of a warp
+  static constexpr int kRowStride = 32 * NB + 4;                // floats; rows 4 banks apart
+  static constexpr int kBars = kDecWarps * kRing;
+  static constexpr int kBytes = kBars + kDecWarps * kDecStages * 8;
+  static_assert((kDecRowTile * (kRowStride + 2)) * 4 <= kRing, "a warp's result fits its ring");
+};
+
+__host__ __device__ constexpr int kv4_part_floats(int row_tile, int hd) { return row_tile * (hd + 2); }
+
+template <int NB>
+__global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4AttnArgs a) {
+  using L = DecSmem<NB>;
+  constexpr int HD = 32 * NB, W = (NB + 1) / 2;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t *ring = sm + warp * L::kRing;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::kBars) + warp * kDecStages;
+  if (lane == 0) {
+    for (int s = 0; s < kDecStages; ++s) sm100::mbar_init(&bars[s], 1);
+    sm100::fence_mbar_init();
+  }
+  sm100::griddep_wait();
+  sm100::griddep_launch_dependents();
+  if (threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
+  Kv4Walk walk;
+  if (!kv4_walk<kDecRowTile, kDecTokens>(a, walk)) return;
+  __syncwarp();
+
+  const int upp = a.c.page / kKv4Unit;  // units of a page
+  const int64_t unit_page = a.c.page_head_bytes * a.c.kv;
+  uint32_t steps_done = 0;  // of this warp, over all segments: the ring's place
+  Kv4Segment s;
+  while (kv4_next<kDecRowTile, kDecTokens>(a, walk, s)) {
+    // This thread's row of the tile: flat row f, and the last token that it sees.
+    const int f = s.tile * kDecRowTile + g;
+    const bool real = f < s.q.flat;
+    const int qi = f / a.group;
+    const int last = min(s.q.base + qi, s.q.len - 1);
+    const int last_min = min(s.q.base + s.tile * kDecRowTile / a.group, s.q.len - 1);
+    const int last_max = min(s.q.base + (min((s.tile + 1) * kDecRowTile, s.q.flat) - 1) / a.group, s.q.len - 1);
+    const int first_unit = s.t0 * (kDecTokens / kKv4Unit);
+    const int end_unit = min(s.t1 * (kDecTokens / kKv4Unit), (last_max + kKv4Unit) / kKv4Unit);
+    const int steps = max(0, (end_unit - first_unit + kDecWarps * kDecUnits - 1) / (kDecWarps * kDecUnits));
+    const int *table = a.tables + (int64_t)s.r * a.width;
+    const uint8_t *slice = kv4_unit(a.c, a.layer, 0, s.head, 0);
+
+    // Queries as A fragments, scaled so that the row's largest element is in [2^14, 2^15).
+    uint32_t qa[2 * NB][4];
+    float init[NB];
+    float fscale;
+    {
+      float x[NB][8];
+      float mx = 0.0f;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        if (real) {
+          const float *p = a.q + (s.q.row0 + qi) * a.ld_q + (s.head * a.group + f % a.group) * a.hs_q + 32 * j + 8 * t;
+          if (a.vec_q) {
+            const float4 u = *reinterpret_cast<const float4 *>(p), v = *reinterpret_cast<const float4 *>(p + 4);
+            x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
+            x[j][4] = v.x, x[j][5] = v.y, x[j][6] = v.z, x[j][7] = v.w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] = p[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[j][i])), bad |= !isfinite(x[j][i]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      bad = __shfl_xor_sync(0xffffffffu, (int)bad, 1) | bad;
+      bad = __shfl_xor_sync(0xffffffffu, (int)bad, 2) | bad;
+      const int e = min(141 - (int)(__float_as_uint(mx) >> 23), 126);  // 2^e mx in [2^14, 2^15)
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+      // The codes in the subnormals are 2^-24 of their values.
+      fscale = bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale, 24 - e);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {  // elements (2p, 2p + 4) and, 16-fold in the codes, (2p + 1, 2p + 5)
+          uint32_t *A = qa[2 * j + p];
+          split_f16(x[j][2 * p] * up, x[j][2 * p + 4] * up, A[0], A[1]);
+          split_f16(x[j][2 * p + 1] * (up * 0.0625f), x[j][2 * p + 5] * (up * 0.0625f), A[2], A[3]);
+          const float2 h0 = __half22float2(bits_h2(A[0])), l0 = __half22float2(bits_h2(A[1]));
+          const float2 h1 = __half22float2(bits_h2(A[2])), l1 = __half22float2(bits_h2(A[3]));
+          sum += (h0.x + l0.x) + (h0.y + l0.y) + 16.0f * ((h1.x + l1.x) + (h1.y + l1.y));
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        init[j] = sum * (-8.0f / 16777216.0f);
+      }
+    }
+
+    float o[4 * NB][4];
+    float ref, sum;       // weights are 2^(score - ref): at most 2^15; their sum over this thread's tokens
+    uint32_t poison = 0;  // blocks of this row with a NaN value that it sees
+    // A row that does not see a token weighs it 0, which a NaN value would not
+    // respect: a segment whose output has a NaN is done again with such values
+    // set to 0 and the rows that see them marked.
+    for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+      for (int i = 0; i < 4 * NB; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
+      ref = -INFINITY, sum = 0.0f;
+
+      // The ring: step k of this warp is units first_unit + (k * 4 + warp) * 2 + {0, 1}.
+      int ids = -1;        // page ids of 16 steps' units, one a lane
+      uint32_t held = 0;   // two bits a stage: units that were fetched
+      auto fetch = [&](int k) {
+        const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
+        if ((k & 15) == 0) {
+          const int u = first_unit + ((k + (lane >> 1)) * kDecWarps + warp) * kDecUnits + (lane & 1);
+          ids = u < end_unit ? __ldg(table + u / upp) : -1;
+          if (ids >= a.c.pages) ids = -1;
+        }
+        const uint32_t stage = (steps_done + k) % kDecStages;
+        uint32_t have = 0;
+        int id[kDecUnits];
+#pragma unroll
+        for (int j = 0; j < kDecUnits; ++j) {
+          id[j] = __shfl_sync(0xffffffffu, ids, (k & 15) * 2 + j);
+          have |= (id[j] >= 0 ? 1u : 0u) << j;
+        }
+        held = (held & ~(3u << (2 * stage))) | have << (2 * stage);
+        if (lane == 0) {
+          sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit);
+#pragma unroll
+          for (int j = 0; j < kDecUnits; ++j)
+            if (id[j] >= 0)
+              sm100::bulk_load(ring + (stage * kDecUnits + j) * L::kUnit,
+                               slice + id[j] * unit_page + (int64_t)((u0 + j) % upp) * L::kUnit, L::kUnit,
+                               &bars[stage]);
+        }
+      };
+      for (int k = 0; k < min(kDecStages - 1, steps); ++k) fetch(k);
+
+      for (int k = 0; k < steps; ++k) {
+        if (k + kDecStages - 1 < steps) fetch(k + kDecStages - 1);
+        const uint32_t stage = (steps_done + k) % kDecStages;
+        if (!sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, nullptr, nullptr, kKv4WaitNs))
+          sum = __uint_as_float(0x7fc00000u);
+        const uint32_t have = (held >> (2 * stage)) & 3u;
+        const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
+        const uint8_t *buf = ring + stage * kDecUnits * L::kUnit;
+
+        // ---- scores: sc[unit][tile i][b] of token t + 4 b + 8 i
+        float sc[kDecUnits][2][2];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kDecUnits; ++j) {
+          const uint8_t *unit = buf + j * L::kUnit;
+          if (!(have >> j & 1u)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[j][i >> 1][i & 1] = -INFINITY;
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t kw[NB];
+            const uint8_t *kp = unit + ((g >> 1) + 4 * (g & 1) + 8 * i) * (16 * NB) + t * (4 * NB);
+            if constexpr (NB == 4) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(kp);
+              kw[0] = v.x, kw[1] = v.y, kw[2] = v.z, kw[3] = v.w;
+            } else if constexpr (NB == 2) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+              kw[0] = v.x, kw[1] = v.y;
+            } else {
+#pragma unroll
+              for (int b = 0; b < NB; ++b) kw[b] = reinterpret_cast<const uint32_t *>(kp)[b];
+            }
+            uint32_t d0[W], d1[W];
+            lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 8 * i) * (2 * NB), d0);
+            lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 4 + 8 * i) * (2 * NB), d1);
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              float c[4] = {init[b], init[b], 0.0f, 0.0f};
+              const uint32_t w = kw[b], w8 = w >> 8;
+              mma16816(c, qa[2 * b], w & 0x000F000Fu, w & 0x00F000F0u);
+              mma16816(c, qa[2 * b + 1], w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+              s0 = fmaf(half_at(d0, b), c[0] + c[2], s0);
+              s1 = fmaf(half_at(d1, b), c[1] + c[3], s1);
+            }
+            sc[j][i][0] = s0 * fscale, sc[j][i][1] = s1 * fscale;
+          }
+          if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_min) {  // some row's end
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((u0 + j) * kKv4Unit + t + 4 * (i & 1) + 8 * (i >> 1) > last) sc[j][i >> 1][i & 1] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[j][i >> 1][i & 1]);
+        }
+
+        // ---- the weights' reference: moved only when a weight would pass 2^15
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool grow = mx > ref + 15.0f || (ref == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float to = grow ? mx - 8.0f : ref;
+          const float old = grow ? ex2(ref - to) : 1.0f;
+          ref = to;
+          sum *= old;
+#pragma unroll
+          for (int i = 0; i < 4 * NB; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[i][c] *= old;
+        }
+        const float shift = ref == -INFINITY ? 0.0f : ref;
+
+        // ---- weights and output
+#pragma unroll
+        for (int j = 0; j < kDecUnits; ++j) {
+          if (!(have >> j & 1u)) continue;
+          const uint8_t *unit = buf + j * L::kUnit;
+          float p[4];  // tokens t, t + 4, t + 8, t + 12
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = ex2(sc[j][i >> 1][i & 1] - shift), sum += p[i];
+          uint32_t pa[4];
+          split_f16(p[0], p[1], pa[0], pa[1]);
+          split_f16(p[2], p[3], pa[2], pa[3]);
+          uint32_t vw[4][W], vd[4][W];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = t + 4 * i;
+            lds_halves<NB>(unit + kv4_v_off(NB) + tok * (16 * NB) + g * (2 * NB), vw[i]);
+            lds_halves<NB>(unit + kv4_v_scale_off(NB) + tok * (2 * NB), vd[i]);
+          }
+          const int tok0 = (u0 + j) * kKv4Unit + t;
+          if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_max) {  // tokens that no row sees may hold anything
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tok0 + 4 * i > last_max)
+#pragma unroll
+                for (int w = 0; w < W; ++w) vd[i][w] = 0u;
+          }
+          if (careful) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                const int sh = b & 1 ? 16 : 0;
+                if ((vd[i][b >> 1] >> sh & 0x7fffu) > 0x7c00u) {
+                  if (tok0 + 4 * i <= last) poison |= 1u << b;
+                  vd[i][b >> 1] &= ~(0xffffu << sh);
+                }
+              }
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint32_t x0 = pair_halves(vw[0], vw[1], b), x1 = pair_halves(vw[2], vw[3], b);
+            const __half2 e0 = bits_h2(pair_halves(vd[0], vd[1], b)), e1 = bits_h2(pair_halves(vd[2], vd[3], b));
+            const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+            mma16816(o[4 * b], pa, h2_bits(__hmul2(code_lo(x0), e0)), h2_bits(__hmul2(code_lo(x1), e1)));
+            mma16816(o[4 * b + 1], pa, h2_bits(__hmul2(code_hi(x0), e0)), h2_bits(__hmul2(code_hi(x1), e1)));
+            mma16816(o[4 * b + 2], pa, h2_bits(__hmul2(code_lo(y0), e0)), h2_bits(__hmul2(code_lo(y1), e1)));
+            mma16816(o[4 * b + 3], pa, h2_bits(__hmul2(code_hi(y0), e0)), h2_bits(__hmul2(code_hi(y1), e1)));
+          }
+        }
+        __syncwarp();  // the stage's readers are done before lane 0 refills it
+      }
+      steps_done += steps;
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < 4 * NB; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) nan |= isnan(o[i][c]);
+      if (!__any_sync(0xffffffffu, nan)) break;
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    poison |= __shfl_xor_sync(0xffffffffu, poison, 1);
+    poison |= __shfl_xor_sync(0xffffffffu, poison, 2);
+
+    // ---- join the warps through their rings
+    float *mine = reinterpret_cast<float *>(ring);
+    if (t == 0) {
+      mine[kDecRowTile * L::kRowStride + g] = ref;
+      mine[kDecRowTile * L::kRowStride + kDecRowTile + g] = sum;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {  // n8-tile i of block b, column n is element 32 b + 4 n + i
+      float4 lo = make_float4(o[4 * b][0] + o[4 * b][2], o[4 * b + 1][0] + o[4 * b + 1][2],
+                              o[4 * b + 2][0] + o[4 * b + 2][2], o[4 * b + 3][0] + o[4 * b + 3][2]);
+      float4 hi = make_float4(o[4 * b][1] + o[4 * b][3], o[4 * b + 1][1] + o[4 * b + 1][3],
+                              o[4 * b + 2][1] + o[4 * b + 2][3], o[4 * b + 3][1] + o[4 * b + 3][3]);
+      if (poison >> b & 1u) {
+        const float x = __uint_as_float(0x7fc00000u);
+        lo = hi = make_float4(x, x, x, x);
+      }
+      float4 *dst = reinterpret_cast<float4 *>(mine + g * L::kRowStride + 32 * b + 8 * t);
+      dst[0] = lo, dst[1] = hi;
+    }
+    __syncthreads();
+    const bool whole = s.t0 == 0 && s.t1 == s.whole;
+    float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kDecRowTile, HD);
+    for (int i = threadIdx.x; i < kDecRowTile * HD / 4; i += kDecWarps * 32) {
+      const int row = i / (HD / 4), e = 4 * (i % (HD / 4)), fr = s.tile * kDecRowTile + row;
+      if (fr >= s.q.flat) continue;
+      float rw[kDecWarps], top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        rw[w] = reinterpret_cast<const float *>(sm + w * L::kRing)[kDecRowTile * L::kRowStride + row];
+        top = fmaxf(top, rw[w]);
+      }
+      const float shift = top == -INFINITY ? 0.0f : top;
+      float total = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float *src = reinterpret_cast<const float *>(sm + w * L::kRing);
+        const float k = ex2(rw[w] - shift);
+        const float4 v = *reinterpret_cast<const float4 *>(src + row * L::kRowStride + e);
+        total += k * src[kDecRowTile * L::kRowStride + kDecRowTile + row];
+        acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+      }
+      if (whole) {
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+        float *dst = a.out + (int64_t)(s.q.row0 + fr / a.group) * a.ld_o +
+                     (int64_t)(s.head * a.group + fr % a.group) * a.hs_o + e;
+        if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
+        else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
+      } else {
+        *reinterpret_cast<float4 *>(part + 2 * kDecRowTile + row * HD + e) = acc;
+        if (e == 0) part[row] = top, part[kDecRowTile + row] = total;
+      }
+    }
+    if (threadIdx.x == 0 && s.t0 == 0 && !whole) {  // the item goes on in the next CTAs
+      a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
+      a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
+    }
+    __syncthreads();
+    sm100::fence_proxy_async_smem();  // the rings' next writers are bulk copies
+  }
+}
+
+// Joins the parts of the items that their first CTA left unfinished. Block
+// (CTA, row of the tile), one thread an element; the parts in order.
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int row_tile) {
+  sm100::griddep_wait();
+  const int b = blockIdx.x, row = blockIdx.y, hd = a.c.hd, e = threadIdx.x;
+  const int parts = a.meta[2 * b + 1].x;
+  if (parts == 0) return;
+  const int4 m = a.meta[2 * b];
+  const int fr = m.y * row_tile + row;
+  if (fr >= m.w) return;
+  const int64_t stride = kv4_part_floats(row_tile, hd);
+  auto part = [&](int i) { return a.parts + (2 * (int64_t)(b + i) + (i == 0)) * stride; };
+  float top = -INFINITY;
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, part(i)[row]);
+  const float shift = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, acc = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float *p = part(i);
+    const float k = ex2(p[row] - shift);
+    total += k * p[row_tile + row];
+    acc += k * p[2 * row_tile + (int64_t)row * hd + e];
+  }
+  a.out[(int64_t)(m.x + fr / a.group) * a.ld_o + (int64_t)(m.z * a.group + fr % a.group) * a.hs_o + e] =
+      total == 0.0f ? 0.0f : acc / total;
 }
 
 }  // namespace mq

@@ -4,8 +4,12 @@ Packing and tables are exact. Attention: with u = 2^-24, every score's error is 
     ds = scale * (2^-22 + 44 * 2^-23) * sum_e |q_e k_e|
 (q enters as fp16 hi + lo, off by 2^-22 of it; at most 44 additions in a row, a tensor core's truncating ones off by
 2^-23 each), exp2 and the weight's own hi + lo split add 2^-22 each, and the weighted sum and the sum of the weights
-at most 256 additions in a row. A weight off by a relative e moves an output by at most 2 e * sum p |v| / sum p, so
-    |d out| <= (2 * (max ds + 2^-21) + 256 * 2^-23) * sum p |v| / sum p.
+at most 256 additions in a row. A weight off by a relative e moves an output by at most 2 e * sum p |v| / sum p.
+Weights far below the largest lose that relative precision: the lo part of a pair is an fp16 number, off by at most
+2^-25 where it is subnormal, in units in which the largest weight is 2^8 or more (the reference is set 8 below a
+score that the row has, and later only raised with the scores). A weight is therefore off by at most 2^-33 of the
+largest weight p_max beside its relative error, and an output by at most 2^-33 * p_max * sum |v|. With sum p = 1:
+    |d out| <= (2 * (max ds + 2^-21) + 256 * 2^-23) * sum p |v| + 2^-33 * p_max * sum |v|.
 """
 from __future__ import annotations
 
@@ -91,6 +95,7 @@ def ref_attention(torch, q, k, v, news, lens, scale):
                 size = torch.einsum("hd,shd->hs", q[row + i].abs(), kk.abs()).amax(-1) * abs(scale)
                 rel = 2 * (size * (2 ** -22 + 44 * 2 ** -23) + 2 ** -21) + 256 * 2 ** -23
                 tol[row + i] = rel[:, None] * torch.einsum("hs,shd->hd", p, vv.abs())
+                tol[row + i] += 2 ** -33 * p.amax(-1)[:, None] * vv.abs().sum(0)
         row += m
     return out, tol
 
