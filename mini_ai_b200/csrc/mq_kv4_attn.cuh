@@ -237,10 +237,10 @@ __device__ __forceinline__ float half_at(const uint32_t (&a)[W], int j) {
 // parts and their lo parts, so that both halves of a score land in one
 // thread's accumulators. The weights of a score fragment are, in place, the A
 // fragment of the product with V, again as hi and lo rows.
-//   Scores: K codes are fed as the integers q = c + 8 in fp16's subnormals
-//   (nibble i of a half-word: one AND; odd nibbles count 16-fold, and the query
-//   elements that meet them are divided by 16), starting the accumulator at
-//   -8 sum(query), and the block's scale is applied to its 32-element sum.
+//   Scores: K enters as its codes c, and the block's scale is applied to its
+//   32-element sum. (Codes q = c + 8, one operation an element pair cheaper,
+//   with -8 sum(query) as the accumulator's start: the difference of large
+//   sums put outputs 3e-6 off.)
 //   Output: V is c d, exact in fp16.
 // Tokens of a unit are taken in the order that keeps shared memory free of
 // bank conflicts: column n of score tile i is token (n >> 1) + 4 (n & 1) + 8 i.
@@ -305,7 +305,6 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
 
     // Queries as A fragments, scaled so that the row's largest element is in [2^14, 2^15).
     uint32_t qa[2 * NB][4];
-    float init[NB];
     float fscale;
     {
       float x[NB][8];
@@ -336,24 +335,15 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       bad = __shfl_xor_sync(0xffffffffu, (int)bad, 2) | bad;
       const int e = min(141 - (int)(__float_as_uint(mx) >> 23), 126);  // 2^e mx in [2^14, 2^15)
       const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-      // The codes in the subnormals are 2^-24 of their values.
-      fscale = bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale, 24 - e);
+      fscale = bad ? __uint_as_float(0x7fc00000u) : ldexpf(a.scale, -e);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        float sum = 0.0f;
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {  // elements (2p, 2p + 4) and, 16-fold in the codes, (2p + 1, 2p + 5)
-          uint32_t *A = qa[2 * j + p];
+        for (int p = 0; p < 2; ++p) {  // the element pairs of nibbles 2p and 2p + 1
+          uint32_t(&A)[4] = qa[2 * j + p];
           split_f16(x[j][2 * p] * up, x[j][2 * p + 4] * up, A[0], A[1]);
-          split_f16(x[j][2 * p + 1] * (up * 0.0625f), x[j][2 * p + 5] * (up * 0.0625f), A[2], A[3]);
-          const float2 h0 = __half22float2(bits_h2(A[0])), l0 = __half22float2(bits_h2(A[1]));
-          const float2 h1 = __half22float2(bits_h2(A[2])), l1 = __half22float2(bits_h2(A[3]));
-          sum += (h0.x + l0.x) + (h0.y + l0.y) + 16.0f * ((h1.x + l1.x) + (h1.y + l1.y));
+          split_f16(x[j][2 * p + 1] * up, x[j][2 * p + 5] * up, A[2], A[3]);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        init[j] = sum * (-8.0f / 16777216.0f);
-      }
     }
 
     float o[4 * NB][4];
@@ -440,10 +430,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
             float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              float c[4] = {init[b], init[b], 0.0f, 0.0f};
+              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
               const uint32_t w = kw[b], w8 = w >> 8;
-              mma16816(c, qa[2 * b], w & 0x000F000Fu, w & 0x00F000F0u);
-              mma16816(c, qa[2 * b + 1], w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+              mma16816(c, qa[2 * b], h2_bits(code_lo(w)), h2_bits(code_hi(w)));
+              mma16816(c, qa[2 * b + 1], h2_bits(code_lo(w8)), h2_bits(code_hi(w8)));
               s0 = fmaf(half_at(d0, b), c[0] + c[2], s0);
               s1 = fmaf(half_at(d1, b), c[1] + c[3], s1);
             }
