@@ -11,6 +11,7 @@
 
 #include "mq_kv4.cuh"
 #include "mq_kv4_attn.cuh"
+#include "mq_kv4_prefill.cuh"
 #include "mq_pages.cuh"
 #include "mq_tcdec_api.h"
 
@@ -109,26 +110,56 @@ int launch_after(const char *what, void (*kernel)(KArgs...), dim3 grid, int thre
   return MQ_OK;
 }
 
-int dec_grid(int sms) { return 3 * sms; }
+// A kernel's workspace: its CTAs' notes on unfinished items, then the parts.
+size_t parts_bytes(int ctas, int row_tile, int hd) {
+  return (size_t)ctas * 2 * (sizeof(int4) + sizeof(float) * kv4_part_floats(row_tile, hd));
+}
+int dec_ctas(int sms) { return 3 * sms; }
 
-size_t attention_bytes(int hd, int sms) {
-  return (size_t)dec_grid(sms) * 2 * (sizeof(int4) + sizeof(float) * kv4_part_floats(kDecRowTile, hd));
+// Flat rows (rows of a request times the query heads of a KV head) up to which
+// the few-row kernel takes a request: it runs 8 of them at a time.
+constexpr int kFewRows = 24;
+bool many_rows(int group, int max_new) { return (int64_t)group * max_new > kFewRows; }
+
+void use_workspace(Kv4AttnArgs &a, uint8_t *ws, int ctas) {
+  a.meta = reinterpret_cast<int4 *>(ws);
+  a.parts = reinterpret_cast<float *>(ws + (size_t)ctas * 2 * sizeof(int4));
+}
+
+// Lets `kernel` use `bytes` of shared memory on `device`; once per device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t> &ready) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (ready.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 template <int NB>
-int launch_decode(const Kv4AttnArgs &a, int device, int sms, cudaStream_t s) {
-  static std::atomic<uint64_t> ready{0};  // devices whose kernel may use this much shared memory
-  const uint64_t bit = 1ull << (device & 63);
-  if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    MQ_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 DecSmem<NB>::kBytes));
-    if (device < 64) ready.fetch_or(bit, std::memory_order_relaxed);
-  }
-  if (int rc = launch_after("cache attention", kv4_decode_kernel<NB>, dim3(dec_grid(sms)), kDecWarps * 32,
+int run_attention(Kv4AttnArgs a, const mq_kv4 *c, uint8_t *ws, bool many, cudaStream_t s) {
+  static std::atomic<uint64_t> dec_ready{0}, pre_ready{0};
+  MQ_CUDA(allow_smem(kv4_decode_kernel<NB>, DecSmem<NB>::kBytes, c->device, dec_ready));
+  Kv4Join j{};
+  j.ctas[0] = dec_ctas(c->sms);
+  use_workspace(a, ws, j.ctas[0]);
+  a.min_rows = 1, a.max_rows = many ? kFewRows : INT_MAX;
+  j.meta[0] = a.meta, j.parts[0] = a.parts;
+  if (int rc = launch_after("cache attention", kv4_decode_kernel<NB>, dim3(j.ctas[0]), kDecWarps * 32,
                             DecSmem<NB>::kBytes, s, a))
     return rc;
-  return launch_after("join attention parts", kv4_join_kernel, dim3(dec_grid(sms), kDecRowTile), 32 * NB, 0, s, a,
-                      kDecRowTile);
+  if (many) {
+    MQ_CUDA(allow_smem(kv4_prefill_kernel<NB>, PreSmem<NB>::kAlloc, c->device, pre_ready));
+    j.ctas[1] = c->sms;
+    use_workspace(a, ws + parts_bytes(j.ctas[0], kDecRowTile, a.c.hd), j.ctas[1]);
+    a.min_rows = kFewRows + 1, a.max_rows = INT_MAX;
+    j.meta[1] = a.meta, j.parts[1] = a.parts;
+    if (int rc = launch_after("cache attention", kv4_prefill_kernel<NB>, dim3(j.ctas[1]), kPreThreads,
+                              PreSmem<NB>::kAlloc, s, a))
+      return rc;
+  }
+  return launch_after("join attention parts", kv4_join_kernel,
+                      dim3(j.ctas[0] + j.ctas[1] * (kPreRows / kJoinRows)), kJoinRows * 8 * NB, 0, s, a, j);
 }
 
 }  // namespace
@@ -251,8 +282,10 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
 }
 
 size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new) {
-  (void)heads, (void)max_new;
-  return c ? attention_bytes(c->v.hd, c->sms) : 0;
+  if (!c || heads < 1) return 0;
+  size_t n = parts_bytes(dec_ctas(c->sms), kDecRowTile, c->v.hd);
+  if (many_rows(heads / c->v.kv, max_new)) n += parts_bytes(c->sms, kPreRows, c->v.hd);
+  return n;
 }
 
 int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
@@ -264,6 +297,7 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   if (rows < 0 || n_seqs < 0) return fail(MQ_ERR_INVALID, "negative count: %d rows, %d requests", rows, n_seqs);
   if (heads < 1 || heads % c->v.kv)
     return fail(MQ_ERR_INVALID, "%d query heads do not share %d key/value heads evenly", heads, c->v.kv);
+  if ((int64_t)rows * heads > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows of %d heads are too many", rows, heads);
   if (max_pages < 1 || max_new < 0) return fail(MQ_ERR_INVALID, "%d pages a request, %d new rows", max_pages, max_new);
   if (!std::isfinite(scale)) return fail(MQ_ERR_INVALID, "the score scale is not finite");
   if (rows == 0 || n_seqs == 0) return MQ_OK;
@@ -285,17 +319,16 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   a.out = out, a.ld_o = ld_out, a.hs_o = hs_out;
   a.offsets = offsets, a.lens = seq_lens, a.tables = block_tables;
   a.n = n_seqs, a.width = max_pages, a.rows = rows, a.group = heads / c->v.kv;
-  a.min_rows = 1, a.max_rows = INT_MAX;
   a.scale = scale * 1.44269504088896341f;
-  a.meta = static_cast<int4 *>(workspace);
-  a.parts = reinterpret_cast<float *>(a.meta + 2 * dec_grid(c->sms));
   a.vec_q = vector16(q, ld_q, hs_q);
   a.vec_o = vector16(out, ld_out, hs_out);
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  const bool many = many_rows(a.group, max_new);
   switch (c->v.nb) {
-  case 1: return launch_decode<1>(a, c->device, c->sms, s);
-  case 2: return launch_decode<2>(a, c->device, c->sms, s);
-  case 3: return launch_decode<3>(a, c->device, c->sms, s);
-  default: return launch_decode<4>(a, c->device, c->sms, s);
+  case 1: return run_attention<1>(a, c, ws, many, s);
+  case 2: return run_attention<2>(a, c, ws, many, s);
+  case 3: return run_attention<3>(a, c, ws, many, s);
+  default: return run_attention<4>(a, c, ws, many, s);
   }
 }
 

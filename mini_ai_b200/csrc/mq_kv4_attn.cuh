@@ -591,31 +591,51 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
   }
 }
 
-// Joins the parts of the items that their first CTA left unfinished. Block
-// (CTA, row of the tile), one thread an element; the parts in order.
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int row_tile) {
+// Joins the parts of the items that their first CTA left unfinished: 8 rows of
+// one item a block, 4 elements a thread, the parts in order. The blocks of the
+// few-row kernel's CTAs come first, then `chunks` for each of the other's.
+struct Kv4Join {
+  const int4 *meta[2];
+  const float *parts[2];
+  int ctas[2];
+};
+constexpr int kJoinRows = 8;
+
+__global__ void __launch_bounds__(kJoinRows * 32) kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
   sm100::griddep_wait();
-  const int b = blockIdx.x, row = blockIdx.y, hd = a.c.hd, e = threadIdx.x;
-  const int parts = a.meta[2 * b + 1].x;
+  const int which = blockIdx.x >= j.ctas[0], row_tile = which ? 128 : kDecRowTile;
+  const int at = which ? blockIdx.x - j.ctas[0] : blockIdx.x, chunks = row_tile / kJoinRows;
+  const int b = at / chunks, hd = a.c.hd, quads = hd / 4;
+  const int4 *meta = (which ? j.meta[1] : j.meta[0]) + 2 * b;
+  const int parts = meta[1].x;
   if (parts == 0) return;
-  const int4 m = a.meta[2 * b];
+  const int4 m = meta[0];
+  const int row = at % chunks * kJoinRows + threadIdx.x / quads, e = 4 * (threadIdx.x % quads);
   const int fr = m.y * row_tile + row;
   if (fr >= m.w) return;
   const int64_t stride = kv4_part_floats(row_tile, hd);
-  auto part = [&](int i) { return a.parts + (2 * (int64_t)(b + i) + (i == 0)) * stride; };
+  const float *parts0 = which ? j.parts[1] : j.parts[0];
+  auto part = [&](int i) { return parts0 + (2 * (int64_t)(b + i) + (i == 0)) * stride; };
   float top = -INFINITY;
+#pragma unroll 8
   for (int i = 0; i < parts; ++i) top = fmaxf(top, part(i)[row]);
   const float shift = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, acc = 0.0f;
-#pragma unroll 4
+  float total = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
   for (int i = 0; i < parts; ++i) {
     const float *p = part(i);
     const float k = ex2(p[row] - shift);
+    const float4 v = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * hd + e);
     total += k * p[row_tile + row];
-    acc += k * p[2 * row_tile + (int64_t)row * hd + e];
+    acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
   }
-  a.out[(int64_t)(m.x + fr / a.group) * a.ld_o + (int64_t)(m.z * a.group + fr % a.group) * a.hs_o + e] =
-      total == 0.0f ? 0.0f : acc / total;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+  float *dst =
+      a.out + (int64_t)(m.x + fr / a.group) * a.ld_o + (int64_t)(m.z * a.group + fr % a.group) * a.hs_o + e;
+  if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
+  else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
 }
 
 }  // namespace mq

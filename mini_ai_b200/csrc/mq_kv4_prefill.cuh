@@ -1,0 +1,581 @@
+// Causal attention over the paged 4-bit cache for many rows a request
+// (prompts and their chunks): 128 flat rows an item, 128 tokens a step, on
+// tcgen05. Work division and row semantics as in mq_kv4_attn.cuh.
+//
+// Per step, with Q and P as fp16 hi + lo pairs (22 bits) in TMEM and the
+// cache's values, exact in fp16, in shared memory:
+//   S = Qhi K^T + Qlo K^T            [128 rows, 128 tokens], fp32 in TMEM
+//   P = 2^(S f - ref) -> Phi, Plo    one thread a row and half of the columns
+//   O = Phi V + Plo V                [128 rows, hd], fp32 in TMEM
+// and the running output of a row is in its threads' registers: adding one
+// step's O there costs hd additions a row, keeps every tensor-core sum at 16
+// additions (they truncate), and lets a moved reference scale registers.
+// Both A operands come from TMEM, so shared memory feeds the tensor cores
+// with B alone (64 of its 128 bytes a clock).
+//
+// Warps: 0-3 and 4-7 softmax (token halves of a step; each half of the
+// output's columns), 8-11 decode (packed units -> swizzled K and V tiles),
+// 12 issues the MMAs, 13 the copies of the packed units.
+// S of step i + 1 is computed while the softmax of step i runs, and O of step
+// i during the softmax of step i + 1.
+//
+// Bound: the tensor cores. Twice 4 hd operations a (row, token) pair (hi and
+// lo) against 1.67 PFLOP/s; the softmax costs about 1100 of a step's 2048
+// issue slots.
+#pragma once
+
+#include "mq_kv4_attn.cuh"
+
+namespace mq {
+
+constexpr int kPreRows = 128;    // RT
+constexpr int kPreTokens = 128;  // BN
+constexpr int kPreThreads = 512;
+constexpr int kPreRaw = 3;       // packed steps in flight
+constexpr int kPreStages = 2;    // K and V tiles
+constexpr int kPreMasks = 4;
+constexpr int kPreUnits = kPreTokens / kKv4Unit;
+constexpr uint64_t kPreDrainNs = 20000000ull;
+
+template <int NB>
+struct PreSmem {
+  static constexpr int HD = 32 * NB;
+  static constexpr int kPanel = kPreTokens * 128;           // 64 head elements of every token
+  static constexpr int kK = (NB + 1) / 2 * kPanel;
+  static constexpr int kVPanel = HD * 128;                  // 64 tokens of every head element
+  static constexpr int kV = 2 * kVPanel;
+  static constexpr int kRaw = kPreUnits * kv4_unit_bytes(NB);
+  static constexpr int kKOff = 0;
+  static constexpr int kVOff = kPreStages * kK;
+  static constexpr int kRawOff = kVOff + kPreStages * kV;
+  static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][2 halves][128 rows]
+  static constexpr int kNanOff = kXchOff + 2 * 2 * kPreRows * 4;  // bytes [masks][NB][16 token groups]
+  static constexpr int kBarOff = kNanOff + kPreMasks * NB * 16;
+  static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 6;
+  static constexpr int kBytes = kBarOff + 8 * kBars + 64;
+  static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
+  static_assert(kAlloc <= 227 * 1024, "shared memory");
+  static_assert(kK % 1024 == 0 && kVPanel % 1024 == 0 && kBarOff % 8 == 0, "swizzle atoms and barriers");
+};
+
+// TMEM columns.
+constexpr uint32_t kTmQ = 0;     // hi [0, hd / 2), lo [64, 64 + hd / 2)
+constexpr uint32_t kTmS = 128;   // 128
+constexpr uint32_t kTmP = 256;   // hi 64, lo 64
+constexpr uint32_t kTmO = 384;   // hd
+
+// Instruction descriptor, kind::f16: F16 x F16 -> F32, both K-major.
+__host__ __device__ constexpr uint32_t idesc_half_f32(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tm_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void set_regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// The 256 softmax threads.
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// A place in a ring of N barriers, and the parity of its current pass.
+template <int N>
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) i = 0, phase ^= 1u;
+  }
+};
+
+template <int NB>
+__global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4AttnArgs a) {
+  using L = PreSmem<NB>;
+  constexpr int HD = L::HD, W = (NB + 1) / 2, UB = kv4_unit_bytes(NB);
+  extern __shared__ uint8_t pre_raw[];
+  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pre_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *raw_full = reinterpret_cast<uint64_t *>(sm + L::kBarOff), *raw_empty = raw_full + kPreRaw;
+  uint64_t *k_full = raw_empty + kPreRaw, *k_empty = k_full + kPreStages;
+  uint64_t *v_full = k_empty + kPreStages, *v_empty = v_full + kPreStages;
+  uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *s_free = s_full + 1, *p_full = s_free + 1,
+           *o_full = p_full + 1, *fin = o_full + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fin + 1);
+  volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  uint32_t *raw_valid = tmem_slot + 2;   // [kPreRaw]: the packed units that were copied
+  uint32_t *unit_mask = raw_valid + kPreRaw;  // [kPreMasks]: the same, for the softmax
+  float *xch = reinterpret_cast<float *>(sm + L::kXchOff);
+  uint8_t *nan_bits = sm + L::kNanOff;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&raw_full[i], 1), sm100::mbar_init(&raw_empty[i], 128);
+    for (int i = 0; i < kPreStages; ++i) {
+      sm100::mbar_init(&k_full[i], 128), sm100::mbar_init(&k_empty[i], 1);
+      sm100::mbar_init(&v_full[i], 128), sm100::mbar_init(&v_empty[i], 1);
+    }
+    sm100::mbar_init(q_full, 256);
+    sm100::mbar_init(s_full, 1);
+    sm100::mbar_init(s_free, 256);
+    sm100::mbar_init(p_full, 256);
+    sm100::mbar_init(o_full, 1);
+    sm100::mbar_init(fin, 1);
+    *abort = 0;
+    sm100::fence_mbar_init();
+  }
+  sm100::griddep_wait();
+  sm100::griddep_launch_dependents();
+  if (threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
+  Kv4Walk walk;
+  const bool work = kv4_walk<kPreRows, kPreTokens>(a, walk);
+  if (work) {
+    if (warp == 12) {
+      sm100::tmem_alloc(tmem_slot, 512);
+      sm100::tmem_relinquish();
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      return sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs);
+    };
+    // Steps of a segment that some row sees.
+    auto steps_of = [&](const Kv4Segment &s) {
+      const int f = min((s.tile + 1) * kPreRows, s.q.flat) - 1;
+      const int last = min(s.q.base + f / a.group, s.q.len - 1);
+      return max(0, min(s.t1, (last + kPreTokens) / kPreTokens) - s.t0);
+    };
+    Kv4Segment s;
+
+    if (warp < 8) {
+      // -------------------------------------------------------- softmax
+      set_regs_up<176>();
+      const int half = warp >> 2, row = 32 * (warp & 3) + lane;
+      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+      uint32_t s_phase = 0, o_phase = 0;
+      Ring<kPreMasks> mask, smask;  // of the output's and of the scores' step
+      int parity = 0;               // of the exchange buffers
+      bool ok = true;
+      auto exchange = [&](float mine) {  // the other half's value of this row
+        float *x = xch + parity * 2 * kPreRows;
+        x[half * kPreRows + row] = mine;
+        softmax_sync();
+        parity ^= 1;
+        return x[(half ^ 1) * kPreRows + row];
+      };
+      while (kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
+        const int steps = steps_of(s);
+        const int f = s.tile * kPreRows + row, qi = f / a.group;
+        const bool real = f < s.q.flat;
+        const int last = real ? min(s.q.base + qi, s.q.len - 1) : -1;
+        float acc[HD / 2];
+#pragma unroll
+        for (int i = 0; i < HD / 2; ++i) acc[i] = 0.0f;
+        float ref = -INFINITY, sum = 0.0f;
+        uint32_t poison = 0;
+        if (steps > 0) {
+          // ---- this half of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
+          float x[HD / 2], mx = 0.0f;
+          const float *p = a.q + (int64_t)(s.q.row0 + qi) * a.ld_q +
+                           (int64_t)(s.head * a.group + f % a.group) * a.hs_q + half * (HD / 2);
+#pragma unroll
+          for (int i = 0; i < HD / 2; i += 4) {
+            if (!real) {
+              x[i] = x[i + 1] = x[i + 2] = x[i + 3] = 0.0f;
+            } else if (a.vec_q) {
+              const float4 v = *reinterpret_cast<const float4 *>(p + i);
+              x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+            } else {
+              x[i] = p[i], x[i + 1] = p[i + 1], x[i + 2] = p[i + 2], x[i + 3] = p[i + 3];
+            }
+          }
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < HD / 2; ++i) mx = fmaxf(mx, fabsf(x[i])), bad |= !isfinite(x[i]);
+          if (bad) mx = INFINITY;
+          mx = fmaxf(mx, exchange(mx));
+          bad = mx == INFINITY;
+          const int e = min(141 - (int)(__float_as_uint(mx) >> 23), 126);
+          float up = __uint_as_float((uint32_t)(127 + e) << 23);
+          if (a.scale < 0.0f) up = -up;  // f is positive: the largest S is the largest score
+          // (never 0, so that f * -inf is -inf; a row that sees nothing is 0 whatever its query)
+          const float scale = bad && last >= 0 ? __uint_as_float(0x7fc00000u) : fmaxf(ldexpf(fabsf(a.scale), -e), 1.2e-38f);
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) {  // 8 elements, in the order of a decoded word
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split_f16(x[8 * c + i] * up, x[8 * c + i + 4] * up, hi[i], lo[i]);
+            const uint32_t col = half * (HD / 4) + 4 * c;
+            tm_st4(lanes + kTmQ + col, hi[0], hi[1], hi[2], hi[3]);
+            tm_st4(lanes + kTmQ + 64 + col, lo[0], lo[1], lo[2], lo[3]);
+          }
+          tm_st_wait();
+          sm100::tc_fence_before();
+          sm100::mbar_arrive(q_full);
+
+          auto add_output = [&](int k) {  // O of step k
+            ok = wait(o_full, o_phase) && ok;
+            o_phase ^= 1u;
+            sm100::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 16) {
+              uint32_t r[16];
+              tm_ld16(lanes + kTmO + half * (HD / 2) + c, r);
+              sm100::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[c + i] += __uint_as_float(r[i]);
+            }
+            // NaN values of the step entered as 0: the rows that see them are marked.
+            const uint64_t *bits = reinterpret_cast<const uint64_t *>(nan_bits + mask.i * NB * 16 + 8 * half);
+            uint64_t any = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) any |= bits[2 * b];
+            if (any) {
+              const int see = last - (s.t0 + k) * kPreTokens - 64 * half;
+              const uint64_t mine = see < 0 ? 0 : see >= 63 ? ~0ull : (2ull << see) - 1;
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                if (bits[2 * b] & mine) poison |= 1u << b;
+            }
+            mask.next();
+          };
+
+          for (int k = 0; k < steps; ++k) {
+            ok = wait(s_full, s_phase) && ok;
+            s_phase ^= 1u;
+            sm100::tc_fence_after();
+            uint32_t r[64];
+            tm_ld16(lanes + kTmS + 64 * half, r);
+            tm_ld16(lanes + kTmS + 64 * half + 16, r + 16);
+            tm_ld16(lanes + kTmS + 64 * half + 32, r + 32);
+            tm_ld16(lanes + kTmS + 64 * half + 48, r + 48);
+            const uint32_t units = unit_mask[smask.i] >> (4 * half) & 15u;
+            smask.next();
+            const int see = last - (s.t0 + k) * kPreTokens - 64 * half;  // columns 0..see
+            sm100::tmem_ld_wait();
+            sm100::tc_fence_before();
+            sm100::mbar_arrive(s_free);
+            if (see < 63 || units != 15u) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (i > see || !(units >> (i >> 4) & 1u)) r[i] = 0xff800000u;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+            top = fmaxf(top, exchange(top)) * scale;
+            float old = 1.0f;
+            if (top > ref + 15.0f || (ref == -INFINITY && top > -INFINITY)) {
+              const float to = top - 8.0f;
+              old = ex2(ref - to);
+              ref = to;
+              sum *= old;
+            }
+            const float shift = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, -shift));
+              const float p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, -shift));
+              sum += p0 + p1;
+              split_f16(p0, p1, r[i], r[i + 1]);
+            }
+            if (k > 0) add_output(k - 1);
+            if (__any_sync(0xffffffffu, old != 1.0f)) {
+#pragma unroll
+              for (int i = 0; i < HD / 2; ++i) acc[i] *= old;
+            }
+            // column 32 half + j of P: tokens 2j, 2j + 1 of this half
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = r[32 * (c & 1) + 2 * i + (c >> 1)];
+              tm_st16(lanes + kTmP + 64 * (c >> 1) + 32 * half + 16 * (c & 1), w);
+            }
+            tm_st_wait();
+            sm100::tc_fence_before();
+            sm100::mbar_arrive(p_full);
+          }
+          add_output(steps - 1);
+        }
+        // ---- the row's end
+        const float total = sum + exchange(sum);
+        poison |= __float_as_uint(exchange(__uint_as_float(poison)));
+        const bool whole = s.t0 == 0 && s.t1 == s.whole;
+        if (!ok) poison = ~0u;
+        if (real) {
+          float *dst;
+          bool vec = true;
+          float inv = 1.0f;
+          if (whole) {
+            dst = a.out + (int64_t)(s.q.row0 + qi) * a.ld_o + (int64_t)(s.head * a.group + f % a.group) * a.hs_o;
+            vec = a.vec_o;
+            inv = total == 0.0f ? 0.0f : 1.0f / total;
+          } else {
+            float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kPreRows, HD);
+            dst = part + 2 * kPreRows + row * HD;
+            if (half == 0) part[row] = ref, part[kPreRows + row] = total;
+          }
+          dst += half * (HD / 2);
+#pragma unroll
+          for (int i = 0; i < HD / 2; i += 4) {
+            float4 v = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+            if (poison >> ((half * (HD / 2) + i) / 32) & 1u) {
+              const float n = __uint_as_float(0x7fc00000u);
+              v = make_float4(n, n, n, n);
+            }
+            if (vec) *reinterpret_cast<float4 *>(dst + i) = v;
+            else dst[i] = v.x, dst[i + 1] = v.y, dst[i + 2] = v.z, dst[i + 3] = v.w;
+          }
+        }
+        if (threadIdx.x == 0 && s.t0 == 0 && !whole) {
+          a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
+          a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
+        }
+      }
+    } else if (warp < 12) {
+      // -------------------------------------------------------- packed units -> K and V tiles
+      set_regs_down<80>();
+      const int dw = warp - 8;
+      Ring<kPreRaw> raw;
+      Ring<kPreStages> st;
+      Ring<kPreMasks> mask;
+      bool ok = true;
+      while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
+        const int steps = steps_of(s);
+        for (int k = 0; k < steps; ++k) {
+          if (!(ok = wait(&raw_full[raw.i], raw.phase))) break;
+          if (!(ok = wait(&k_empty[st.i], st.phase ^ 1u))) break;
+          const uint8_t *src = sm + L::kRawOff + raw.i * L::kRaw;
+          const uint32_t valid = raw_valid[raw.i];
+          if (dw == 0 && lane == 0) unit_mask[mask.i] = valid;
+          uint8_t *kt = sm + L::kKOff + st.i * L::kK;
+#pragma unroll 2
+          for (int it = 0; it < 4; ++it) {
+            // 8 tokens x 4 chunks a warp, paired so that neither the loads nor the stores meet a bank twice
+            const int tok = 8 * (4 * it + dw) + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tok & 15;
+            const uint8_t *u = src + (tok >> 4) * UB;
+            uint32_t kw[NB], d[W];
+            const uint8_t *kp = u + tk * (16 * NB) + t * (4 * NB);
+            if constexpr (NB == 4) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(kp);
+              kw[0] = v.x, kw[1] = v.y, kw[2] = v.z, kw[3] = v.w;
+            } else if constexpr (NB == 2) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+              kw[0] = v.x, kw[1] = v.y;
+            } else {
+#pragma unroll
+              for (int b = 0; b < NB; ++b) kw[b] = reinterpret_cast<const uint32_t *>(kp)[b];
+            }
+            lds_halves<NB>(u + kv4_k_scale_off(NB) + tk * (2 * NB), d);
+            if (!(valid >> (tok >> 4) & 1u)) {
+#pragma unroll
+              for (int i = 0; i < W; ++i) d[i] = 0u;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const __half2 dd = bits_h2(pair_halves(d, d, b));
+              const uint32_t w = kw[b], w8 = w >> 8;
+              uint4 o;
+              o.x = h2_bits(__hmul2(code_lo(w), dd)), o.y = h2_bits(__hmul2(code_hi(w), dd));
+              o.z = h2_bits(__hmul2(code_lo(w8), dd)), o.w = h2_bits(__hmul2(code_hi(w8), dd));
+              *reinterpret_cast<uint4 *>(kt + (b >> 1) * L::kPanel + tok * 128 +
+                                         ((((b & 1) * 4 + t) ^ (tok & 7)) << 4)) = o;
+            }
+          }
+          sm100::fence_proxy_async_smem();
+          sm100::mbar_arrive(&k_full[st.i]);
+
+          if (!(ok = wait(&v_empty[st.i], st.phase ^ 1u))) break;
+          uint8_t *vt = sm + L::kVOff + st.i * L::kV;
+          {
+            // 8 tokens and 4 elements of every block a thread; odd groups read their tokens in pairs swapped
+            const int m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
+            const uint8_t *u = src + (m >> 1) * UB;
+            uint32_t vw[8][W], vd[8][W];
+            __half2 check = __float2half2_rn(0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int tk = (8 * m + (i ^ odd)) & 15;
+              lds_halves<NB>(u + kv4_v_off(NB) + tk * (16 * NB) + g * (2 * NB), vw[i]);
+              lds_halves<NB>(u + kv4_v_scale_off(NB) + tk * (2 * NB), vd[i]);
+              if (!(valid >> (m >> 1) & 1u)) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) vd[i][j] = 0u;
+              }
+#pragma unroll
+              for (int j = 0; j < W; ++j) check = __hadd2(check, __habs2(bits_h2(vd[i][j])));
+            }
+            uint32_t bad[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) bad[b] = 0u;
+            const uint32_t cb = h2_bits(check);
+            if ((cb & 0x7c00u) == 0x7c00u || (cb & 0x7c000000u) == 0x7c000000u) {  // a NaN scale, or many large ones
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                  const int sh = b & 1 ? 16 : 0;
+                  if ((vd[i][b >> 1] >> sh & 0x7fffu) >= 0x7c00u) {
+                    bad[b] |= 1u << (i ^ odd);
+                    vd[i][b >> 1] &= ~(0xffffu << sh);
+                  }
+                }
+            }
+            if (g == 0) {
+#pragma unroll
+              for (int b = 0; b < NB; ++b) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[b];
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t sel = odd ? (b & 1 ? 0x3276u : 0x1054u) : (b & 1 ? 0x7632u : 0x5410u);
+              uint32_t o[4][4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                const uint32_t x = __byte_perm(vw[2 * p][b >> 1], vw[2 * p + 1][b >> 1], sel), y = x >> 8;
+                const __half2 dd = bits_h2(__byte_perm(vd[2 * p][b >> 1], vd[2 * p + 1][b >> 1], sel));
+                o[0][p] = h2_bits(__hmul2(code_lo(x), dd)), o[1][p] = h2_bits(__hmul2(code_hi(x), dd));
+                o[2][p] = h2_bits(__hmul2(code_lo(y), dd)), o[3][p] = h2_bits(__hmul2(code_hi(y), dd));
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int e = 32 * b + 4 * g + i;
+                *reinterpret_cast<uint4 *>(vt + (m >> 3) * L::kVPanel + e * 128 + (((m & 7) ^ (e & 7)) << 4)) =
+                    make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+              }
+            }
+          }
+          sm100::fence_proxy_async_smem();
+          sm100::mbar_arrive(&v_full[st.i]);
+          sm100::mbar_arrive(&raw_empty[raw.i]);
+          raw.next(), st.next(), mask.next();
+        }
+      }
+    } else {
+      set_regs_down<80>();
+      if (warp == 12 && lane == 0) {
+        // ------------------------------------------------------ MMA issue
+        constexpr uint32_t id_s = idesc_half_f32(kPreRows, kPreTokens), id_o = idesc_half_f32(kPreRows, HD);
+        Ring<kPreStages> ks, vs;
+        uint32_t q_phase = 0, p_phase = 0, free_phase = 1;  // S is free at first
+        bool ok = true;
+        while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
+          const int steps = steps_of(s);
+          if (steps == 0) continue;
+          if (!(ok = wait(q_full, q_phase))) break;
+          q_phase ^= 1u;
+          auto scores = [&]() {
+            if (!wait(&k_full[ks.i], ks.phase) || !wait(s_free, free_phase)) return false;
+            free_phase ^= 1u;
+            sm100::tc_fence_after();
+            const uint32_t base = sm100::smem_u32(sm + L::kKOff + ks.i * L::kK);
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int kk = 0; kk < 2 * NB; ++kk)
+                umma_f16_ts(tmem + kTmS, tmem + kTmQ + 64 * part + 8 * kk,
+                            sm100::umma_desc_sw128(base + (kk >> 2) * L::kPanel) + 2 * (kk & 3), id_s, part || kk);
+            sm100::umma_commit(s_full);
+            sm100::umma_commit(&k_empty[ks.i]);
+            ks.next();
+            return true;
+          };
+          if (!(ok = scores())) break;
+          for (int k = 0; k < steps; ++k) {
+            if (k + 1 < steps && !(ok = scores())) break;
+            if (!(ok = wait(&v_full[vs.i], vs.phase) && wait(p_full, p_phase))) break;
+            p_phase ^= 1u;
+            sm100::tc_fence_after();
+            const uint32_t base = sm100::smem_u32(sm + L::kVOff + vs.i * L::kV);
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int kk = 0; kk < kPreTokens / 16; ++kk)
+                umma_f16_ts(tmem + kTmO, tmem + kTmP + 64 * part + 8 * kk,
+                            sm100::umma_desc_sw128(base + (kk >> 2) * L::kVPanel) + 2 * (kk & 3), id_o, part || kk);
+            sm100::umma_commit(o_full);
+            sm100::umma_commit(&v_empty[vs.i]);
+            vs.next();
+          }
+        }
+        sm100::umma_commit(fin);  // every MMA has completed before the TMEM is released
+        sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
+      } else if (warp == 13) {
+        // ------------------------------------------------------ copies of the packed units
+        const int upp = a.c.page / kKv4Unit;
+        const int64_t unit_page = a.c.page_head_bytes * a.c.kv;
+        Ring<kPreRaw> raw;
+        bool ok = true;
+        int issued = 0;
+        while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
+          const int steps = steps_of(s), end_unit = (s.q.len + kKv4Unit - 1) / kKv4Unit;
+          const int *table = a.tables + (int64_t)s.r * a.width;
+          const uint8_t *slice = kv4_unit(a.c, a.layer, 0, s.head, 0);
+          for (int k = 0; k < steps; ++k) {
+            const int u = (s.t0 + k) * kPreUnits + lane;
+            int id = lane < kPreUnits && u < end_unit ? __ldg(table + u / upp) : -1;
+            if (id >= a.c.pages) id = -1;
+            const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+            ok = __all_sync(0xffffffffu, wait(&raw_empty[raw.i], raw.phase ^ 1u));
+            if (!ok) break;
+            if (lane == 0) {
+              raw_valid[raw.i] = have;
+              sm100::mbar_arrive_expect_tx(&raw_full[raw.i], __popc(have) * UB);
+            }
+            __syncwarp();
+            if (id >= 0)
+              sm100::bulk_load(sm + L::kRawOff + raw.i * L::kRaw + lane * UB,
+                               slice + id * unit_page + (int64_t)(u % upp) * UB, UB, &raw_full[raw.i]);
+            raw.next();
+            ++issued;
+          }
+        }
+        // the last copies have landed before the CTA can exit
+        for (int i = max(0, issued - kPreRaw); i < issued; ++i)
+          sm100::mbar_wait(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u, nullptr, nullptr, kPreDrainNs);
+      }
+    }
+    __syncwarp();
+    sm100::tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+      sm100::tc_fence_after();
+      sm100::tmem_dealloc(tmem, 512);
+    }
+  }
+}
+
+}  // namespace mq
