@@ -50,31 +50,28 @@ struct Kv4Request {
   int64_t work;  // of one KV head
 };
 
-// sum of floor((a i + b) / m) for i in [0, n); a, b >= 0, m > 0 (the Euclid-like recursion).
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t s = 0;
-  for (;;) {
-    s += (n - 1) * n / 2 * (a / m) + n * (b / m);
-    a %= m, b %= m;
-    const int64_t y = a * n + b;
-    if (y < m) return s;
-    n = y / m, b = y % m;
-    const int64_t t = m;
-    m = a, a = t;
-  }
+// Quotients of two non-negative 64-bit numbers that are nearly always small:
+// a 64-bit division costs about 100 instructions.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
 
-// Work of the first `tiles` row tiles: tile i costs floor((base G + RT (i + 1) - 1) / (G BN)) + 1,
-// the BN-token tiles up to its last row (a tile cut short by the request's end may see fewer).
+// Work of the first n row tiles of a request. With `period` = G BN / RT row
+// tiles to a step of BN tokens, and the tokens before the request's rows
+// rounded up to whole steps, tile i counts floor(i / period) + 1 steps more:
+// never fewer than its last row sees, and at most one more.
 template <int RT, int BN>
-__device__ __forceinline__ int64_t kv4_work(int base, int group, int tiles) {
-  const int64_t b = (int64_t)max(base, 0) * group + RT - 1, m = (int64_t)group * BN;
-  if (tiles == 1) return b / m + 1;
-  return tiles ? floor_sum(tiles, m, RT, b) + tiles : 0;
+__device__ __forceinline__ int64_t kv4_work(int base, int group, int n) {
+  const int64_t before = (max(base, 0) + BN - 1) / BN + 1;
+  if (n <= 1) return n ? before : 0;
+  const int period = group * (BN / RT), full = n / period, rest = n % period;
+  return n * before + (int64_t)period * full * (full - 1) / 2 + (int64_t)rest * full;
 }
 
 template <int RT, int BN>
 __device__ __forceinline__ Kv4Request kv4_request(const Kv4AttnArgs &a, int r) {
+  static_assert(BN % RT == 0, "");
   Kv4Request q;
   const int first = __ldg(a.offsets + r), end = __ldg(a.offsets + r + 1);
   const int64_t fresh = (int64_t)end - first;
@@ -91,11 +88,12 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4AttnArgs &a, int r) {
 
 // A walk along this CTA's piece of the line.
 struct Kv4Walk {
-  int r;               // request at the current place
-  int64_t at;          // place within it
-  int64_t left;        // work left to this CTA
+  int r;                // request at the current place
+  int loaded;           // the request in the segment
+  int64_t at;           // place within it
+  int64_t left;         // work left to this CTA
   int64_t line, place;  // the whole line, and the current place on it
-  int ctas;            // pieces
+  int ctas;             // pieces
 };
 
 // All threads; two block-wide scans. false: no work for this CTA.
@@ -111,8 +109,8 @@ __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
   if (w.line == 0) return false;
   w.ctas = (int)min((int64_t)gridDim.x, w.line);
   if ((int)blockIdx.x >= w.ctas) return false;
-  w.place = blockIdx.x * w.line / w.ctas;
-  w.left = (blockIdx.x + 1) * w.line / w.ctas - w.place;
+  w.place = quotient(blockIdx.x * w.line, w.ctas);
+  w.left = quotient((blockIdx.x + 1) * w.line, w.ctas) - w.place;
   if (w.place >= upto - mine && w.place < upto) {
     int64_t at = w.place - (upto - mine);
     int r = r0;
@@ -124,7 +122,7 @@ __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
     s_r = r, s_at = at;
   }
   __syncthreads();
-  w.r = s_r, w.at = s_at;
+  w.r = s_r, w.at = s_at, w.loaded = -1;
   return true;
 }
 
@@ -140,13 +138,13 @@ template <int RT, int BN>
 __device__ __forceinline__ bool kv4_next(const Kv4AttnArgs &a, Kv4Walk &w, Kv4Segment &s) {
   if (w.left == 0) return false;
   for (;; ++w.r) {
-    s.q = kv4_request<RT, BN>(a, w.r);
+    if (w.loaded != w.r) s.q = kv4_request<RT, BN>(a, w.r), w.loaded = w.r;
     if (w.at < a.c.kv * s.q.work) break;
     w.at -= a.c.kv * s.q.work;
   }
   s.r = w.r;
-  s.head = (int)(w.at / s.q.work);
-  const int64_t in_head = w.at % s.q.work;
+  s.head = (int)quotient(w.at, s.q.work);
+  const int64_t in_head = w.at - s.head * s.q.work;
   int lo = 0, hi = s.q.tiles - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -165,7 +163,7 @@ __device__ __forceinline__ bool kv4_next(const Kv4AttnArgs &a, Kv4Walk &w, Kv4Se
 
 // The CTAs from this one on that an item which ends at place `end` is spread over.
 __device__ __forceinline__ int kv4_spread(const Kv4Walk &w, int64_t end) {
-  return (int)((end * w.ctas - 1) / w.line) - (int)blockIdx.x + 1;
+  return (int)quotient(end * w.ctas - 1, w.line) - (int)blockIdx.x + 1;
 }
 
 // ------------------------------------------------------------ fragments
