@@ -178,10 +178,16 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cas
 
 // (x, y) as fp16 hi + lo pairs: 22 bits of each.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = h2_bits(h);
-  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+  hi = h2_bits(__floats2half2_rn(x, y));
+  float a, b;  // x and y less their hi parts, in one mixed-precision instruction each
+  asm("{\n\t.reg .f16 h0, h1, m;\n\t"
+      "mov.b32 {h0, h1}, %2;\n\t"
+      "mov.b16 m, 0xBC00;\n\t"
+      "fma.rn.f32.f16 %0, h0, m, %3;\n\t"
+      "fma.rn.f32.f16 %1, h1, m, %4;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "r"(hi), "f"(x), "f"(y));
+  lo = h2_bits(__floats2half2_rn(a, b));
 }
 
 // D = A B + D: A 16 x 16 row-major, B 16 x 8 column-major, fp16; D fp32.

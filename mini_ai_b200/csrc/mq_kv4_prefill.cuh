@@ -58,11 +58,11 @@ struct PreSmem {
   static_assert(kK % 1024 == 0 && kVPanel % 1024 == 0 && kBarOff % 8 == 0, "swizzle atoms and barriers");
 };
 
-// TMEM columns.
-constexpr uint32_t kTmQ = 0;     // hi [0, hd / 2), lo [64, 64 + hd / 2)
-constexpr uint32_t kTmS = 128;   // 128
-constexpr uint32_t kTmP = 256;   // hi 64, lo 64
-constexpr uint32_t kTmO = 384;   // hd
+// TMEM columns. P replaces S in place: the 16 columns of 16 tokens' scores
+// become 8 of their weights' hi parts and 8 of the lo parts.
+constexpr uint32_t kTmQ = 0;    // hi [0, hd / 2), lo [64, 64 + hd / 2)
+constexpr uint32_t kTmS = 128;  // 2 x 128: even and odd steps
+constexpr uint32_t kTmO = 384;  // hd
 
 // Instruction descriptor, kind::f16: F16 x F16 -> F32, both K-major.
 __host__ __device__ constexpr uint32_t idesc_half_f32(int M, int N) {
@@ -86,6 +86,7 @@ __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t *r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) { sm100::tmem_ld_32x32b_x32(addr, r); }
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -130,8 +131,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   uint64_t *raw_full = reinterpret_cast<uint64_t *>(sm + L::kBarOff), *raw_empty = raw_full + kPreRaw;
   uint64_t *k_full = raw_empty + kPreRaw, *k_empty = k_full + kPreStages;
   uint64_t *v_full = k_empty + kPreStages, *v_empty = v_full + kPreStages;
-  uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *s_free = s_full + 1, *p_full = s_free + 1,
-           *o_full = p_full + 1, *fin = o_full + 1;
+  uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 1,
+           *fin = o_full + 1;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fin + 1);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   uint32_t *raw_valid = tmem_slot + 2;   // [kPreRaw]: the packed units that were copied
@@ -147,8 +148,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       sm100::mbar_init(&v_full[i], 128), sm100::mbar_init(&v_empty[i], 1);
     }
     sm100::mbar_init(q_full, 256);
-    sm100::mbar_init(s_full, 1);
-    sm100::mbar_init(s_free, 256);
+    sm100::mbar_init(&s_full[0], 1), sm100::mbar_init(&s_full[1], 1);
     sm100::mbar_init(p_full, 256);
     sm100::mbar_init(o_full, 1);
     sm100::mbar_init(fin, 1);
@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       set_regs_up<176>();
       const int half = warp >> 2, row = 32 * (warp & 3) + lane;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-      uint32_t s_phase = 0, o_phase = 0;
+      uint32_t o_phase = 0;
+      Ring<2> score;
       Ring<kPreMasks> mask, smask;  // of the output's and of the scores' step
       int parity = 0;               // of the exchange buffers
       bool ok = true;
@@ -274,28 +275,28 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           };
 
           for (int k = 0; k < steps; ++k) {
-            ok = wait(s_full, s_phase) && ok;
-            s_phase ^= 1u;
+            ok = wait(&s_full[score.i], score.phase) && ok;
+            const uint32_t cols = lanes + kTmS + 128 * score.i + 64 * half;
+            score.next();
             sm100::tc_fence_after();
-            uint32_t r[64];
-            tm_ld16(lanes + kTmS + 64 * half, r);
-            tm_ld16(lanes + kTmS + 64 * half + 16, r + 16);
-            tm_ld16(lanes + kTmS + 64 * half + 32, r + 32);
-            tm_ld16(lanes + kTmS + 64 * half + 48, r + 48);
             const uint32_t units = unit_mask[smask.i] >> (4 * half) & 15u;
             smask.next();
             const int see = last - (s.t0 + k) * kPreTokens - 64 * half;  // columns 0..see
-            sm100::tmem_ld_wait();
-            sm100::tc_fence_before();
-            sm100::mbar_arrive(s_free);
-            if (see < 63 || units != 15u) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i > see || !(units >> (i >> 4) & 1u)) r[i] = 0xff800000u;
-            }
+            const bool cut = see < 63 || units != 15u;
             float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {
+              uint32_t r[32];
+              tm_ld32(cols + c, r);
+              sm100::tmem_ld_wait();
+              if (cut) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+                for (int i = 0; i < 32; ++i)
+                  if (c + i > see || !(units >> ((c + i) >> 4) & 1u)) r[i] = 0xff800000u;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+            }
             top = fmaxf(top, exchange(top)) * scale;
             float old = 1.0f;
             if (top > ref + 15.0f || (ref == -INFINITY && top > -INFINITY)) {
@@ -305,25 +306,32 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               sum *= old;
             }
             const float shift = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {
+              uint32_t r[32], w[2][16];
+              tm_ld32(cols + c, r);
+              sm100::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, -shift));
-              const float p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, -shift));
-              sum += p0 + p1;
-              split_f16(p0, p1, r[i], r[i + 1]);
+              for (int i = 0; i < 32; ++i)
+                r[i] = __float_as_uint(ex2(fmaf(__uint_as_float(r[i]), scale, -shift)));
+              if (cut) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (c + i > see || !(units >> ((c + i) >> 4) & 1u)) r[i] = 0u;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float p0 = __uint_as_float(r[i]), p1 = __uint_as_float(r[i + 1]);
+                sum += p0 + p1;
+                split_f16(p0, p1, w[i >> 4][(i & 15) >> 1], w[i >> 4][8 + ((i & 15) >> 1)]);
+              }
+              tm_st16(cols + c, w[0]);
+              tm_st16(cols + c + 16, w[1]);
             }
             if (k > 0) add_output(k - 1);
             if (__any_sync(0xffffffffu, old != 1.0f)) {
 #pragma unroll
               for (int i = 0; i < HD / 2; ++i) acc[i] *= old;
-            }
-            // column 32 half + j of P: tokens 2j, 2j + 1 of this half
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = r[32 * (c & 1) + 2 * i + (c >> 1)];
-              tm_st16(lanes + kTmP + 64 * (c >> 1) + 32 * half + 16 * (c & 1), w);
             }
             tm_st_wait();
             sm100::tc_fence_before();
@@ -383,7 +391,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           const uint32_t valid = raw_valid[raw.i];
           if (dw == 0 && lane == 0) unit_mask[mask.i] = valid;
           uint8_t *kt = sm + L::kKOff + st.i * L::kK;
-#pragma unroll 2
+#pragma unroll 1
           for (int it = 0; it < 4; ++it) {
             // 8 tokens x 4 chunks a warp, paired so that neither the loads nor the stores meet a bank twice
             const int tok = 8 * (4 * it + dw) + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tok & 15;
@@ -490,27 +498,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         // ------------------------------------------------------ MMA issue
         constexpr uint32_t id_s = idesc_half_f32(kPreRows, kPreTokens), id_o = idesc_half_f32(kPreRows, HD);
         Ring<kPreStages> ks, vs;
-        uint32_t q_phase = 0, p_phase = 0, free_phase = 1;  // S is free at first
+        uint32_t q_phase = 0, p_phase = 0;
+        int sb = 0, pb = 0;  // S buffers of the next scores and of the next output
         bool ok = true;
         while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
           const int steps = steps_of(s);
           if (steps == 0) continue;
           if (!(ok = wait(q_full, q_phase))) break;
           q_phase ^= 1u;
+          // S of a step may replace the P of two steps before: the MMAs of one thread run in order.
           auto scores = [&]() {
-            if (!wait(&k_full[ks.i], ks.phase) || !wait(s_free, free_phase)) return false;
-            free_phase ^= 1u;
+            if (!wait(&k_full[ks.i], ks.phase)) return false;
             sm100::tc_fence_after();
             const uint32_t base = sm100::smem_u32(sm + L::kKOff + ks.i * L::kK);
 #pragma unroll
             for (int part = 0; part < 2; ++part)
 #pragma unroll
               for (int kk = 0; kk < 2 * NB; ++kk)
-                umma_f16_ts(tmem + kTmS, tmem + kTmQ + 64 * part + 8 * kk,
+                umma_f16_ts(tmem + kTmS + 128 * sb, tmem + kTmQ + 64 * part + 8 * kk,
                             sm100::umma_desc_sw128(base + (kk >> 2) * L::kPanel) + 2 * (kk & 3), id_s, part || kk);
-            sm100::umma_commit(s_full);
+            sm100::umma_commit(&s_full[sb]);
             sm100::umma_commit(&k_empty[ks.i]);
             ks.next();
+            sb ^= 1;
             return true;
           };
           if (!(ok = scores())) break;
@@ -521,14 +531,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             sm100::tc_fence_after();
             const uint32_t base = sm100::smem_u32(sm + L::kVOff + vs.i * L::kV);
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int kk = 0; kk < kPreTokens / 16; ++kk)
 #pragma unroll
-              for (int kk = 0; kk < kPreTokens / 16; ++kk)
-                umma_f16_ts(tmem + kTmO, tmem + kTmP + 64 * part + 8 * kk,
+              for (int part = 0; part < 2; ++part)
+                umma_f16_ts(tmem + kTmO, tmem + kTmS + 128 * pb + 16 * kk + 8 * part,
                             sm100::umma_desc_sw128(base + (kk >> 2) * L::kVPanel) + 2 * (kk & 3), id_o, part || kk);
             sm100::umma_commit(o_full);
             sm100::umma_commit(&v_empty[vs.i]);
             vs.next();
+            pb ^= 1;
           }
         }
         sm100::umma_commit(fin);  // every MMA has completed before the TMEM is released
