@@ -282,18 +282,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             const uint32_t units = unit_mask[smask.i] >> (4 * half) & 15u;
             smask.next();
             const int see = last - (s.t0 + k) * kPreTokens - 64 * half;  // columns 0..see
-            const bool cut = see < 63 || units != 15u;
+            // (Loops of 16 columns keep the instruction cache: unrolled further, the roles' code evicted itself and
+            // a step took three times as long.)
+            // Hide what the row does not see (TMEM is read and written by whole warps).
+            if (__any_sync(0xffffffffu, see < 63 || units != 15u)) {
+#pragma unroll 1
+              for (int c = 0; c < 64; c += 16) {
+                uint32_t r[16];
+                tm_ld16(cols + c, r);
+                sm100::tmem_ld_wait();
+                const int seen = units >> (c >> 4) & 1u ? see - c : -1;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  if (i > seen) r[i] = 0xff800000u;
+                tm_st16(cols + c, r);
+              }
+              tm_st_wait();
+            }
             float top = -INFINITY;
 #pragma unroll 1
             for (int c = 0; c < 64; c += 32) {
               uint32_t r[32];
               tm_ld32(cols + c, r);
               sm100::tmem_ld_wait();
-              if (cut) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (c + i > see || !(units >> ((c + i) >> 4) & 1u)) r[i] = 0xff800000u;
-              }
 #pragma unroll
               for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
             }
@@ -307,26 +318,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             }
             const float shift = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll 1
-            for (int c = 0; c < 64; c += 32) {
-              uint32_t r[32], w[2][16];
-              tm_ld32(cols + c, r);
+            for (int c = 0; c < 64; c += 16) {
+              uint32_t r[16], w[16];
+              tm_ld16(cols + c, r);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                r[i] = __float_as_uint(ex2(fmaf(__uint_as_float(r[i]), scale, -shift)));
-              if (cut) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (c + i > see || !(units >> ((c + i) >> 4) & 1u)) r[i] = 0u;
-              }
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float p0 = __uint_as_float(r[i]), p1 = __uint_as_float(r[i + 1]);
+              for (int i = 0; i < 16; i += 2) {
+                const float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, -shift));
+                const float p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, -shift));
                 sum += p0 + p1;
-                split_f16(p0, p1, w[i >> 4][(i & 15) >> 1], w[i >> 4][8 + ((i & 15) >> 1)]);
+                split_f16(p0, p1, w[i >> 1], w[8 + (i >> 1)]);
               }
-              tm_st16(cols + c, w[0]);
-              tm_st16(cols + c + 16, w[1]);
+              tm_st16(cols + c, w);
             }
             if (k > 0) add_output(k - 1);
             if (__any_sync(0xffffffffu, old != 1.0f)) {
@@ -430,59 +433,64 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           if (!(ok = wait(&v_empty[st.i], st.phase ^ 1u))) break;
           uint8_t *vt = sm + L::kVOff + st.i * L::kV;
           {
-            // 8 tokens and 4 elements of every block a thread; odd groups read their tokens in pairs swapped
+            // 8 tokens and, two blocks at a time, 4 elements of a block a thread; odd groups read their tokens in
+            // pairs swapped
             const int m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
-            const uint8_t *u = src + (m >> 1) * UB;
-            uint32_t vw[8][W], vd[8][W];
-            __half2 check = __float2half2_rn(0.0f);
+            const bool have = valid >> (m >> 1) & 1u;
+            const uint8_t *u = src + (m >> 1) * UB + kv4_v_off(NB) + (8 * (m & 1)) * (16 * NB) + g * (2 * NB);
+            const uint8_t *us = src + (m >> 1) * UB + kv4_v_scale_off(NB) + (8 * (m & 1)) * (2 * NB);
+#pragma unroll 1
+            for (int b2 = 0; b2 < W; ++b2) {
+              constexpr int kTwo = NB == 1 ? 1 : 2;
+              uint32_t vw[8], vd[8];
+              __half2 check = __float2half2_rn(0.0f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int tk = (8 * m + (i ^ odd)) & 15;
-              lds_halves<NB>(u + kv4_v_off(NB) + tk * (16 * NB) + g * (2 * NB), vw[i]);
-              lds_halves<NB>(u + kv4_v_scale_off(NB) + tk * (2 * NB), vd[i]);
-              if (!(valid >> (m >> 1) & 1u)) {
-#pragma unroll
-                for (int j = 0; j < W; ++j) vd[i][j] = 0u;
-              }
-#pragma unroll
-              for (int j = 0; j < W; ++j) check = __hadd2(check, __habs2(bits_h2(vd[i][j])));
-            }
-            uint32_t bad[NB];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) bad[b] = 0u;
-            const uint32_t cb = h2_bits(check);
-            if ((cb & 0x7c00u) == 0x7c00u || (cb & 0x7c000000u) == 0x7c000000u) {  // a NaN scale, or many large ones
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                  const int sh = b & 1 ? 16 : 0;
-                  if ((vd[i][b >> 1] >> sh & 0x7fffu) >= 0x7c00u) {
-                    bad[b] |= 1u << (i ^ odd);
-                    vd[i][b >> 1] &= ~(0xffffu << sh);
+              for (int i = 0; i < 8; ++i) {
+                const uint8_t *pw = u + (i ^ odd) * (16 * NB) + 4 * b2, *pd = us + (i ^ odd) * (2 * NB) + 4 * b2;
+                if constexpr (NB % 2 == 0) {
+                  vw[i] = *reinterpret_cast<const uint32_t *>(pw), vd[i] = *reinterpret_cast<const uint32_t *>(pd);
+                } else {  // half-words; a row's last block stands alone
+                  vw[i] = *reinterpret_cast<const uint16_t *>(pw), vd[i] = *reinterpret_cast<const uint16_t *>(pd);
+                  if (2 * b2 + 1 < NB) {
+                    vw[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pw)[1] << 16;
+                    vd[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pd)[1] << 16;
                   }
                 }
-            }
-            if (g == 0) {
+                if (!have) vd[i] = 0u;
+                check = __hadd2(check, __habs2(bits_h2(vd[i])));
+              }
+              uint32_t bad[2] = {0u, 0u};
+              const uint32_t cb = h2_bits(check);
+              if ((cb & 0x7c00u) == 0x7c00u || (cb & 0x7c000000u) == 0x7c000000u) {  // a NaN scale, or large ones
 #pragma unroll
-              for (int b = 0; b < NB; ++b) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[b];
-            }
+                for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              const uint32_t sel = odd ? (b & 1 ? 0x3276u : 0x1054u) : (b & 1 ? 0x7632u : 0x5410u);
-              uint32_t o[4][4];
-#pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                const uint32_t x = __byte_perm(vw[2 * p][b >> 1], vw[2 * p + 1][b >> 1], sel), y = x >> 8;
-                const __half2 dd = bits_h2(__byte_perm(vd[2 * p][b >> 1], vd[2 * p + 1][b >> 1], sel));
-                o[0][p] = h2_bits(__hmul2(code_lo(x), dd)), o[1][p] = h2_bits(__hmul2(code_hi(x), dd));
-                o[2][p] = h2_bits(__hmul2(code_lo(y), dd)), o[3][p] = h2_bits(__hmul2(code_hi(y), dd));
+                  for (int h = 0; h < 2; ++h)
+                    if ((vd[i] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
+                      bad[h] |= 1u << (i ^ odd);
+                      vd[i] &= ~(0xffffu << (16 * h));
+                    }
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int e = 32 * b + 4 * g + i;
-                *reinterpret_cast<uint4 *>(vt + (m >> 3) * L::kVPanel + e * 128 + (((m & 7) ^ (e & 7)) << 4)) =
-                    make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+              for (int h = 0; h < kTwo; ++h) {
+                const int b = 2 * b2 + h;
+                if (b >= NB) break;
+                if (g == 0) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[h];
+                const uint32_t sel = odd ? (h ? 0x3276u : 0x1054u) : (h ? 0x7632u : 0x5410u);
+                uint32_t o[4][4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  const uint32_t x = __byte_perm(vw[2 * p], vw[2 * p + 1], sel), y = x >> 8;
+                  const __half2 dd = bits_h2(__byte_perm(vd[2 * p], vd[2 * p + 1], sel));
+                  o[0][p] = h2_bits(__hmul2(code_lo(x), dd)), o[1][p] = h2_bits(__hmul2(code_hi(x), dd));
+                  o[2][p] = h2_bits(__hmul2(code_lo(y), dd)), o[3][p] = h2_bits(__hmul2(code_hi(y), dd));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int e = 32 * b + 4 * g + i;
+                  *reinterpret_cast<uint4 *>(vt + (m >> 3) * L::kVPanel + e * 128 + (((m & 7) ^ (e & 7)) << 4)) =
+                      make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                }
               }
             }
           }
