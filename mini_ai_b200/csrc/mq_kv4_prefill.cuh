@@ -169,8 +169,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     __syncthreads();
     sm100::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // Waits sleep in the barrier: polling took as many issue slots as the work.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-      return sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs);
+      return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, kKv4WaitNs);
     };
     // Steps of a segment that some row sees.
     auto steps_of = [&](const Kv4Segment &s) {
