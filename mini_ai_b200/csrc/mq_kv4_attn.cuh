@@ -86,17 +86,23 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4AttnArgs &a, int r) {
   return q;
 }
 
-// A walk along this CTA's piece of the line.
+// Work of row tile i.
+template <int RT, int BN>
+__device__ __forceinline__ int kv4_tile_work(const Kv4Request &q, int group, int i) {
+  return (max(q.base, 0) + BN - 1) / BN + 1 + i / (group * (BN / RT));
+}
+
+// A walk along this CTA's piece of the line: the item it stands in, and what is left.
 struct Kv4Walk {
-  int r;                // request at the current place
-  int loaded;           // the request in the segment
-  int64_t at;           // place within it
+  Kv4Request q;
+  int r, head, tile;    // request, KV head, row tile
+  int t, whole;         // BN-token tiles of the item behind this place, and all of them
   int64_t left;         // work left to this CTA
   int64_t line, place;  // the whole line, and the current place on it
   int ctas;             // pieces
 };
 
-// All threads; two block-wide scans. false: no work for this CTA.
+// All threads; a block-wide scan. false: no work for this CTA.
 template <int RT, int BN>
 __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
   __shared__ int64_t sums[32], s_at;
@@ -122,7 +128,19 @@ __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
     s_r = r, s_at = at;
   }
   __syncthreads();
-  w.r = s_r, w.at = s_at, w.loaded = -1;
+  w.r = s_r;
+  w.q = kv4_request<RT, BN>(a, w.r);
+  w.head = (int)quotient(s_at, w.q.work);
+  const int64_t in_head = s_at - w.head * w.q.work;
+  int lo = 0, hi = w.q.tiles - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (kv4_work<RT, BN>(w.q.base, a.group, mid + 1) > in_head) hi = mid;
+    else lo = mid + 1;
+  }
+  w.tile = lo;
+  w.t = (int)(in_head - kv4_work<RT, BN>(w.q.base, a.group, lo));
+  w.whole = kv4_tile_work<RT, BN>(w.q, a.group, lo);
   return true;
 }
 
@@ -137,27 +155,24 @@ struct Kv4Segment {
 template <int RT, int BN>
 __device__ __forceinline__ bool kv4_next(const Kv4AttnArgs &a, Kv4Walk &w, Kv4Segment &s) {
   if (w.left == 0) return false;
-  for (;; ++w.r) {
-    if (w.loaded != w.r) s.q = kv4_request<RT, BN>(a, w.r), w.loaded = w.r;
-    if (w.at < a.c.kv * s.q.work) break;
-    w.at -= a.c.kv * s.q.work;
+  if (w.t == w.whole) {
+    w.t = 0;
+    if (++w.tile == w.q.tiles) {
+      w.tile = 0;
+      if (++w.head == a.c.kv) {
+        w.head = 0;
+        do w.q = kv4_request<RT, BN>(a, ++w.r);
+        while (w.q.work == 0);
+      }
+    }
+    w.whole = kv4_tile_work<RT, BN>(w.q, a.group, w.tile);
   }
-  s.r = w.r;
-  s.head = (int)quotient(w.at, s.q.work);
-  const int64_t in_head = w.at - s.head * s.q.work;
-  int lo = 0, hi = s.q.tiles - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (kv4_work<RT, BN>(s.q.base, a.group, mid + 1) > in_head) hi = mid;
-    else lo = mid + 1;
-  }
-  s.tile = lo;
-  const int64_t before = kv4_work<RT, BN>(s.q.base, a.group, lo);
-  s.whole = (int)(kv4_work<RT, BN>(s.q.base, a.group, lo + 1) - before);
-  s.t0 = (int)(in_head - before);
-  s.t1 = (int)min((int64_t)s.whole, s.t0 + w.left);
+  s.q = w.q;
+  s.r = w.r, s.head = w.head, s.tile = w.tile;
+  s.t0 = w.t, s.whole = w.whole;
+  s.t1 = (int)min((int64_t)w.whole, w.t + w.left);
   const int n = s.t1 - s.t0;
-  w.at += n, w.left -= n, w.place += n;
+  w.t = s.t1, w.left -= n, w.place += n;
   return true;
 }
 

@@ -5,7 +5,7 @@
 // Per step, with Q and P as fp16 hi + lo pairs (22 bits) in TMEM and the
 // cache's values, exact in fp16, in shared memory:
 //   S = Qhi K^T + Qlo K^T            [128 rows, 128 tokens], fp32 in TMEM
-//   P = 2^(S f - ref) -> Phi, Plo    one thread a row and half of the columns
+//   P = 2^(S f - ref) -> Phi, Plo    one thread a row and quarter of the columns
 //   O = Phi V + Plo V                [128 rows, hd], fp32 in TMEM
 // and the running output of a row is in its threads' registers: adding one
 // step's O there costs hd additions a row, keeps every tensor-core sum at 16
@@ -13,15 +13,14 @@
 // Both A operands come from TMEM, so shared memory feeds the tensor cores
 // with B alone (64 of its 128 bytes a clock).
 //
-// Warps: 0-3 and 4-7 softmax (token halves of a step; each half of the
-// output's columns), 8-11 decode (packed units -> swizzled K and V tiles),
-// 12 issues the MMAs, 13 the copies of the packed units.
+// Warps: 0-15 softmax (a thread: one row, a quarter of a step's tokens and of
+// the output's columns), 16-19 decode K and 20-23 V (packed units -> swizzled
+// tiles), 24 issues the MMAs, 25 the copies of the packed units.
 // S of step i + 1 is computed while the softmax of step i runs, and O of step
 // i during the softmax of step i + 1.
 //
 // Bound: the tensor cores. Twice 4 hd operations a (row, token) pair (hi and
-// lo) against 1.67 PFLOP/s; the softmax costs about 1100 of a step's 2048
-// issue slots.
+// lo) against 1.67 PFLOP/s.
 #pragma once
 
 #include "mq_kv4_attn.cuh"
@@ -30,7 +29,8 @@ namespace mq {
 
 constexpr int kPreRows = 128;    // RT
 constexpr int kPreTokens = 128;  // BN
-constexpr int kPreThreads = 512;
+constexpr int kPreThreads = 896;
+constexpr int kPreSoft = 512;    // softmax threads
 constexpr int kPreRaw = 3;       // packed steps in flight
 constexpr int kPreStages = 2;    // K and V tiles
 constexpr int kPreMasks = 4;
@@ -48,8 +48,8 @@ struct PreSmem {
   static constexpr int kKOff = 0;
   static constexpr int kVOff = kPreStages * kK;
   static constexpr int kRawOff = kVOff + kPreStages * kV;
-  static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][2 halves][128 rows]
-  static constexpr int kNanOff = kXchOff + 2 * 2 * kPreRows * 4;  // bytes [masks][NB][16 token groups]
+  static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][4 quarters][128 rows]
+  static constexpr int kNanOff = kXchOff + 2 * 4 * kPreRows * 4;  // bytes [masks][NB][16 token groups]
   static constexpr int kBarOff = kNanOff + kPreMasks * NB * 16;
   static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 6;
   static constexpr int kBytes = kBarOff + 8 * kBars + 64;
@@ -86,7 +86,11 @@ __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t *r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) { sm100::tmem_ld_32x32b_x32(addr, r); }
+__device__ __forceinline__ void tm_ld8(uint32_t addr, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -109,8 +113,7 @@ template <int N>
 __device__ __forceinline__ void set_regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
-// The 256 softmax threads.
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPreSoft) : "memory"); }
 
 // A place in a ring of N barriers, and the parity of its current pass.
 template <int N>
@@ -142,14 +145,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&raw_full[i], 1), sm100::mbar_init(&raw_empty[i], 128);
+    for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&raw_full[i], 1), sm100::mbar_init(&raw_empty[i], 256);
     for (int i = 0; i < kPreStages; ++i) {
       sm100::mbar_init(&k_full[i], 128), sm100::mbar_init(&k_empty[i], 1);
       sm100::mbar_init(&v_full[i], 128), sm100::mbar_init(&v_empty[i], 1);
     }
-    sm100::mbar_init(q_full, 256);
+    sm100::mbar_init(q_full, kPreSoft);
     sm100::mbar_init(&s_full[0], 1), sm100::mbar_init(&s_full[1], 1);
-    sm100::mbar_init(p_full, 256);
+    sm100::mbar_init(p_full, kPreSoft);
     sm100::mbar_init(o_full, 1);
     sm100::mbar_init(fin, 1);
     *abort = 0;
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   Kv4Walk walk;
   const bool work = kv4_walk<kPreRows, kPreTokens>(a, walk);
   if (work) {
-    if (warp == 12) {
+    if (warp == 24) {
       sm100::tmem_alloc(tmem_slot, 512);
       sm100::tmem_relinquish();
     }
@@ -181,40 +184,45 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     };
     Kv4Segment s;
 
-    if (warp < 8) {
+    if (warp < 16) {
       // -------------------------------------------------------- softmax
-      set_regs_up<176>();
-      const int half = warp >> 2, row = 32 * (warp & 3) + lane;
+      set_regs_up<80>();
+      const int qr = warp >> 2, row = 32 * (warp & 3) + lane;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
       uint32_t o_phase = 0;
       Ring<2> score;
       Ring<kPreMasks> mask, smask;  // of the output's and of the scores' step
       int parity = 0;               // of the exchange buffers
       bool ok = true;
-      auto exchange = [&](float mine) {  // the other half's value of this row
-        float *x = xch + parity * 2 * kPreRows;
-        x[half * kPreRows + row] = mine;
+      // The four quarters' values of this row, by `join`.
+      auto exchange = [&](float mine, auto join) {
+        float *x = xch + parity * 4 * kPreRows + row;
+        x[qr * kPreRows] = mine;
         softmax_sync();
         parity ^= 1;
-        return x[(half ^ 1) * kPreRows + row];
+        return join(join(x[0], x[kPreRows]), join(x[2 * kPreRows], x[3 * kPreRows]));
       };
+      auto larger = [](float x, float y) { return fmaxf(x, y); };
+      auto plus = [](float x, float y) { return x + y; };
+      auto either = [](float x, float y) { return __uint_as_float(__float_as_uint(x) | __float_as_uint(y)); };
+      constexpr int QC = HD / 4;  // elements and output columns of a quarter
       while (kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
         const int steps = steps_of(s);
         const int f = s.tile * kPreRows + row, qi = f / a.group;
         const bool real = f < s.q.flat;
         const int last = real ? min(s.q.base + qi, s.q.len - 1) : -1;
-        float acc[HD / 2];
+        float acc[QC];
 #pragma unroll
-        for (int i = 0; i < HD / 2; ++i) acc[i] = 0.0f;
+        for (int i = 0; i < QC; ++i) acc[i] = 0.0f;
         float ref = -INFINITY, sum = 0.0f;
         uint32_t poison = 0;
         if (steps > 0) {
-          // ---- this half of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
-          float x[HD / 2], mx = 0.0f;
+          // ---- this quarter of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
+          float x[QC], mx = 0.0f;
           const float *p = a.q + (int64_t)(s.q.row0 + qi) * a.ld_q +
-                           (int64_t)(s.head * a.group + f % a.group) * a.hs_q + half * (HD / 2);
+                           (int64_t)(s.head * a.group + f % a.group) * a.hs_q + qr * QC;
 #pragma unroll
-          for (int i = 0; i < HD / 2; i += 4) {
+          for (int i = 0; i < QC; i += 4) {
             if (!real) {
               x[i] = x[i + 1] = x[i + 2] = x[i + 3] = 0.0f;
             } else if (a.vec_q) {
@@ -226,9 +234,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           }
           bool bad = false;
 #pragma unroll
-          for (int i = 0; i < HD / 2; ++i) mx = fmaxf(mx, fabsf(x[i])), bad |= !isfinite(x[i]);
+          for (int i = 0; i < QC; ++i) mx = fmaxf(mx, fabsf(x[i])), bad |= !isfinite(x[i]);
           if (bad) mx = INFINITY;
-          mx = fmaxf(mx, exchange(mx));
+          mx = exchange(mx, larger);
           bad = mx == INFINITY;
           const int e = min(141 - (int)(__float_as_uint(mx) >> 23), 126);
           float up = __uint_as_float((uint32_t)(127 + e) << 23);
@@ -236,11 +244,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           // (never 0, so that f * -inf is -inf; a row that sees nothing is 0 whatever its query)
           const float scale = bad && last >= 0 ? __uint_as_float(0x7fc00000u) : fmaxf(ldexpf(fabsf(a.scale), -e), 1.2e-38f);
 #pragma unroll
-          for (int c = 0; c < HD / 16; ++c) {  // 8 elements, in the order of a decoded word
+          for (int c = 0; c < QC / 8; ++c) {  // 8 elements, in the order of a decoded word
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) split_f16(x[8 * c + i] * up, x[8 * c + i + 4] * up, hi[i], lo[i]);
-            const uint32_t col = half * (HD / 4) + 4 * c;
+            const uint32_t col = qr * (QC / 2) + 4 * c;
             tm_st4(lanes + kTmQ + col, hi[0], hi[1], hi[2], hi[3]);
             tm_st4(lanes + kTmQ + 64 + col, lo[0], lo[1], lo[2], lo[3]);
           }
@@ -253,42 +261,42 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             o_phase ^= 1u;
             sm100::tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < HD / 2; c += 16) {
-              uint32_t r[16];
-              tm_ld16(lanes + kTmO + half * (HD / 2) + c, r);
+            for (int c = 0; c < QC; c += 8) {
+              uint32_t r[8];
+              tm_ld8(lanes + kTmO + qr * QC + c, r);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) acc[c + i] += __uint_as_float(r[i]);
+              for (int i = 0; i < 8; ++i) acc[c + i] += __uint_as_float(r[i]);
             }
             // NaN values of the step entered as 0: the rows that see them are marked.
-            const uint64_t *bits = reinterpret_cast<const uint64_t *>(nan_bits + mask.i * NB * 16 + 8 * half);
-            uint64_t any = 0;
+            const uint32_t *bits = reinterpret_cast<const uint32_t *>(nan_bits + mask.i * NB * 16 + 4 * qr);
+            uint32_t any = 0;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) any |= bits[2 * b];
+            for (int b = 0; b < NB; ++b) any |= bits[4 * b];
             if (any) {
-              const int see = last - (s.t0 + k) * kPreTokens - 64 * half;
-              const uint64_t mine = see < 0 ? 0 : see >= 63 ? ~0ull : (2ull << see) - 1;
+              const int see = last - (s.t0 + k) * kPreTokens - 32 * qr;
+              const uint32_t mine = see < 0 ? 0 : see >= 31 ? ~0u : (2u << see) - 1;
 #pragma unroll
               for (int b = 0; b < NB; ++b)
-                if (bits[2 * b] & mine) poison |= 1u << b;
+                if (bits[4 * b] & mine) poison |= 1u << b;
             }
             mask.next();
           };
 
           for (int k = 0; k < steps; ++k) {
             ok = wait(&s_full[score.i], score.phase) && ok;
-            const uint32_t cols = lanes + kTmS + 128 * score.i + 64 * half;
+            const uint32_t cols = lanes + kTmS + 128 * score.i + 32 * qr;
             score.next();
             sm100::tc_fence_after();
-            const uint32_t units = unit_mask[smask.i] >> (4 * half) & 15u;
+            const uint32_t units = unit_mask[smask.i] >> (2 * qr) & 3u;
             smask.next();
-            const int see = last - (s.t0 + k) * kPreTokens - 64 * half;  // columns 0..see
+            const int see = last - (s.t0 + k) * kPreTokens - 32 * qr;  // columns 0..see
             // (Loops of 16 columns keep the instruction cache: unrolled further, the roles' code evicted itself and
             // a step took three times as long.)
             // Hide what the row does not see (TMEM is read and written by whole warps).
-            if (__any_sync(0xffffffffu, see < 63 || units != 15u)) {
+            if (__any_sync(0xffffffffu, see < 31 || units != 3u)) {
 #pragma unroll 1
-              for (int c = 0; c < 64; c += 16) {
+              for (int c = 0; c < 32; c += 16) {
                 uint32_t r[16];
                 tm_ld16(cols + c, r);
                 sm100::tmem_ld_wait();
@@ -301,15 +309,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               tm_st_wait();
             }
             float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 64; c += 32) {
-              uint32_t r[32];
-              tm_ld32(cols + c, r);
+#pragma unroll
+            for (int c = 0; c < 32; c += 16) {
+              uint32_t r[16];
+              tm_ld16(cols + c, r);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+              for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(r[i]));
             }
-            top = fmaxf(top, exchange(top)) * scale;
+            top = exchange(top, larger) * scale;
             float old = 1.0f;
             if (top > ref + 15.0f || (ref == -INFINITY && top > -INFINITY)) {
               const float to = top - 8.0f;
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             }
             const float shift = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll 1
-            for (int c = 0; c < 64; c += 16) {
+            for (int c = 0; c < 32; c += 16) {
               uint32_t r[16], w[16];
               tm_ld16(cols + c, r);
               sm100::tmem_ld_wait();
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             if (k > 0) add_output(k - 1);
             if (__any_sync(0xffffffffu, old != 1.0f)) {
 #pragma unroll
-              for (int i = 0; i < HD / 2; ++i) acc[i] *= old;
+              for (int i = 0; i < QC; ++i) acc[i] *= old;
             }
             tm_st_wait();
             sm100::tc_fence_before();
@@ -344,8 +352,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           add_output(steps - 1);
         }
         // ---- the row's end
-        const float total = sum + exchange(sum);
-        poison |= __float_as_uint(exchange(__uint_as_float(poison)));
+        const float total = exchange(sum, plus);
+        poison = __float_as_uint(exchange(__uint_as_float(poison), either));
         const bool whole = s.t0 == 0 && s.t1 == s.whole;
         if (!ok) poison = ~0u;
         if (real) {
@@ -359,13 +367,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           } else {
             float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kPreRows, HD);
             dst = part + 2 * kPreRows + row * HD;
-            if (half == 0) part[row] = ref, part[kPreRows + row] = total;
+            if (qr == 0) part[row] = ref, part[kPreRows + row] = total;
           }
-          dst += half * (HD / 2);
+          dst += qr * QC;
 #pragma unroll
-          for (int i = 0; i < HD / 2; i += 4) {
+          for (int i = 0; i < QC; i += 4) {
             float4 v = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-            if (poison >> ((half * (HD / 2) + i) / 32) & 1u) {
+            if (poison >> ((qr * QC + i) / 32) & 1u) {
               const float n = __uint_as_float(0x7fc00000u);
               v = make_float4(n, n, n, n);
             }
@@ -378,10 +386,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
         }
       }
-    } else if (warp < 12) {
-      // -------------------------------------------------------- packed units -> K and V tiles
-      set_regs_down<80>();
-      const int dw = warp - 8;
+    } else if (warp < 20) {
+      // -------------------------------------------------------- packed units -> K tiles
+      // A warp takes 8 tokens x 4 chunks at a time, paired so that neither the loads nor the stores meet a bank
+      // twice. Token: 32 it + tk0, whose unit is 2 it + half a warp pair's.
+      const int dw = warp - 16, tk0 = 8 * dw + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tk0 & 15;
+      const int u0 = tk0 >> 4;
+      const uint32_t src0 = L::kRawOff + u0 * UB + tk * (16 * NB) + t * (4 * NB);
+      const uint32_t scale0 = L::kRawOff + u0 * UB + kv4_k_scale_off(NB) + tk * (2 * NB);
+      const uint32_t dst0 = L::kKOff + tk0 * 128 + ((t ^ (lane & 7)) << 4);  // even blocks; odd ones are 64 bytes away
       Ring<kPreRaw> raw;
       Ring<kPreStages> st;
       Ring<kPreMasks> mask;
@@ -391,17 +404,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         for (int k = 0; k < steps; ++k) {
           if (!(ok = wait(&raw_full[raw.i], raw.phase))) break;
           if (!(ok = wait(&k_empty[st.i], st.phase ^ 1u))) break;
-          const uint8_t *src = sm + L::kRawOff + raw.i * L::kRaw;
           const uint32_t valid = raw_valid[raw.i];
-          if (dw == 0 && lane == 0) unit_mask[mask.i] = valid;
-          uint8_t *kt = sm + L::kKOff + st.i * L::kK;
-#pragma unroll 1
+          if (threadIdx.x == 512) unit_mask[mask.i] = valid;
+          const uint8_t *src = sm + src0 + raw.i * L::kRaw, *scale = sm + scale0 + raw.i * L::kRaw;
+          uint8_t *dst = sm + dst0 + st.i * L::kK;
+#pragma unroll 2
           for (int it = 0; it < 4; ++it) {
-            // 8 tokens x 4 chunks a warp, paired so that neither the loads nor the stores meet a bank twice
-            const int tok = 8 * (4 * it + dw) + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tok & 15;
-            const uint8_t *u = src + (tok >> 4) * UB;
             uint32_t kw[NB], d[W];
-            const uint8_t *kp = u + tk * (16 * NB) + t * (4 * NB);
+            const uint8_t *kp = src + it * 2 * UB;
             if constexpr (NB == 4) {
               const uint4 v = *reinterpret_cast<const uint4 *>(kp);
               kw[0] = v.x, kw[1] = v.y, kw[2] = v.z, kw[3] = v.w;
@@ -412,8 +422,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
 #pragma unroll
               for (int b = 0; b < NB; ++b) kw[b] = reinterpret_cast<const uint32_t *>(kp)[b];
             }
-            lds_halves<NB>(u + kv4_k_scale_off(NB) + tk * (2 * NB), d);
-            if (!(valid >> (tok >> 4) & 1u)) {
+            lds_halves<NB>(scale + it * 2 * UB, d);
+            if (!(valid >> (2 * it + u0) & 1u)) {
 #pragma unroll
               for (int i = 0; i < W; ++i) d[i] = 0u;
             }
@@ -424,75 +434,88 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               uint4 o;
               o.x = h2_bits(__hmul2(code_lo(w), dd)), o.y = h2_bits(__hmul2(code_hi(w), dd));
               o.z = h2_bits(__hmul2(code_lo(w8), dd)), o.w = h2_bits(__hmul2(code_hi(w8), dd));
-              *reinterpret_cast<uint4 *>(kt + (b >> 1) * L::kPanel + tok * 128 +
-                                         ((((b & 1) * 4 + t) ^ (tok & 7)) << 4)) = o;
+              uint8_t *p = b & 1 ? sm + ((uint32_t)(dst - sm) ^ 64u) : dst;
+              *reinterpret_cast<uint4 *>(p + (b >> 1) * L::kPanel + it * 32 * 128) = o;
             }
           }
           sm100::fence_proxy_async_smem();
           sm100::mbar_arrive(&k_full[st.i]);
-
+          sm100::mbar_arrive(&raw_empty[raw.i]);
+          raw.next(), st.next(), mask.next();
+        }
+      }
+    } else if (warp < 24) {
+      // -------------------------------------------------------- packed units -> V tiles
+      // A thread takes 8 tokens and 4 elements of every block, two blocks at a time. Odd token groups read their
+      // tokens in pairs swapped, which spares half of the bank conflicts.
+      const int dw = warp - 20, m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
+      const uint32_t src0 = L::kRawOff + (m >> 1) * UB + kv4_v_off(NB) + (8 * odd) * (16 * NB) + g * (2 * NB);
+      const uint32_t scale0 = L::kRawOff + (m >> 1) * UB + kv4_v_scale_off(NB) + (8 * odd) * (2 * NB);
+      const uint32_t dst0 = L::kVOff + (m >> 3) * L::kVPanel + 4 * g * 128;
+      Ring<kPreRaw> raw;
+      Ring<kPreStages> st;
+      Ring<kPreMasks> mask;
+      bool ok = true;
+      while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
+        const int steps = steps_of(s);
+        for (int k = 0; k < steps; ++k) {
+          if (!(ok = wait(&raw_full[raw.i], raw.phase))) break;
           if (!(ok = wait(&v_empty[st.i], st.phase ^ 1u))) break;
-          uint8_t *vt = sm + L::kVOff + st.i * L::kV;
-          {
-            // 8 tokens and, two blocks at a time, 4 elements of a block a thread; odd groups read their tokens in
-            // pairs swapped
-            const int m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
-            const bool have = valid >> (m >> 1) & 1u;
-            const uint8_t *u = src + (m >> 1) * UB + kv4_v_off(NB) + (8 * (m & 1)) * (16 * NB) + g * (2 * NB);
-            const uint8_t *us = src + (m >> 1) * UB + kv4_v_scale_off(NB) + (8 * (m & 1)) * (2 * NB);
+          const bool have = raw_valid[raw.i] >> (m >> 1) & 1u;
+          // tokens 0, 2, 4, 6 and 1, 3, 5, 7 of the group, or the other way round
+          const uint8_t *w0 = sm + src0 + raw.i * L::kRaw + odd * (16 * NB), *w1 = w0 + (1 - 2 * odd) * (16 * NB);
+          const uint8_t *d0 = sm + scale0 + raw.i * L::kRaw + odd * (2 * NB), *d1 = d0 + (1 - 2 * odd) * (2 * NB);
+          uint8_t *dst = sm + dst0 + st.i * L::kV;
 #pragma unroll 1
-            for (int b2 = 0; b2 < W; ++b2) {
-              constexpr int kTwo = NB == 1 ? 1 : 2;
-              uint32_t vw[8], vd[8];
-              __half2 check = __float2half2_rn(0.0f);
+          for (int b2 = 0; b2 < W; ++b2) {
+            uint32_t vw[8], vd[8];
+            __half2 check = __float2half2_rn(0.0f);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint8_t *pw = u + (i ^ odd) * (16 * NB) + 4 * b2, *pd = us + (i ^ odd) * (2 * NB) + 4 * b2;
-                if constexpr (NB % 2 == 0) {
-                  vw[i] = *reinterpret_cast<const uint32_t *>(pw), vd[i] = *reinterpret_cast<const uint32_t *>(pd);
-                } else {  // half-words; a row's last block stands alone
-                  vw[i] = *reinterpret_cast<const uint16_t *>(pw), vd[i] = *reinterpret_cast<const uint16_t *>(pd);
-                  if (2 * b2 + 1 < NB) {
-                    vw[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pw)[1] << 16;
-                    vd[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pd)[1] << 16;
+            for (int i = 0; i < 8; ++i) {
+              const uint8_t *pw = (i & 1 ? w1 : w0) + (i & ~1) * (16 * NB) + 4 * b2;
+              const uint8_t *pd = (i & 1 ? d1 : d0) + (i & ~1) * (2 * NB) + 4 * b2;
+              if constexpr (NB % 2 == 0) {
+                vw[i] = *reinterpret_cast<const uint32_t *>(pw), vd[i] = *reinterpret_cast<const uint32_t *>(pd);
+              } else {  // half-words; a row's last block stands alone
+                vw[i] = *reinterpret_cast<const uint16_t *>(pw), vd[i] = *reinterpret_cast<const uint16_t *>(pd);
+                if (2 * b2 + 1 < NB) {
+                  vw[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pw)[1] << 16;
+                  vd[i] |= (uint32_t)reinterpret_cast<const uint16_t *>(pd)[1] << 16;
+                }
+              }
+              if (!have) vd[i] = 0u;
+              check = __hadd2(check, __habs2(bits_h2(vd[i])));
+            }
+            uint32_t bad[2] = {0u, 0u};
+            const uint32_t cb = h2_bits(check);
+            if ((cb & 0x7c00u) == 0x7c00u || (cb & 0x7c000000u) == 0x7c000000u) {  // a NaN scale, or large ones
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if ((vd[i] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
+                    bad[h] |= 1u << (i ^ odd);
+                    vd[i] &= ~(0xffffu << (16 * h));
                   }
-                }
-                if (!have) vd[i] = 0u;
-                check = __hadd2(check, __habs2(bits_h2(vd[i])));
+            }
+#pragma unroll
+            for (int h = 0; h < (NB == 1 ? 1 : 2); ++h) {
+              const int b = 2 * b2 + h;
+              if (b >= NB) break;
+              if (g == 0) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[h];
+              const uint32_t sel = odd ? (h ? 0x3276u : 0x1054u) : (h ? 0x7632u : 0x5410u);
+              uint32_t o[4][4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                const uint32_t x = __byte_perm(vw[2 * p], vw[2 * p + 1], sel), y = x >> 8;
+                const __half2 dd = bits_h2(__byte_perm(vd[2 * p], vd[2 * p + 1], sel));
+                o[0][p] = h2_bits(__hmul2(code_lo(x), dd)), o[1][p] = h2_bits(__hmul2(code_hi(x), dd));
+                o[2][p] = h2_bits(__hmul2(code_lo(y), dd)), o[3][p] = h2_bits(__hmul2(code_hi(y), dd));
               }
-              uint32_t bad[2] = {0u, 0u};
-              const uint32_t cb = h2_bits(check);
-              if ((cb & 0x7c00u) == 0x7c00u || (cb & 0x7c000000u) == 0x7c000000u) {  // a NaN scale, or large ones
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h)
-                    if ((vd[i] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
-                      bad[h] |= 1u << (i ^ odd);
-                      vd[i] &= ~(0xffffu << (16 * h));
-                    }
-              }
-#pragma unroll
-              for (int h = 0; h < kTwo; ++h) {
-                const int b = 2 * b2 + h;
-                if (b >= NB) break;
-                if (g == 0) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[h];
-                const uint32_t sel = odd ? (h ? 0x3276u : 0x1054u) : (h ? 0x7632u : 0x5410u);
-                uint32_t o[4][4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                  const uint32_t x = __byte_perm(vw[2 * p], vw[2 * p + 1], sel), y = x >> 8;
-                  const __half2 dd = bits_h2(__byte_perm(vd[2 * p], vd[2 * p + 1], sel));
-                  o[0][p] = h2_bits(__hmul2(code_lo(x), dd)), o[1][p] = h2_bits(__hmul2(code_hi(x), dd));
-                  o[2][p] = h2_bits(__hmul2(code_lo(y), dd)), o[3][p] = h2_bits(__hmul2(code_hi(y), dd));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int e = 32 * b + 4 * g + i;
-                  *reinterpret_cast<uint4 *>(vt + (m >> 3) * L::kVPanel + e * 128 + (((m & 7) ^ (e & 7)) << 4)) =
-                      make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                }
-              }
+              for (int i = 0; i < 4; ++i)  // element 32 b + 4 g + i
+                *reinterpret_cast<uint4 *>(dst + (32 * b + i) * 128 + (((m & 7) ^ (4 * (g & 1) + i)) << 4)) =
+                    make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
             }
           }
           sm100::fence_proxy_async_smem();
@@ -502,8 +525,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
       }
     } else {
-      set_regs_down<80>();
-      if (warp == 12 && lane == 0) {
+      set_regs_down<40>();
+      if (warp == 24 && lane == 0) {
         // ------------------------------------------------------ MMA issue
         constexpr uint32_t id_s = idesc_half_f32(kPreRows, kPreTokens), id_o = idesc_half_f32(kPreRows, HD);
         Ring<kPreStages> ks, vs;
@@ -553,7 +576,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
         sm100::umma_commit(fin);  // every MMA has completed before the TMEM is released
         sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
-      } else if (warp == 13) {
+      } else if (warp == 25) {
         // ------------------------------------------------------ copies of the packed units
         const int upp = a.c.page / kKv4Unit;
         const int64_t unit_page = a.c.page_head_bytes * a.c.kv;
@@ -591,7 +614,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     __syncwarp();
     sm100::tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 24) {
       sm100::tc_fence_after();
       sm100::tmem_dealloc(tmem, 512);
     }
