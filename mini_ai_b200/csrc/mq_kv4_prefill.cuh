@@ -105,6 +105,17 @@ __device__ __forceinline__ void tm_st4(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t leader;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(leader));
+  return leader != 0;
+}
+
 template <int N>
 __device__ __forceinline__ void set_regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -143,7 +154,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   float *xch = reinterpret_cast<float *>(sm + L::kXchOff);
   uint8_t *nan_bits = sm + L::kNanOff;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&raw_full[i], 1), sm100::mbar_init(&raw_empty[i], 256);
     for (int i = 0; i < kPreStages; ++i) {
@@ -171,7 +182,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     sm100::tc_fence_before();
     __syncthreads();
     sm100::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Waits sleep in the barrier: polling took as many issue slots as the work.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, kKv4WaitNs);
@@ -526,31 +537,43 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       }
     } else {
       set_regs_down<40>();
-      if (warp == 24 && lane == 0) {
+      if (warp == 24) {
         // ------------------------------------------------------ MMA issue
+        // The whole warp walks and waits, one lane issues: operands computed by whole warps stay in uniform
+        // registers, where the instruction wants them (from one lane's registers an MMA took 95 clocks to issue,
+        // and 64 to run).
         constexpr uint32_t id_s = idesc_half_f32(kPreRows, kPreTokens), id_o = idesc_half_f32(kPreRows, HD);
+        const uint64_t k_desc = sm100::umma_desc_sw128(sm100::smem_u32(sm + L::kKOff));
+        const uint64_t v_desc = sm100::umma_desc_sw128(sm100::smem_u32(sm + L::kVOff));
         Ring<kPreStages> ks, vs;
         uint32_t q_phase = 0, p_phase = 0;
         int sb = 0, pb = 0;  // S buffers of the next scores and of the next output
         bool ok = true;
+        auto all_wait = [&](uint64_t *bar, uint32_t parity) {
+          return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs)) != 0;
+        };
         while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
           const int steps = steps_of(s);
           if (steps == 0) continue;
-          if (!(ok = wait(q_full, q_phase))) break;
+          if (!(ok = all_wait(q_full, q_phase))) break;
           q_phase ^= 1u;
           // S of a step may replace the P of two steps before: the MMAs of one thread run in order.
           auto scores = [&]() {
-            if (!wait(&k_full[ks.i], ks.phase)) return false;
+            if (!all_wait(&k_full[ks.i], ks.phase)) return false;
             sm100::tc_fence_after();
-            const uint32_t base = sm100::smem_u32(sm + L::kKOff + ks.i * L::kK);
+            const uint64_t desc = k_desc + (uint64_t)(ks.i * (L::kK >> 4));
+            const uint32_t d = tmem + kTmS + 128 * sb;
+            if (elect_one()) {
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+              for (int part = 0; part < 2; ++part)
 #pragma unroll
-              for (int kk = 0; kk < 2 * NB; ++kk)
-                umma_f16_ts(tmem + kTmS + 128 * sb, tmem + kTmQ + 64 * part + 8 * kk,
-                            sm100::umma_desc_sw128(base + (kk >> 2) * L::kPanel) + 2 * (kk & 3), id_s, part || kk);
-            sm100::umma_commit(&s_full[sb]);
-            sm100::umma_commit(&k_empty[ks.i]);
+                for (int kk = 0; kk < 2 * NB; ++kk)
+                  umma_f16_ts(d, tmem + kTmQ + 64 * part + 8 * kk, desc + (kk >> 2) * (L::kPanel >> 4) + 2 * (kk & 3),
+                              id_s, part || kk);
+              sm100::umma_commit(&s_full[sb]);
+              sm100::umma_commit(&k_empty[ks.i]);
+            }
+            __syncwarp();
             ks.next();
             sb ^= 1;
             return true;
@@ -558,24 +581,30 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           if (!(ok = scores())) break;
           for (int k = 0; k < steps; ++k) {
             if (k + 1 < steps && !(ok = scores())) break;
-            if (!(ok = wait(&v_full[vs.i], vs.phase) && wait(p_full, p_phase))) break;
+            if (!(ok = all_wait(&v_full[vs.i], vs.phase) && all_wait(p_full, p_phase))) break;
             p_phase ^= 1u;
             sm100::tc_fence_after();
-            const uint32_t base = sm100::smem_u32(sm + L::kVOff + vs.i * L::kV);
+            const uint64_t desc = v_desc + (uint64_t)(vs.i * (L::kV >> 4));
+            const uint32_t p = tmem + kTmS + 128 * pb;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kPreTokens / 16; ++kk)
+              for (int kk = 0; kk < kPreTokens / 16; ++kk)
 #pragma unroll
-              for (int part = 0; part < 2; ++part)
-                umma_f16_ts(tmem + kTmO, tmem + kTmS + 128 * pb + 16 * kk + 8 * part,
-                            sm100::umma_desc_sw128(base + (kk >> 2) * L::kVPanel) + 2 * (kk & 3), id_o, part || kk);
-            sm100::umma_commit(o_full);
-            sm100::umma_commit(&v_empty[vs.i]);
+                for (int part = 0; part < 2; ++part)
+                  umma_f16_ts(tmem + kTmO, p + 16 * kk + 8 * part,
+                              desc + (kk >> 2) * (L::kVPanel >> 4) + 2 * (kk & 3), id_o, part || kk);
+              sm100::umma_commit(o_full);
+              sm100::umma_commit(&v_empty[vs.i]);
+            }
+            __syncwarp();
             vs.next();
             pb ^= 1;
           }
         }
-        sm100::umma_commit(fin);  // every MMA has completed before the TMEM is released
-        sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
+        if (elect_one()) {  // every MMA has completed before the TMEM is released
+          sm100::umma_commit(fin);
+          sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
+        }
       } else if (warp == 25) {
         // ------------------------------------------------------ copies of the packed units
         const int upp = a.c.page / kKv4Unit;
