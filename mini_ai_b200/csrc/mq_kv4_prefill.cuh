@@ -5,7 +5,7 @@
 // Per step, with Q and P as fp16 hi + lo pairs (22 bits) in TMEM and the
 // cache's values, exact in fp16, in shared memory:
 //   S = Qhi K^T + Qlo K^T            [128 rows, 128 tokens], fp32 in TMEM
-//   P = 2^(S f - ref) -> Phi, Plo    one thread a row and quarter of the columns
+//   P = 2^(S f - ref) -> Phi, Plo    one thread a row and half of the columns
 //   O = Phi V + Plo V                [128 rows, hd], fp32 in TMEM
 // and the running output of a row is in its threads' registers: adding one
 // step's O there costs hd additions a row, keeps every tensor-core sum at 16
@@ -13,9 +13,10 @@
 // Both A operands come from TMEM, so shared memory feeds the tensor cores
 // with B alone (64 of its 128 bytes a clock).
 //
-// Warps: 0-15 softmax (a thread: one row, a quarter of a step's tokens and of
-// the output's columns), 16-19 decode K and 20-23 V (packed units -> swizzled
-// tiles), 24 issues the MMAs, 25 the copies of the packed units.
+// Warps: 0-7 softmax (a thread: one row, half of a step's tokens and of the
+// output's columns), 8-11 decode K and 12-15 V (packed units -> swizzled
+// tiles), 16 issues the MMAs, 17 the copies of the packed units, 18 walks the
+// items and hands their segments to the others through a ring.
 // S of step i + 1 is computed while the softmax of step i runs, and O of step
 // i during the softmax of step i + 1.
 //
@@ -29,13 +30,27 @@ namespace mq {
 
 constexpr int kPreRows = 128;    // RT
 constexpr int kPreTokens = 128;  // BN
-constexpr int kPreThreads = 896;
-constexpr int kPreSoft = 512;    // softmax threads
+constexpr int kPreSoft = 256;      // softmax threads
+constexpr int kPreThreads = kPreSoft + 384;
+constexpr int kPreGroups = kPreSoft / kPreRows;      // threads of a row
+constexpr int kPreCols = kPreTokens / kPreGroups;    // of S a thread
+constexpr int kWarpK = kPreSoft / 32, kWarpV = kWarpK + 4, kWarpMma = kWarpV + 4, kWarpCopy = kWarpMma + 1,
+              kWarpWalk = kWarpMma + 2;
 constexpr int kPreRaw = 3;       // packed steps in flight
 constexpr int kPreStages = 2;    // K and V tiles
 constexpr int kPreMasks = 4;
+constexpr int kPreSegs = 4;
 constexpr int kPreUnits = kPreTokens / kKv4Unit;
 constexpr uint64_t kPreDrainNs = 20000000ull;
+
+// A segment as the roles need it.
+enum { kSegEnd = 0, kSegWhole = 1, kSegTail = 2, kSegHead = 3 };  // of an item: all, a later part, its first part
+struct PreSegment {
+  int kind;
+  int row0, flat, base, len;  // Kv4Request
+  int request, head, tile;
+  int t0, steps;              // first step, and the steps that some row sees
+};
 
 template <int NB>
 struct PreSmem {
@@ -48,11 +63,13 @@ struct PreSmem {
   static constexpr int kKOff = 0;
   static constexpr int kVOff = kPreStages * kK;
   static constexpr int kRawOff = kVOff + kPreStages * kV;
-  static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][4 quarters][128 rows]
-  static constexpr int kNanOff = kXchOff + 2 * 4 * kPreRows * 4;  // bytes [masks][NB][16 token groups]
-  static constexpr int kBarOff = kNanOff + kPreMasks * NB * 16;
-  static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 6;
-  static constexpr int kBytes = kBarOff + 8 * kBars + 64;
+  static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][groups][128 rows]
+  static constexpr int kNanOff = kXchOff + 2 * kPreGroups * kPreRows * 4;  // bytes [masks][NB][16 token groups]
+  static constexpr int kStageRow = HD / kPreGroups * 4 + 16;   // a thread's part of a row; rows 4 banks apart
+  static constexpr int kStageOff = kNanOff + kPreMasks * NB * 16;  // 16 rows a softmax warp
+  static constexpr int kBarOff = kStageOff + kPreSoft / 32 * 16 * kStageRow;
+  static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 6 + 2 * kPreSegs;
+  static constexpr int kBytes = kBarOff + 8 * kBars + 64 + 16 * kPreSegs / 4 + kPreSegs * (int)sizeof(PreSegment);
   static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
   static_assert(kAlloc <= 227 * 1024, "shared memory");
   static_assert(kK % 1024 == 0 && kVPanel % 1024 == 0 && kBarOff % 8 == 0, "swizzle atoms and barriers");
@@ -86,11 +103,6 @@ __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t *r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void tm_ld8(uint32_t addr, uint32_t *r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
-}
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -104,6 +116,38 @@ __device__ __forceinline__ void tm_st4(uint32_t addr, uint32_t a, uint32_t b, ui
                : "memory");
 }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Pairs of floats in one instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 of_two(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ float max_three(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
@@ -146,11 +190,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   uint64_t *k_full = raw_empty + kPreRaw, *k_empty = k_full + kPreStages;
   uint64_t *v_full = k_empty + kPreStages, *v_empty = v_full + kPreStages;
   uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 1,
-           *fin = o_full + 1;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fin + 1);
+           *fin = o_full + 1, *seg_full = fin + 1, *seg_empty = seg_full + kPreSegs;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + kPreSegs);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   uint32_t *raw_valid = tmem_slot + 2;   // [kPreRaw]: the packed units that were copied
   uint32_t *unit_mask = raw_valid + kPreRaw;  // [kPreMasks]: the same, for the softmax
+  volatile uint32_t *nan_step = unit_mask + kPreMasks;  // [kPreMasks]: the last step in this place that had NaN values
+  volatile int *soft_kind = reinterpret_cast<volatile int *>(const_cast<uint32_t *>(nan_step) + kPreMasks);
+  PreSegment *segs = reinterpret_cast<PreSegment *>(const_cast<int *>(soft_kind) + 1);
   float *xch = reinterpret_cast<float *>(sm + L::kXchOff);
   uint8_t *nan_bits = sm + L::kNanOff;
 
@@ -166,16 +213,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     sm100::mbar_init(p_full, kPreSoft);
     sm100::mbar_init(o_full, 1);
     sm100::mbar_init(fin, 1);
+    for (int i = 0; i < kPreSegs; ++i) sm100::mbar_init(&seg_full[i], 1), sm100::mbar_init(&seg_empty[i], 11);
     *abort = 0;
+    for (int i = 0; i < kPreMasks; ++i) nan_step[i] = ~0u;
     sm100::fence_mbar_init();
   }
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
-  if (threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
+  if (threadIdx.x == kWarpWalk * 32) a.meta[2 * blockIdx.x + 1].x = 0;  // the walker's
   Kv4Walk walk;
   const bool work = kv4_walk<kPreRows, kPreTokens>(a, walk);
   if (work) {
-    if (warp == 24) {
+    if (warp == kWarpMma) {
       sm100::tmem_alloc(tmem_slot, 512);
       sm100::tmem_relinquish();
     }
@@ -187,61 +236,97 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, kKv4WaitNs);
     };
-    // Steps of a segment that some row sees.
-    auto steps_of = [&](const Kv4Segment &s) {
-      const int f = min((s.tile + 1) * kPreRows, s.q.flat) - 1;
-      const int last = min(s.q.base + f / a.group, s.q.len - 1);
-      return max(0, min(s.t1, (last + kPreTokens) / kPreTokens) - s.t0);
+    Ring<kPreSegs> sg;
+    // The next segment of a role's warp; false at the end. seg_done() lets the walker reuse its place.
+    auto seg_next = [&]() {
+      return __all_sync(0xffffffffu, wait(&seg_full[sg.i], sg.phase)) && segs[sg.i].kind != kSegEnd;
     };
-    Kv4Segment s;
+    auto seg_done = [&]() {
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&seg_empty[sg.i]);
+      sg.next();
+    };
 
-    if (warp < 16) {
+    if (warp < kWarpK) {
       // -------------------------------------------------------- softmax
-      set_regs_up<80>();
-      const int qr = warp >> 2, row = 32 * (warp & 3) + lane;
+      set_regs_up<152>();
+      const int grp = warp >> 2, row = 32 * (warp & 3) + lane;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
       uint32_t o_phase = 0;
       Ring<2> score;
+      uint8_t *stage = sm + L::kStageOff + warp * 16 * L::kStageRow;
+      uint32_t step = 0;  // of this CTA, counted by the decode warps alike
       Ring<kPreMasks> mask, smask;  // of the output's and of the scores' step
       int parity = 0;               // of the exchange buffers
       bool ok = true;
-      // The four quarters' values of this row, by `join`.
+      // The values of this row's threads, by `join`.
       auto exchange = [&](float mine, auto join) {
-        float *x = xch + parity * 4 * kPreRows + row;
-        x[qr * kPreRows] = mine;
+        float *x = xch + parity * kPreGroups * kPreRows + row;
+        x[grp * kPreRows] = mine;
         softmax_sync();
         parity ^= 1;
-        return join(join(x[0], x[kPreRows]), join(x[2 * kPreRows], x[3 * kPreRows]));
+        return join(x[0], x[kPreRows]);
       };
       auto larger = [](float x, float y) { return fmaxf(x, y); };
       auto plus = [](float x, float y) { return x + y; };
       auto either = [](float x, float y) { return __uint_as_float(__float_as_uint(x) | __float_as_uint(y)); };
-      constexpr int QC = HD / 4;  // elements and output columns of a quarter
-      while (kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
-        const int steps = steps_of(s);
-        const int f = s.tile * kPreRows + row, qi = f / a.group;
-        const bool real = f < s.q.flat;
-        const int last = real ? min(s.q.base + qi, s.q.len - 1) : -1;
-        float acc[QC];
+      constexpr int QC = HD / kPreGroups;  // elements and output columns of a thread
+      static_assert(kPreGroups == 2, "");
+      for (;;) {
+        // One warp waits for the segment and decides for all, whatever comes: they share barriers.
+        if (warp == 0) {
+          const bool got = wait(&seg_full[sg.i], sg.phase);
+          if (lane == 0) *soft_kind = got ? segs[sg.i].kind : (int)kSegEnd;
+        }
+        softmax_sync();
+        const int kind = *soft_kind;
+        if (kind == kSegEnd) break;
+        const PreSegment &s = segs[sg.i];
+        const int steps = s.steps, f = s.tile * kPreRows + row, qi = f / a.group;
+        const bool real = f < s.flat;
+        // The last token that the row sees, from the first of this thread's.
+        int see = (real ? min(s.base + qi, s.len - 1) : -1) - s.t0 * kPreTokens - kPreCols * grp;
+        const bool sees = real && min(s.base + qi, s.len - 1) >= 0;
+        const int64_t out_row = s.row0 + qi, head = s.head * a.group + f % a.group;
+        uint64_t acc[QC / 2], sums = 0;  // pairs; two sums of the weights
 #pragma unroll
-        for (int i = 0; i < QC; ++i) acc[i] = 0.0f;
-        float ref = -INFINITY, sum = 0.0f;
+        for (int i = 0; i < QC / 2; ++i) acc[i] = 0;
+        float ref = -INFINITY;
         uint32_t poison = 0;
         if (steps > 0) {
-          // ---- this quarter of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
+          // ---- the thread's part of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
           float x[QC], mx = 0.0f;
-          const float *p = a.q + (int64_t)(s.q.row0 + qi) * a.ld_q +
-                           (int64_t)(s.head * a.group + f % a.group) * a.hs_q + qr * QC;
+          const float *p = real ? a.q + out_row * a.ld_q + head * a.hs_q + grp * QC : nullptr;
+          // Read along the rows and handed out by row, 16 rows at a time.
+          float4 v[QC / 4];
 #pragma unroll
-          for (int i = 0; i < QC; i += 4) {
-            if (!real) {
-              x[i] = x[i + 1] = x[i + 2] = x[i + 3] = 0.0f;
-            } else if (a.vec_q) {
-              const float4 v = *reinterpret_cast<const float4 *>(p + i);
-              x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-            } else {
-              x[i] = p[i], x[i + 1] = p[i + 1], x[i + 2] = p[i + 2], x[i + 3] = p[i + 3];
+          for (int i = 0; i < QC / 4; ++i) {
+            const int at = 32 * (i % (QC / 8)) + lane, r = 16 * (i / (QC / 8)) + at / (QC / 4), e = at % (QC / 4);
+            const float *src = reinterpret_cast<const float *>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), r));
+            v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (src) {
+              if (a.vec_q) v[i] = *reinterpret_cast<const float4 *>(src + 4 * e);
+              else v[i] = make_float4(src[4 * e], src[4 * e + 1], src[4 * e + 2], src[4 * e + 3]);
             }
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < QC / 8; ++i) {
+              const int at = 32 * i + lane;
+              *reinterpret_cast<float4 *>(stage + at / (QC / 4) * L::kStageRow + 16 * (at % (QC / 4))) =
+                  v[half * (QC / 8) + i];
+            }
+            __syncwarp();
+            if (lane >> 4 == half) {
+#pragma unroll
+              for (int i = 0; i < QC; i += 4) {
+                const float4 u = *reinterpret_cast<const float4 *>(stage + (lane & 15) * L::kStageRow + 4 * i);
+                x[i] = u.x, x[i + 1] = u.y, x[i + 2] = u.z, x[i + 3] = u.w;
+              }
+            }
+            __syncwarp();
           }
           bool bad = false;
 #pragma unroll
@@ -253,13 +338,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           float up = __uint_as_float((uint32_t)(127 + e) << 23);
           if (a.scale < 0.0f) up = -up;  // f is positive: the largest S is the largest score
           // (never 0, so that f * -inf is -inf; a row that sees nothing is 0 whatever its query)
-          const float scale = bad && last >= 0 ? __uint_as_float(0x7fc00000u) : fmaxf(ldexpf(fabsf(a.scale), -e), 1.2e-38f);
+          const float scale = bad && sees ? __uint_as_float(0x7fc00000u) : fmaxf(ldexpf(fabsf(a.scale), -e), 1.2e-38f);
 #pragma unroll
           for (int c = 0; c < QC / 8; ++c) {  // 8 elements, in the order of a decoded word
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) split_f16(x[8 * c + i] * up, x[8 * c + i + 4] * up, hi[i], lo[i]);
-            const uint32_t col = qr * (QC / 2) + 4 * c;
+            const uint32_t col = grp * (QC / 2) + 4 * c;
             tm_st4(lanes + kTmQ + col, hi[0], hi[1], hi[2], hi[3]);
             tm_st4(lanes + kTmQ + 64 + col, lo[0], lo[1], lo[2], lo[3]);
           }
@@ -267,47 +352,44 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           sm100::tc_fence_before();
           sm100::mbar_arrive(q_full);
 
-          auto add_output = [&](int k) {  // O of step k
+          auto add_output = [&](int see) {  // O of a step
             ok = wait(o_full, o_phase) && ok;
             o_phase ^= 1u;
             sm100::tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < QC; c += 8) {
-              uint32_t r[8];
-              tm_ld8(lanes + kTmO + qr * QC + c, r);
+            for (int c = 0; c < QC; c += 16) {
+              uint32_t r[16];
+              tm_ld16(lanes + kTmO + grp * QC + c, r);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) acc[c + i] += __uint_as_float(r[i]);
+              for (int i = 0; i < 16; i += 2)
+                acc[(c + i) / 2] = add_two(acc[(c + i) / 2], two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
             }
             // NaN values of the step entered as 0: the rows that see them are marked.
-            const uint32_t *bits = reinterpret_cast<const uint32_t *>(nan_bits + mask.i * NB * 16 + 4 * qr);
-            uint32_t any = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) any |= bits[4 * b];
-            if (any) {
-              const int see = last - (s.t0 + k) * kPreTokens - 32 * qr;
-              const uint32_t mine = see < 0 ? 0 : see >= 31 ? ~0u : (2u << see) - 1;
+            if (nan_step[mask.i] == step) {
+              const uint64_t *bits = reinterpret_cast<const uint64_t *>(nan_bits + mask.i * NB * 16 + 8 * grp);
+              const uint64_t mine = see < 0 ? 0 : see >= 63 ? ~0ull : (2ull << see) - 1;
 #pragma unroll
               for (int b = 0; b < NB; ++b)
-                if (bits[4 * b] & mine) poison |= 1u << b;
+                if (bits[2 * b] & mine) poison |= 1u << b;
             }
+            ++step;
             mask.next();
           };
 
           for (int k = 0; k < steps; ++k) {
             ok = wait(&s_full[score.i], score.phase) && ok;
-            const uint32_t cols = lanes + kTmS + 128 * score.i + 32 * qr;
+            const uint32_t cols = lanes + kTmS + 128 * score.i + kPreCols * grp;
             score.next();
             sm100::tc_fence_after();
-            const uint32_t units = unit_mask[smask.i] >> (2 * qr) & 3u;
+            const uint32_t units = unit_mask[smask.i] >> (4 * grp) & 15u;
             smask.next();
-            const int see = last - (s.t0 + k) * kPreTokens - 32 * qr;  // columns 0..see
             // (Loops of 16 columns keep the instruction cache: unrolled further, the roles' code evicted itself and
             // a step took three times as long.)
             // Hide what the row does not see (TMEM is read and written by whole warps).
-            if (__any_sync(0xffffffffu, see < 31 || units != 3u)) {
+            if (__any_sync(0xffffffffu, see < 63 || units != 15u)) {
 #pragma unroll 1
-              for (int c = 0; c < 32; c += 16) {
+              for (int c = 0; c < kPreCols; c += 16) {
                 uint32_t r[16];
                 tm_ld16(cols + c, r);
                 sm100::tmem_ld_wait();
@@ -321,12 +403,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 32; c += 16) {
-              uint32_t r[16];
+            for (int c = 0; c < kPreCols; c += 32) {
+              uint32_t r[32];
               tm_ld16(cols + c, r);
+              tm_ld16(cols + c + 16, r + 16);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+              for (int i = 0; i < 32; i += 2) top = max_three(top, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
             }
             top = exchange(top, larger) * scale;
             float old = 1.0f;
@@ -334,89 +417,108 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               const float to = top - 8.0f;
               old = ex2(ref - to);
               ref = to;
-              sum *= old;
             }
             const float shift = ref == -INFINITY ? 0.0f : ref;
+            const uint64_t shifts = two(-shift, -shift), scales = two(scale, scale);
+            sums = mul_two(sums, two(old, old));
 #pragma unroll 1
-            for (int c = 0; c < 32; c += 16) {
-              uint32_t r[16], w[16];
+            for (int c = 0; c < kPreCols; c += 32) {
+              uint32_t r[32], w[2][16];
               tm_ld16(cols + c, r);
+              tm_ld16(cols + c + 16, r + 16);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, -shift));
-                const float p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, -shift));
-                sum += p0 + p1;
-                split_f16(p0, p1, w[i >> 1], w[8 + (i >> 1)]);
+              for (int i = 0; i < 32; i += 2) {
+                const float2 z = of_two(fma_two(two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scales, shifts));
+                const float p0 = ex2(z.x), p1 = ex2(z.y);
+                sums = add_two(sums, two(p0, p1));
+                split_f16(p0, p1, w[i >> 4][(i & 15) >> 1], w[i >> 4][8 + ((i & 15) >> 1)]);
               }
-              tm_st16(cols + c, w);
+              tm_st16(cols + c, w[0]);
+              tm_st16(cols + c + 16, w[1]);
             }
-            if (k > 0) add_output(k - 1);
+            if (k > 0) add_output(see + kPreTokens);
             if (__any_sync(0xffffffffu, old != 1.0f)) {
 #pragma unroll
-              for (int i = 0; i < QC; ++i) acc[i] *= old;
+              for (int i = 0; i < QC / 2; ++i) acc[i] = mul_two(acc[i], two(old, old));
             }
             tm_st_wait();
             sm100::tc_fence_before();
             sm100::mbar_arrive(p_full);
+            see -= kPreTokens;
           }
-          add_output(steps - 1);
+          add_output(see + kPreTokens);
         }
         // ---- the row's end
-        const float total = exchange(sum, plus);
+        const float2 halves = of_two(sums);
+        const float total = exchange(halves.x + halves.y, plus);
         poison = __float_as_uint(exchange(__uint_as_float(poison), either));
-        const bool whole = s.t0 == 0 && s.t1 == s.whole;
+        if (threadIdx.x == 0) sm100::mbar_arrive(&seg_empty[sg.i]);  // all have read it
+        sg.next();
+        const bool whole = kind == kSegWhole;
         if (!ok) poison = ~0u;
-        if (real) {
-          float *dst;
-          bool vec = true;
-          float inv = 1.0f;
-          if (whole) {
-            dst = a.out + (int64_t)(s.q.row0 + qi) * a.ld_o + (int64_t)(s.head * a.group + f % a.group) * a.hs_o;
-            vec = a.vec_o;
-            inv = total == 0.0f ? 0.0f : 1.0f / total;
-          } else {
-            float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kPreRows, HD);
-            dst = part + 2 * kPreRows + row * HD;
-            if (qr == 0) part[row] = ref, part[kPreRows + row] = total;
-          }
-          dst += qr * QC;
-#pragma unroll
-          for (int i = 0; i < QC; i += 4) {
-            float4 v = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-            if (poison >> ((qr * QC + i) / 32) & 1u) {
-              const float n = __uint_as_float(0x7fc00000u);
-              v = make_float4(n, n, n, n);
-            }
-            if (vec) *reinterpret_cast<float4 *>(dst + i) = v;
-            else dst[i] = v.x, dst[i + 1] = v.y, dst[i + 2] = v.z, dst[i + 3] = v.w;
-          }
+        float *dst = nullptr;
+        float inv = 1.0f;
+        if (real && whole) {
+          dst = a.out + out_row * a.ld_o + head * a.hs_o + grp * QC;
+          inv = total == 0.0f ? 0.0f : 1.0f / total;
+        } else if (real) {
+          float *part = a.parts + (int64_t)(2 * blockIdx.x + (kind == kSegHead)) * kv4_part_floats(kPreRows, HD);
+          dst = part + 2 * kPreRows + row * HD + grp * QC;
+          if (grp == 0) part[row] = ref, part[kPreRows + row] = total;
         }
-        if (threadIdx.x == 0 && s.t0 == 0 && !whole) {
-          a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
-          a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
+        const bool vec = a.vec_o || !whole;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {  // 16 rows at a time, written along the rows
+          if (lane >> 4 == half) {
+#pragma unroll
+            for (int i = 0; i < QC; i += 4) {
+              const float2 u = of_two(mul_two(acc[i / 2], two(inv, inv)));
+              const float2 v = of_two(mul_two(acc[i / 2 + 1], two(inv, inv)));
+              float4 o = make_float4(u.x, u.y, v.x, v.y);
+              if (poison >> ((grp * QC + i) / 32) & 1u) {
+                const float n = __uint_as_float(0x7fc00000u);
+                o = make_float4(n, n, n, n);
+              }
+              *reinterpret_cast<float4 *>(stage + (lane & 15) * L::kStageRow + 4 * i) = o;
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < QC / 8; ++i) {
+            const int at = 32 * i + lane, r = at / (QC / 4), e = at % (QC / 4);
+            float *d = reinterpret_cast<float *>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), 16 * half + r));
+            const float4 o = *reinterpret_cast<const float4 *>(stage + r * L::kStageRow + 16 * e);
+            if (d) {
+              if (vec) *reinterpret_cast<float4 *>(d + 4 * e) = o;
+              else d[4 * e] = o.x, d[4 * e + 1] = o.y, d[4 * e + 2] = o.z, d[4 * e + 3] = o.w;
+            }
+          }
+          __syncwarp();
         }
       }
-    } else if (warp < 20) {
+    } else if (warp < kWarpV) {
       // -------------------------------------------------------- packed units -> K tiles
       // A warp takes 8 tokens x 4 chunks at a time, paired so that neither the loads nor the stores meet a bank
       // twice. Token: 32 it + tk0, whose unit is 2 it + half a warp pair's.
-      const int dw = warp - 16, tk0 = 8 * dw + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tk0 & 15;
+      const int dw = warp - kWarpK, tk0 = 8 * dw + (lane & 7), t = (lane >> 3) ^ ((lane & 7) >> 1), tk = tk0 & 15;
       const int u0 = tk0 >> 4;
       const uint32_t src0 = L::kRawOff + u0 * UB + tk * (16 * NB) + t * (4 * NB);
       const uint32_t scale0 = L::kRawOff + u0 * UB + kv4_k_scale_off(NB) + tk * (2 * NB);
       const uint32_t dst0 = L::kKOff + tk0 * 128 + ((t ^ (lane & 7)) << 4);  // even blocks; odd ones are 64 bytes away
+      set_regs_down<64>();
       Ring<kPreRaw> raw;
       Ring<kPreStages> st;
       Ring<kPreMasks> mask;
       bool ok = true;
-      while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
-        const int steps = steps_of(s);
+      for (; ok && seg_next(); seg_done()) {
+        const int steps = segs[sg.i].steps;
         for (int k = 0; k < steps; ++k) {
           if (!(ok = wait(&raw_full[raw.i], raw.phase))) break;
           if (!(ok = wait(&k_empty[st.i], st.phase ^ 1u))) break;
           const uint32_t valid = raw_valid[raw.i];
-          if (threadIdx.x == 512) unit_mask[mask.i] = valid;
+          if (threadIdx.x == kWarpK * 32) unit_mask[mask.i] = valid;
           const uint8_t *src = sm + src0 + raw.i * L::kRaw, *scale = sm + scale0 + raw.i * L::kRaw;
           uint8_t *dst = sm + dst0 + st.i * L::kK;
 #pragma unroll 2
@@ -455,20 +557,22 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           raw.next(), st.next(), mask.next();
         }
       }
-    } else if (warp < 24) {
+    } else if (warp < kWarpMma) {
       // -------------------------------------------------------- packed units -> V tiles
       // A thread takes 8 tokens and 4 elements of every block, two blocks at a time. Odd token groups read their
       // tokens in pairs swapped, which spares half of the bank conflicts.
-      const int dw = warp - 20, m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
+      const int dw = warp - kWarpV, m = 4 * dw + (lane & 3), g = lane >> 2, odd = m & 1;
       const uint32_t src0 = L::kRawOff + (m >> 1) * UB + kv4_v_off(NB) + (8 * odd) * (16 * NB) + g * (2 * NB);
       const uint32_t scale0 = L::kRawOff + (m >> 1) * UB + kv4_v_scale_off(NB) + (8 * odd) * (2 * NB);
       const uint32_t dst0 = L::kVOff + (m >> 3) * L::kVPanel + 4 * g * 128;
+      uint32_t step = 0;
+      set_regs_down<64>();
       Ring<kPreRaw> raw;
       Ring<kPreStages> st;
       Ring<kPreMasks> mask;
       bool ok = true;
-      while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
-        const int steps = steps_of(s);
+      for (; ok && seg_next(); seg_done()) {
+        const int steps = segs[sg.i].steps;
         for (int k = 0; k < steps; ++k) {
           if (!(ok = wait(&raw_full[raw.i], raw.phase))) break;
           if (!(ok = wait(&v_empty[st.i], st.phase ^ 1u))) break;
@@ -508,6 +612,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
                     bad[h] |= 1u << (i ^ odd);
                     vd[i] &= ~(0xffffu << (16 * h));
                   }
+              if (bad[0] | bad[1]) nan_step[mask.i] = step;
             }
 #pragma unroll
             for (int h = 0; h < (NB == 1 ? 1 : 2); ++h) {
@@ -533,11 +638,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           sm100::mbar_arrive(&v_full[st.i]);
           sm100::mbar_arrive(&raw_empty[raw.i]);
           raw.next(), st.next(), mask.next();
+          ++step;
         }
       }
     } else {
-      set_regs_down<40>();
-      if (warp == 24) {
+      set_regs_down<48>();
+      if (warp == kWarpMma) {
         // ------------------------------------------------------ MMA issue
         // The whole warp walks and waits, one lane issues: operands computed by whole warps stay in uniform
         // registers, where the instruction wants them (from one lane's registers an MMA took 95 clocks to issue,
@@ -552,8 +658,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         auto all_wait = [&](uint64_t *bar, uint32_t parity) {
           return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs)) != 0;
         };
-        while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
-          const int steps = steps_of(s);
+        for (; ok && seg_next(); seg_done()) {
+          const int steps = segs[sg.i].steps;
           if (steps == 0) continue;
           if (!(ok = all_wait(q_full, q_phase))) break;
           q_phase ^= 1u;
@@ -605,16 +711,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           sm100::umma_commit(fin);
           sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
         }
-      } else if (warp == 25) {
+      } else if (warp == kWarpCopy) {
         // ------------------------------------------------------ copies of the packed units
         const int upp = a.c.page / kKv4Unit;
         const int64_t unit_page = a.c.page_head_bytes * a.c.kv;
         Ring<kPreRaw> raw;
         bool ok = true;
         int issued = 0;
-        while (ok && kv4_next<kPreRows, kPreTokens>(a, walk, s)) {
-          const int steps = steps_of(s), end_unit = (s.q.len + kKv4Unit - 1) / kKv4Unit;
-          const int *table = a.tables + (int64_t)s.r * a.width;
+        for (; ok && seg_next(); seg_done()) {
+          const PreSegment s = segs[sg.i];
+          const int steps = s.steps, end_unit = (s.len + kKv4Unit - 1) / kKv4Unit;
+          const int *table = a.tables + (int64_t)s.request * a.width;
           const uint8_t *slice = kv4_unit(a.c, a.layer, 0, s.head, 0);
           for (int k = 0; k < steps; ++k) {
             const int u = (s.t0 + k) * kPreUnits + lane;
@@ -638,12 +745,35 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         // the last copies have landed before the CTA can exit
         for (int i = max(0, issued - kPreRaw); i < issued; ++i)
           sm100::mbar_wait(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u, nullptr, nullptr, kPreDrainNs);
+      } else if (warp == kWarpWalk && lane == 0) {
+        // ------------------------------------------------------ the walk over the items
+        Kv4Segment s;
+        for (bool more = true; more; sg.next()) {
+          more = kv4_next<kPreRows, kPreTokens>(a, walk, s);
+          if (!wait(&seg_empty[sg.i], sg.phase ^ 1u)) break;
+          PreSegment &d = segs[sg.i];
+          if (more) {
+            const bool whole = s.t0 == 0 && s.t1 == s.whole;
+            const int f = min((s.tile + 1) * kPreRows, s.q.flat) - 1, last = min(s.q.base + f / a.group, s.q.len - 1);
+            d.kind = whole ? kSegWhole : s.t0 == 0 ? kSegHead : kSegTail;
+            d.row0 = s.q.row0, d.flat = s.q.flat, d.base = s.q.base, d.len = s.q.len;
+            d.request = s.r, d.head = s.head, d.tile = s.tile, d.t0 = s.t0;
+            d.steps = max(0, min(s.t1, (last + kPreTokens) / kPreTokens) - s.t0);
+            if (d.kind == kSegHead) {  // the item goes on in the next CTAs
+              a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
+              a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
+            }
+          } else {
+            d.kind = kSegEnd;
+          }
+          sm100::mbar_arrive(&seg_full[sg.i]);
+        }
       }
     }
     __syncwarp();
     sm100::tc_fence_before();
     __syncthreads();
-    if (warp == 24) {
+    if (warp == kWarpMma) {
       sm100::tc_fence_after();
       sm100::tmem_dealloc(tmem, 512);
     }
