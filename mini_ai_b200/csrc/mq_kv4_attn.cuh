@@ -34,6 +34,7 @@ struct Kv4AttnArgs {
   const int *offsets, *lens, *tables;
   int n, width, rows, group;
   int min_rows, max_rows;  // requests of min_rows..max_rows flat rows are this kernel's
+  bool cut;                // items may be cut (and joined)
   float scale;             // times log2(e): the softmax is in powers of two
   float *parts;            // [grid][2] partial items
   int4 *meta;              // [grid][2]: the item that a CTA leaves unfinished
@@ -146,7 +147,7 @@ __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
   w.tile = lo;
   w.t = (int)(in_head - kv4_work<RT, BN>(w.q.base, a.group, lo));
   w.whole = kv4_tile_work<RT, BN>(w.q, a.group, lo);
-  if (w.t <= kv4_setup<RT>()) w.left += w.t, w.place -= w.t, w.t = 0;  // no item is cut in its setup: see kv4_next
+  if (!a.cut || w.t <= kv4_setup<RT>()) w.left += w.t, w.place -= w.t, w.t = 0;  // no item is cut in its setup: see kv4_next
   return true;
 }
 
@@ -174,7 +175,7 @@ __device__ __forceinline__ bool kv4_next(const Kv4AttnArgs &a, Kv4Walk &w, Kv4Se
     w.whole = kv4_tile_work<RT, BN>(w.q, a.group, w.tile);
   }
   const int setup = kv4_setup<RT>(), end = (int)min((int64_t)w.whole, w.t + w.left);
-  if (end < w.whole && end <= setup) {  // the next CTA begins this item
+  if (end < w.whole && (!a.cut || end <= setup)) {  // a later CTA does this item
     w.left = 0;
     return false;
   }
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
   }
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
-  if (threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
+  if (a.cut && threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
   Kv4Walk walk;
   if (!kv4_walk<kDecRowTile, kDecTokens>(a, walk)) return;
   __syncwarp();

@@ -38,29 +38,32 @@ struct PagesArgs {
   const int *n_free;
   int rows;
   int *offsets, *lens, *slots, *positions, *n_free_out, *refused;
+  bool vec;  // slots and positions are aligned to 16 bytes
 };
 
 __host__ __device__ constexpr size_t pages_smem(int n) { return (size_t)(3 * n + 1) * sizeof(int); }
 
-// Inclusive sum over the CTA's threads; `total` the CTA's sum. Two barriers.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int64_t &total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
+  return v;
+}
+
+// Inclusive sum over the CTA's threads (whole warps); `total` the CTA's sum. Two barriers.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  v = warp_scan(v);
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < nwarps; ++w) {
-    const int64_t s = warp_sums[w];
-    if (w < warp) before += s;
-    all += s;
-  }
-  total = all;
+  const int64_t sums = warp_scan(lane < nwarps ? warp_sums[lane] : 0);
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, sums, warp ? warp - 1 : 0);
   __syncthreads();
-  return v + before;
+  return v + (warp ? before : 0);
 }
 
 __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesArgs a) {
@@ -93,9 +96,8 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesAr
     }
   }
   if (threadIdx.x == 0) off[0] = 0;
-  int64_t all_refused, all_taken;
-  block_scan(refused, warp_sums, all_refused);
-  block_scan(taken, warp_sums, all_taken);  // its barriers order the writes of off, ctx and first
+  int64_t both;  // refused requests and, below them, taken pages; the barriers order the writes of off, ctx and first
+  block_scan((int64_t)refused << 40 | taken, warp_sums, both);
   // seq_lens may be ctx_lens, and n_free_out may be n_free: every CTA has read them.
   if (ncta > 1) sm100::cluster_sync();
   if (cta == 0) {
@@ -105,36 +107,51 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesAr
     }
     if (threadIdx.x == 0) {
       a.offsets[0] = 0;
-      *a.n_free_out = n_free - (int)all_taken;
-      *a.refused = (int)all_refused;
+      *a.n_free_out = n_free - (int)(both & ((1ll << 40) - 1));
+      *a.refused = (int)(both >> 40);
     }
   }
-  for (int64_t row = (int64_t)cta * blockDim.x + threadIdx.x; row < a.rows; row += (int64_t)ncta * blockDim.x) {
-    int slot = -1, pos = -1;
-    if (row < off[a.n]) {
+  // Four neighbouring rows a thread: one search, mostly one page.
+  const int total = off[a.n];
+  for (int64_t row0 = 4 * ((int64_t)cta * blockDim.x + threadIdx.x); row0 < a.rows;
+       row0 += 4 * (int64_t)ncta * blockDim.x) {
+    int slot[4], pos[4], r = 0, known = -1, id = 0;  // `id`: page `known` of request r
+    if (row0 < total) {
       int lo = 0, hi = a.n - 1;  // the first request that ends behind the row
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (off[mid + 1] > row) hi = mid;
+        if (off[mid + 1] > row0) hi = mid;
         else lo = mid + 1;
       }
-      if (first[lo] >= 0) {
-        pos = ctx[lo] + (int)row - off[lo];
-        const int held = (int)(((int64_t)ctx[lo] + a.page - 1) / a.page), i = pos / a.page;
-        int *entry = a.tables + (int64_t)lo * a.width + i;
-        int id;
-        if (i < held) {
-          id = *entry;
-        } else {
-          id = a.stack[n_free - 1 - (first[lo] + i - held)];
-          if (pos % a.page == 0) *entry = id;  // a new page's first token is one of the new rows
-        }
-        const int64_t s = (int64_t)id * a.page + pos % a.page;
-        slot = id >= 0 && s <= INT_MAX ? (int)s : -1;
-      }
+      r = lo;
     }
-    a.slots[row] = slot;
-    a.positions[row] = pos;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + i;
+      slot[i] = pos[i] = -1;
+      if (row >= total) continue;
+      while (off[r + 1] <= row) ++r, known = -1;
+      if (first[r] < 0) continue;
+      const int p = ctx[r] + (int)(row - off[r]), page = p / a.page, in = p - page * a.page;
+      if (page != known) {
+        const int held = (int)(((int64_t)ctx[r] + a.page - 1) / a.page);
+        int *entry = a.tables + (int64_t)r * a.width + page;
+        id = page < held ? *entry : a.stack[n_free - 1 - (first[r] + page - held)];
+        if (page >= held && in == 0) *entry = id;  // a new page's first token is one of the new rows
+        known = page;
+      }
+      const int64_t s = (int64_t)id * a.page + in;
+      slot[i] = id >= 0 && s <= INT_MAX ? (int)s : -1;
+      pos[i] = p;
+    }
+    if (a.vec && row0 + 4 <= a.rows) {
+      *reinterpret_cast<int4 *>(a.slots + row0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4 *>(a.positions + row0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row0 + i < a.rows) a.slots[row0 + i] = slot[i], a.positions[row0 + i] = pos[i];
+    }
   }
 }
 

@@ -10,45 +10,64 @@ A step over ragged requests, as the batched forward runs it:
 Lengths, offsets, slots and tables are int32 tensors on the cache's device and are read when the
 kernels run, so that a step can be captured in a CUDA graph. Wrong arguments raise ``ValueError``
 or ``RuntimeError`` before anything is launched.
+
+A decode step's kernels take a few microseconds each, so the calls do little else: arguments are
+checked by single comparisons, and spelled out only once one fails.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
-from typing import NamedTuple
 
 from . import _lib
 from ._lib import check, lib
 
 
 def _torch():
+    global _current
     import torch  # plumbing only: device memory and streams
 
+    if _current is False:  # the handle itself, without a Stream object around it (1.5 us)
+        _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) if torch.cuda.is_available() else None
     return torch
+
+
+_current = False
 
 
 def _stream_on(torch, device: int, stream) -> int:
     """The handle of `stream`, or of the current stream of `device`."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return _current(device) if _current else torch.cuda.current_stream(device).cuda_stream
     if stream.device.index != device:
         raise ValueError(f"the stream is of device {stream.device.index}, the call's of device {device}")
     return stream.cuda_stream
 
 
-def _allocating_on(torch, stream):
-    """The allocator reuses memory in the order of the stream that it was allocated on: the launch's."""
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+def _empty(torch, shape, dtype, device, stream):
+    """Memory for a call on `stream`: the allocator reuses it in the order of the stream it was allocated on."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _ints(torch, name: str, t, device: int, shape: tuple | None = None) -> int:
-    """The address of an int32 tensor on `device` with `shape` (None: any number of elements)."""
-    if t.dtype is not torch.int32 or not t.is_cuda or t.get_device() != device:
+def _ints(torch, name: str, t, device: int, n: int) -> int:
+    """The address of `n` contiguous int32 values on `device`."""
+    if t.dtype is torch.int32 and t.get_device() == device and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not torch.int32 or t.get_device() != device:
         raise RuntimeError(f"{name}: an int32 tensor on cuda:{device} is needed, not {t.dtype} on {t.device}")
-    if not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise RuntimeError(f"{name}: shape mismatch (contiguous {shape} is needed, not {tuple(t.shape)})")
-    return t.data_ptr()
+    raise RuntimeError(f"{name}: shape mismatch ({n} contiguous values are needed, not {tuple(t.shape)})")
+
+
+def _table(torch, t):
+    """(device, requests, pages, address) of block tables."""
+    if t.dim() != 2:
+        raise RuntimeError("block_tables: shape mismatch ([requests, pages] is needed)")
+    device = t.get_device()
+    n, width = t.shape
+    return device, n, width, _ints(torch, "block_tables", t, max(device, 0), n * width)
 
 
 def _ok(rc: int, what: str) -> None:
@@ -57,22 +76,34 @@ def _ok(rc: int, what: str) -> None:
     check(rc, what)
 
 
-class PagePlan(NamedTuple):
+class PagePlan:
     """What ``PlanPages`` writes: row offsets ``[n + 1]`` and lengths ``[n]`` of the requests, slots and
-    positions ``[rows]`` (-1 behind the last request), the free pages left and the requests refused ``[1]``."""
+    positions ``[rows]`` (-1 behind the last request), the free pages left and the requests refused ``[1]``.
 
-    offsets: object
-    seq_lens: object
-    slots: object
-    positions: object
-    n_free: object
-    refused: object
+    The tensors are checked here once and stay the plan's for its life.
+    """
+
+    __slots__ = ("offsets", "seq_lens", "slots", "positions", "n_free", "refused", "device", "_sizes", "_addresses")
+
+    def __init__(self, offsets, seq_lens, slots, positions, n_free, refused):
+        torch = _torch()
+        self.offsets, self.seq_lens, self.slots = offsets, seq_lens, slots
+        self.positions, self.n_free, self.refused = positions, n_free, refused
+        self.device = max(offsets.get_device(), 0)
+        n, rows = seq_lens.numel(), slots.numel()
+        self._sizes = (n, rows)
+        self._addresses = tuple(_ints(torch, name, t, self.device, size) for name, t, size in (
+            ("offsets", offsets, n + 1), ("seq_lens", seq_lens, n), ("slots", slots, rows),
+            ("positions", positions, rows), ("n_free", n_free, 1), ("refused", refused, 1)))
 
     @classmethod
-    def empty(cls, n_seqs: int, rows: int, device: int = 0) -> "PagePlan":
+    def empty(cls, n_seqs: int, rows: int, device: int = 0, seq_lens=None, n_free=None, stream=None) -> "PagePlan":
+        """A plan of its own memory; with ``seq_lens`` or ``n_free`` those, as a step that advances the lengths and
+        the stack in place wants it."""
         torch = _torch()
-        at = torch.device("cuda", device)
-        return cls(*(torch.empty(n, dtype=torch.int32, device=at) for n in (n_seqs + 1, n_seqs, rows, rows, 1, 1)))
+        make = lambda n: _empty(torch, n, torch.int32, torch.device("cuda", device), stream)  # noqa: E731
+        return cls(make(n_seqs + 1), make(n_seqs) if seq_lens is None else seq_lens, make(rows), make(rows),
+                   make(1) if n_free is None else n_free, make(1))
 
 
 def PlanPages(ctx_lens, new_lens, block_tables, free_pages, n_free, page_size: int, rows: int | None = None,
@@ -83,24 +114,20 @@ def PlanPages(ctx_lens, new_lens, block_tables, free_pages, n_free, page_size: i
     ``out`` (whose ``seq_lens`` may be ``ctx_lens`` and whose ``n_free`` may be ``n_free``) it is theirs.
     """
     torch = _torch()
-    if block_tables.dim() != 2:
-        raise RuntimeError("block_tables: shape mismatch ([requests, pages] is needed)")
-    n, width = block_tables.shape
-    device = block_tables.get_device()
+    if out is None and rows is None:
+        raise ValueError("PlanPages needs rows (the row arrays' capacity) or out")
+    device, n, width, tables = _table(torch, block_tables)
     if out is None:
-        if rows is None:
-            raise ValueError("PlanPages needs rows (the row arrays' capacity) or out")
-        out = PagePlan.empty(n, rows, max(device, 0))
-    elif rows is None:
-        rows = out.slots.shape[0]
+        out = PagePlan.empty(n, rows, device, stream=stream)
+    if out._sizes[0] != n or out.device != device or (rows is not None and rows != out._sizes[1]):
+        raise RuntimeError(f"out: shape mismatch (a plan of {n} requests on cuda:{device} is needed)")
+    offsets, seq_lens, slots, positions, n_free_out, refused = out._addresses
+    free = free_pages.numel()
     _ok(lib().mq_pages_plan(
-        device, _ints(torch, "ctx_lens", ctx_lens, device, (n,)), _ints(torch, "new_lens", new_lens, device, (n,)), n,
-        page_size, _ints(torch, "block_tables", block_tables, device), width,
-        _ints(torch, "free_pages", free_pages, device), free_pages.numel(),
-        _ints(torch, "n_free", n_free, device, (1,)), rows, _ints(torch, "offsets", out.offsets, device, (n + 1,)),
-        _ints(torch, "seq_lens", out.seq_lens, device, (n,)), _ints(torch, "slots", out.slots, device, (rows,)),
-        _ints(torch, "positions", out.positions, device, (rows,)), _ints(torch, "n_free", out.n_free, device, (1,)),
-        _ints(torch, "refused", out.refused, device, (1,)), _stream_on(torch, device, stream)), "PlanPages")
+        device, _ints(torch, "ctx_lens", ctx_lens, device, n), _ints(torch, "new_lens", new_lens, device, n), n,
+        page_size, tables, width, _ints(torch, "free_pages", free_pages, device, free), free,
+        _ints(torch, "n_free", n_free, device, 1), out._sizes[1], offsets, seq_lens, slots, positions, n_free_out,
+        refused, _stream_on(torch, device, stream)), "PlanPages")
     return out
 
 
@@ -108,15 +135,13 @@ def ReleasePages(requests, seq_lens, block_tables, free_pages, n_free, page_size
     """Ends the requests of these rows of ``block_tables``: their pages go back to the stack and their lengths
     become 0, all in place (mq_pages_release)."""
     torch = _torch()
-    if block_tables.dim() != 2:
-        raise RuntimeError("block_tables: shape mismatch ([requests, pages] is needed)")
-    n, width = block_tables.shape
-    device = block_tables.get_device()
+    device, n, width, tables = _table(torch, block_tables)
+    count, free = requests.numel(), free_pages.numel()
     _ok(lib().mq_pages_release(
-        device, _ints(torch, "requests", requests, device), requests.numel(), n, page_size,
-        _ints(torch, "seq_lens", seq_lens, device, (n,)), _ints(torch, "block_tables", block_tables, device), width,
-        _ints(torch, "free_pages", free_pages, device), free_pages.numel(),
-        _ints(torch, "n_free", n_free, device, (1,)), _stream_on(torch, device, stream)), "ReleasePages")
+        device, _ints(torch, "requests", requests, device, count), count, n, page_size,
+        _ints(torch, "seq_lens", seq_lens, device, n), tables, width,
+        _ints(torch, "free_pages", free_pages, device, free), free, _ints(torch, "n_free", n_free, device, 1),
+        _stream_on(torch, device, stream)), "ReleasePages")
 
 
 class Kv4Cache:
@@ -132,16 +157,16 @@ class Kv4Cache:
         need = lib().mq_kv4_bytes(layers, pages, page_size, kv_heads, head_dim)
         if not need:
             raise ValueError(f"Kv4Cache: {_lib.last_error()}")
+        if not torch.cuda.is_available():
+            raise RuntimeError("Kv4Cache needs a GPU")
         sh = _stream_on(torch, device, stream)
-        with _allocating_on(torch, stream):
-            self.memory = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
+        self.memory = _empty(torch, need, torch.uint8, torch.device("cuda", device), stream)
         handle = C.c_void_p()
         _ok(lib().mq_kv4_create(device, layers, pages, page_size, kv_heads, head_dim, self.memory.data_ptr(), need, sh,
                                 C.byref(handle)), "Kv4Cache")
         self.handle = handle
         self.device, self.layers, self.pages, self.page_size = device, layers, pages, page_size
         self.kv_heads, self.head_dim = kv_heads, head_dim
-        self._workspace = {}  # bytes by (heads, max_new)
 
     @property
     def device_bytes(self) -> int:
@@ -149,37 +174,40 @@ class Kv4Cache:
         check(lib().mq_kv4_info(self.handle, None, None, None, None, None, None, C.byref(n)))
         return n.value
 
-    def _rows(self, torch, name: str, t, heads: int | None):
-        """``t`` ``[rows, heads, head_dim]``, checked."""
-        if t.dtype is not torch.float32 or not t.is_cuda or t.get_device() != self.device:
-            raise RuntimeError(f"{name}: F32 rows on the cache's device are needed, not {t.dtype} on {t.device}")
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise RuntimeError(f"{name}: shape mismatch ([rows, {heads or 'heads'}, {self.head_dim}] is needed, not "
-                               f"{tuple(t.shape)})")
-        if t.stride(2) != 1:
+    def _rows(self, torch, name: str, t, rows: int | None, heads: int | None):
+        """(shape, strides) of F32 `t` [rows, heads, head_dim] whose heads are contiguous."""
+        shape = t.shape
+        if (t.dtype is torch.float32 and t.get_device() == self.device and len(shape) == 3
+                and shape[2] == self.head_dim and (heads is None or shape[1] == heads)
+                and (rows is None or shape[0] == rows)):
+            strides = t.stride()
+            if strides[2] == 1:
+                return shape, strides
             raise RuntimeError(f"{name}: the elements of a head must be contiguous")
-        return t
+        if t.dtype is not torch.float32 or t.get_device() != self.device:
+            raise RuntimeError(f"{name}: F32 rows on the cache's device are needed, not {t.dtype} on {t.device}")
+        raise RuntimeError(f"{name}: shape mismatch ([{'rows' if rows is None else rows}, {heads or 'heads'}, "
+                           f"{self.head_dim}] is needed, not {tuple(shape)})")
 
     def store(self, layer: int, k, v, slots, stream=None) -> None:
         """Packs ``k`` and ``v`` ``[rows, kv_heads, head_dim]`` into ``layer`` at ``slots`` (mq_kv4_store)."""
         torch = _torch()
-        k, v = self._rows(torch, "keys", k, self.kv_heads), self._rows(torch, "values", v, self.kv_heads)
-        rows = k.shape[0]
-        if v.shape[0] != rows:
-            raise RuntimeError(f"values: shape mismatch ({v.shape[0]} rows, {rows} of keys)")
-        _ok(lib().mq_kv4_store(self.handle, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                               v.stride(1), _ints(torch, "slots", slots, self.device, (rows,)), rows,
+        (rows, _, _), (ld_k, hs_k, _) = self._rows(torch, "keys", k, None, self.kv_heads)
+        _, (ld_v, hs_v, _) = self._rows(torch, "values", v, rows, self.kv_heads)
+        _ok(lib().mq_kv4_store(self.handle, layer, k.data_ptr(), ld_k, hs_k, v.data_ptr(), ld_v, hs_v,
+                               _ints(torch, "slots", slots, self.device, rows), rows,
                                _stream_on(torch, self.device, stream)), "Kv4Cache.store")
 
     def load(self, layer: int, slots, stream=None):
         """The values that ``layer`` holds at ``slots``: ``(k, v)``, ``[rows, kv_heads, head_dim]`` (mq_kv4_load)."""
         torch = _torch()
-        at = _ints(torch, "slots", slots, self.device)
         rows = slots.numel()
-        handle = _stream_on(torch, self.device, stream)
-        with _allocating_on(torch, stream):
-            k, v = torch.empty((2, rows, self.kv_heads, self.head_dim), dtype=torch.float32, device=slots.device)
-        _ok(lib().mq_kv4_load(self.handle, layer, at, rows, k.data_ptr(), v.data_ptr(), handle), "Kv4Cache.load")
+        at = _ints(torch, "slots", slots, self.device, rows)
+        sh = _stream_on(torch, self.device, stream)
+        shape = (rows, self.kv_heads, self.head_dim)
+        k = _empty(torch, shape, torch.float32, slots.device, stream)
+        v = _empty(torch, shape, torch.float32, slots.device, stream)
+        _ok(lib().mq_kv4_load(self.handle, layer, at, rows, k.data_ptr(), v.data_ptr(), sh), "Kv4Cache.load")
         return k, v
 
     def attention(self, layer: int, q, offsets, seq_lens, block_tables, max_new: int | None = None,
@@ -192,31 +220,31 @@ class Kv4Cache:
         1 / sqrt(head_dim).
         """
         torch = _torch()
-        q = self._rows(torch, "queries", q, None)
-        rows, heads = q.shape[0], q.shape[1]
-        if block_tables.dim() != 2:
-            raise RuntimeError("block_tables: shape mismatch ([requests, pages] is needed)")
-        n, width = block_tables.shape
-        handle = _stream_on(torch, self.device, stream)
-        if out is not None and self._rows(torch, "output", out, heads).shape[0] < rows:
-            raise RuntimeError(f"output: shape mismatch ({out.shape[0]} rows, {rows} of queries)")
+        device = self.device
+        (rows, heads, _), (ld_q, hs_q, _) = self._rows(torch, "queries", q, None, None)
+        on, n, width, tables = _table(torch, block_tables)
+        if on != device:
+            raise RuntimeError(f"block_tables: an int32 tensor on cuda:{device} is needed")
+        sh = _stream_on(torch, device, stream)
+        if out is None:
+            out = _empty(torch, (rows, heads, self.head_dim), torch.float32, q.device, stream)
+            if stream is None:
+                out.zero_()
+            else:
+                with torch.cuda.stream(stream):
+                    out.zero_()
+        (out_rows, _, _), (ld_o, hs_o, _) = self._rows(torch, "output", out, None, heads)
+        if out_rows < rows:
+            raise RuntimeError(f"output: shape mismatch ({out_rows} rows, {rows} of queries)")
         if max_new is None:
             max_new = rows
-        need = self._workspace.get((heads, max_new))
-        if need is None:
-            need = lib().mq_kv4_attention_workspace(self.handle, heads, max_new)
-            self._workspace[heads, max_new] = need
-        with _allocating_on(torch, stream):
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-            if out is None:
-                out = torch.zeros((rows, heads, self.head_dim), dtype=torch.float32, device=q.device)
+        need = lib().mq_kv4_attention_workspace(self.handle, heads, max_new)
+        ws = _empty(torch, need, torch.uint8, q.device, stream)
         _ok(lib().mq_kv4_attention(
-            self.handle, layer, q.data_ptr(), q.stride(0), q.stride(1), rows, heads,
-            _ints(torch, "offsets", offsets, self.device, (n + 1,)),
-            _ints(torch, "seq_lens", seq_lens, self.device, (n,)),
-            _ints(torch, "block_tables", block_tables, self.device), n, width, max_new,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
-            ws.data_ptr(), need, handle), "Kv4Cache.attention")
+            self.handle, layer, q.data_ptr(), ld_q, hs_q, rows, heads, _ints(torch, "offsets", offsets, device, n + 1),
+            _ints(torch, "seq_lens", seq_lens, device, n), tables, n, width, max_new,
+            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(), ld_o, hs_o, ws.data_ptr(),
+            need, sh), "Kv4Cache.attention")
         return out
 
     def close(self) -> None:

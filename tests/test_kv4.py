@@ -84,7 +84,9 @@ def test_python_refuses_host_tensors(mq):
     i = torch.zeros(2, dtype=torch.int32)
     tables = torch.zeros((2, 4), dtype=torch.int32)
     with pytest.raises(RuntimeError, match="int32 tensor on cuda"):
-        mq.PlanPages(i, i, tables, i, i[:1], 16, out=mq.PagePlan(i, i, i, i, i, i))
+        mq.PagePlan(torch.zeros(3, dtype=torch.int32), i, i, i, i[:1], i[:1])
+    with pytest.raises(RuntimeError, match="int32 tensor on cuda"):
+        mq.PlanPages(i, i, tables, i, i[:1], 16, rows=4)
     with pytest.raises(ValueError, match="rows"):
         mq.PlanPages(i, i, tables, i, i[:1], 16)
     with pytest.raises(RuntimeError, match="shape"):

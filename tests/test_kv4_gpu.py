@@ -281,8 +281,7 @@ def _check_plan(mq, torch, ctx, new, tables, free, n_free, page, rows, in_place=
     t, c, nf = ints(torch, tables), ints(torch, ctx), ints(torch, [n_free])
     out = None
     if in_place:
-        e = mq.PagePlan.empty(len(ctx), rows)
-        out = e._replace(seq_lens=c, n_free=nf)
+        out = mq.PagePlan.empty(len(ctx), rows, seq_lens=c, n_free=nf)
     p = mq.PlanPages(c, ints(torch, new), t, ints(torch, free), nf, page, rows=rows, out=out)
     got = (t, p.seq_lens, p.offsets, p.slots, p.positions, p.n_free, p.refused)
     for name, g, w in zip(("tables", "lens", "offsets", "slots", "positions", "n_free", "refused"), got, want):
@@ -617,7 +616,7 @@ class Server:
     def step(self, news, gen):
         torch, mq = self.torch, self.mq
         rows = sum(news) + 3
-        plan = mq.PagePlan.empty(len(news), rows)._replace(seq_lens=self.lens, n_free=self.n_free)
+        plan = mq.PagePlan.empty(len(news), rows, seq_lens=self.lens, n_free=self.n_free)
         mq.PlanPages(self.lens, ints(torch, news), self.tables, self.free, self.n_free, self.page, out=plan)
         assert int(plan.refused) == 0
         for layer in range(self.layers):
@@ -669,7 +668,7 @@ def test_graph_of_a_step(mq, torch):
     free = ints(torch, [p for p in range(b.cache.pages) if p not in used])
     n_free, ctx = ints(torch, [free.numel()]), ints(torch, lens)
     tables = torch.cat([b.tables, torch.full((4, 2), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
-    plan = mq.PagePlan.empty(4, 4)._replace(seq_lens=ctx, n_free=n_free)
+    plan = mq.PagePlan.empty(4, 4, seq_lens=ctx, n_free=n_free)
     one = ints(torch, [1] * 4)
     x = torch.zeros(4, 8 * 64, device="cuda")
     q, k, v = (z.reshape(4, -1, 64) for z in x.split([4 * 64, 2 * 64, 2 * 64], 1))
