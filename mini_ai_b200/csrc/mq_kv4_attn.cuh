@@ -216,6 +216,33 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
   lo = h2_bits(__floats2half2_rn(a, b));
 }
 
+// Pairs of floats in one instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 of_two(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+
 // D = A B + D: A 16 x 16 row-major, B 16 x 8 column-major, fp16; D fp32.
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -390,33 +417,24 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       ref = -INFINITY, sum = 0.0f;
 
       // The ring: step k of this warp is units first_unit + (k * 4 + warp) * 2 + {0, 1}.
-      int ids = -1;        // page ids of 16 steps' units, one a lane
-      uint32_t held = 0;   // two bits a stage: units that were fetched
+      uint32_t held = 0;  // two bits a stage: units that were fetched
+      // Every 16 steps each lane looks up one unit of the next 16, and copies it when its step comes.
+      const uint8_t *unit_at = nullptr;
+      uint32_t there = 0;  // lanes whose unit is in the cache
       auto fetch = [&](int k) {
-        const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
         if ((k & 15) == 0) {
           const int u = first_unit + ((k + (lane >> 1)) * kDecWarps + warp) * kDecUnits + (lane & 1);
-          ids = u < end_unit ? __ldg(table + u / upp) : -1;
-          if (ids >= a.c.pages) ids = -1;
+          const int id = u < end_unit ? __ldg(table + u / upp) : -1;
+          const bool in = id >= 0 && id < a.c.pages;
+          unit_at = slice + id * unit_page + (int64_t)(u % upp) * L::kUnit;
+          there = __ballot_sync(0xffffffffu, in);
         }
-        const uint32_t stage = (steps_done + k) % kDecStages;
-        uint32_t have = 0;
-        int id[kDecUnits];
-#pragma unroll
-        for (int j = 0; j < kDecUnits; ++j) {
-          id[j] = __shfl_sync(0xffffffffu, ids, (k & 15) * 2 + j);
-          have |= (id[j] >= 0 ? 1u : 0u) << j;
-        }
+        const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (2 * (k & 15)) & 3u;
         held = (held & ~(3u << (2 * stage))) | have << (2 * stage);
-        if (lane == 0) {
-          sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit);
-#pragma unroll
-          for (int j = 0; j < kDecUnits; ++j)
-            if (id[j] >= 0)
-              sm100::bulk_load(ring + (stage * kDecUnits + j) * L::kUnit,
-                               slice + id[j] * unit_page + (int64_t)((u0 + j) % upp) * L::kUnit, L::kUnit,
-                               &bars[stage]);
-        }
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit);
+        __syncwarp();
+        if (lane >> 1 == (k & 15) && (there >> lane & 1u))
+          sm100::bulk_load(ring + (stage * kDecUnits + (lane & 1)) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
       };
       for (int k = 0; k < min(kDecStages - 1, steps); ++k) fetch(k);
 
@@ -457,17 +475,19 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
             uint32_t d0[W], d1[W];
             lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 8 * i) * (2 * NB), d0);
             lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 4 + 8 * i) * (2 * NB), d1);
-            float s0 = 0.0f, s1 = 0.0f;
+            uint64_t s01 = 0;  // the two tokens' scores
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
               const uint32_t w = kw[b], w8 = w >> 8;
               mma16816(c, qa[2 * b], h2_bits(code_lo(w)), h2_bits(code_hi(w)));
               mma16816(c, qa[2 * b + 1], h2_bits(code_lo(w8)), h2_bits(code_hi(w8)));
-              s0 = fmaf(half_at(d0, b), c[0] + c[2], s0);
-              s1 = fmaf(half_at(d1, b), c[1] + c[3], s1);
+              const uint64_t dd = two(half_at(d0, b), half_at(d1, b));
+              s01 = fma_two(dd, two(c[0], c[1]), s01);
+              s01 = fma_two(dd, two(c[2], c[3]), s01);
             }
-            sc[j][i][0] = s0 * fscale, sc[j][i][1] = s1 * fscale;
+            const float2 s2 = of_two(mul_two(s01, two(fscale, fscale)));
+            sc[j][i][0] = s2.x, sc[j][i][1] = s2.y;
           }
           if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_min) {  // some row's end
 #pragma unroll

@@ -117,32 +117,6 @@ __device__ __forceinline__ void tm_st4(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Pairs of floats in one instruction.
-__device__ __forceinline__ uint64_t two(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 of_two(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_two(uint64_t x, uint64_t y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul_two(uint64_t x, uint64_t y) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_two(uint64_t x, uint64_t y, uint64_t z) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-  return r;
-}
 __device__ __forceinline__ float max_three(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
