@@ -327,6 +327,8 @@ template <int NB>
 __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4AttnArgs a) {
   using L = DecSmem<NB>;
   constexpr int HD = 32 * NB, W = (NB + 1) / 2;
+  constexpr int kPer = 32 / kDecUnits;  // steps a lookup
+  constexpr uint32_t kAll = (1u << kDecUnits) - 1;
   extern __shared__ __align__(128) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t *ring = sm + warp * L::kRing;
@@ -417,24 +419,24 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       ref = -INFINITY, sum = 0.0f;
 
       // The ring: step k of this warp is units first_unit + (k * 4 + warp) * 2 + {0, 1}.
-      uint32_t held = 0;  // two bits a stage: units that were fetched
-      // Every 16 steps each lane looks up one unit of the next 16, and copies it when its step comes.
+      uint32_t held = 0;  // kDecUnits bits a stage: units that were fetched
+      // Every kPer steps each lane looks up one unit of the next kPer, and copies it when its step comes.
       const uint8_t *unit_at = nullptr;
       uint32_t there = 0;  // lanes whose unit is in the cache
       auto fetch = [&](int k) {
-        if ((k & 15) == 0) {
-          const int u = first_unit + ((k + (lane >> 1)) * kDecWarps + warp) * kDecUnits + (lane & 1);
+        if (k % kPer == 0) {
+          const int u = first_unit + ((k + lane / kDecUnits) * kDecWarps + warp) * kDecUnits + lane % kDecUnits;
           const int id = u < end_unit ? __ldg(table + u / upp) : -1;
           const bool in = id >= 0 && id < a.c.pages;
           unit_at = slice + id * unit_page + (int64_t)(u % upp) * L::kUnit;
           there = __ballot_sync(0xffffffffu, in);
         }
-        const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (2 * (k & 15)) & 3u;
-        held = (held & ~(3u << (2 * stage))) | have << (2 * stage);
+        const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (kDecUnits * (k % kPer)) & kAll;
+        held = (held & ~(kAll << (kDecUnits * stage))) | have << (kDecUnits * stage);
         if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit);
         __syncwarp();
-        if (lane >> 1 == (k & 15) && (there >> lane & 1u))
-          sm100::bulk_load(ring + (stage * kDecUnits + (lane & 1)) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
+        if (lane / kDecUnits == k % kPer && (there >> lane & 1u))
+          sm100::bulk_load(ring + (stage * kDecUnits + lane % kDecUnits) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
       };
       for (int k = 0; k < min(kDecStages - 1, steps); ++k) fetch(k);
 
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
         const uint32_t stage = (steps_done + k) % kDecStages;
         if (!sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, nullptr, nullptr, kKv4WaitNs))
           sum = __uint_as_float(0x7fc00000u);
-        const uint32_t have = (held >> (2 * stage)) & 3u;
+        const uint32_t have = held >> (kDecUnits * stage) & kAll;
         const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
         const uint8_t *buf = ring + stage * kDecUnits * L::kUnit;
 
@@ -642,44 +644,68 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
 }
 
 // Joins the parts of the items that their first CTA left unfinished: 8 rows of
-// one item a block, 4 elements a thread, the parts in order. The blocks of the
-// few-row kernel's CTAs come first, then `chunks` for each of the other's.
+// one item a block, 4 elements a thread, every kJoinSlices-th part a slice. A
+// slice adds its parts in order, and the slices are added in order. The blocks
+// of the few-row kernel's CTAs come first, then `chunks` for each of the other's.
 struct Kv4Join {
   const int4 *meta[2];
   const float *parts[2];
   int ctas[2];
 };
 constexpr int kJoinRows = 8;
+constexpr int kJoinSlices = 4;
 
-__global__ void __launch_bounds__(kJoinRows * 32) kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
+template <int NB>
+__global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices) kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
+  constexpr int HD = 32 * NB, kQuads = HD / 4, kLanes = kJoinRows * kQuads;
+  __shared__ float4 s_acc[kJoinSlices][kLanes];
+  __shared__ float s_top[kJoinSlices][kJoinRows], s_sum[kJoinSlices][kJoinRows];
   sm100::griddep_wait();
   const int which = blockIdx.x >= j.ctas[0], row_tile = which ? 128 : kDecRowTile;
-  const int at = which ? blockIdx.x - j.ctas[0] : blockIdx.x, chunks = row_tile / kJoinRows;
-  const int b = at / chunks, hd = a.c.hd, quads = hd / 4;
+  const int at = which ? blockIdx.x - j.ctas[0] : blockIdx.x, chunks = row_tile / kJoinRows, b = at / chunks;
   const int4 *meta = (which ? j.meta[1] : j.meta[0]) + 2 * b;
   const int parts = meta[1].x;
   if (parts == 0) return;
   const int4 m = meta[0];
-  const int row = at % chunks * kJoinRows + threadIdx.x / quads, e = 4 * (threadIdx.x % quads);
-  const int fr = m.y * row_tile + row;
-  if (fr >= m.w) return;
-  const int64_t stride = kv4_part_floats(row_tile, hd);
+  const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes, r = lane / kQuads, e = 4 * (lane % kQuads);
+  const int row = at % chunks * kJoinRows + r, fr = m.y * row_tile + row;
+  const bool real = fr < m.w;  // rows past the item's have no parts
+  const int64_t stride = kv4_part_floats(row_tile, HD);
   const float *parts0 = which ? j.parts[1] : j.parts[0];
   auto part = [&](int i) { return parts0 + (2 * (int64_t)(b + i) + (i == 0)) * stride; };
-  float top = -INFINITY;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, part(i)[row]);
-  const float shift = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f;
+  float top = -INFINITY, total = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (real) {
 #pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float *p = part(i);
-    const float k = ex2(p[row] - shift);
-    const float4 v = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * hd + e);
-    total += k * p[row_tile + row];
-    acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+    for (int i = slice; i < parts; i += kJoinSlices) top = fmaxf(top, part(i)[row]);
   }
+  if (e == 0) s_top[slice][r] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinSlices; ++i) top = fmaxf(top, s_top[i][r]);
+  const float shift = top == -INFINITY ? 0.0f : top;
+  if (real) {
+#pragma unroll 8
+    for (int i = slice; i < parts; i += kJoinSlices) {
+      const float *p = part(i);
+      const float k = ex2(p[row] - shift);
+      const float4 v = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * HD + e);
+      total += k * p[row_tile + row];
+      acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+    }
+  }
+  s_acc[slice][lane] = acc;
+  if (e == 0) s_sum[slice][r] = total;
+  __syncthreads();
+  if (slice || !real) return;
+#pragma unroll
+  for (int i = 1; i < kJoinSlices; ++i) {
+    const float4 v = s_acc[i][lane];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+  }
+  total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kJoinSlices; ++i) total += s_sum[i][r];
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
   float *dst =
