@@ -58,6 +58,9 @@ bool vector16(const void *p, int64_t ld, int64_t hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0 && hs % 4 == 0;
 }
 
+// Whether the blocks that so many CTAs of a store or load pack count in 32 bits.
+bool fits32(int64_t ctas) { return ctas * (kKv4Threads / 4) < (int64_t)1 << 32; }
+
 int check_cache(const mq_kv4 *c, int layer) {
   if (!c) return fail(MQ_ERR_INVALID, "null cache handle");
   if (layer < 0 || layer >= c->v.layers) return fail(MQ_ERR_INVALID, "layer %d of %d", layer, c->v.layers);
@@ -257,10 +260,10 @@ int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Kv4Rows kr{k, ld_k, hs_k}, vr{v, ld_v, hs_v};
-  if (vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v))
-    kv4_store_kernel<true><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
-  else
-    kv4_store_kernel<false><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
+  const bool vec = vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v);
+  auto *kernel = fits32(blocks) ? (vec ? kv4_store_kernel<true, uint32_t> : kv4_store_kernel<false, uint32_t>)
+                                : (vec ? kv4_store_kernel<true, int64_t> : kv4_store_kernel<false, int64_t>);
+  kernel<<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
   return launched("cache store");
 }
 
@@ -278,10 +281,10 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (vector16(k, 0, 0) && vector16(v, 0, 0))
-    kv4_load_kernel<true><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
-  else
-    kv4_load_kernel<false><<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
+  const bool vec = vector16(k, 0, 0) && vector16(v, 0, 0);
+  auto *kernel = fits32(blocks) ? (vec ? kv4_load_kernel<true, uint32_t> : kv4_load_kernel<false, uint32_t>)
+                                : (vec ? kv4_load_kernel<true, int64_t> : kv4_load_kernel<false, int64_t>);
+  kernel<<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
   return launched("cache load");
 }
 

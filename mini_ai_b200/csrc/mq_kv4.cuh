@@ -78,16 +78,30 @@ __device__ __forceinline__ uint32_t kv4_pack(const float (&x)[8], uint16_t &scal
   const __half dh = __float2half_rn(d8);
   const float d = __half2float(dh);
   scale = bad ? (uint16_t)0x7e00u : __half_as_ushort(dh);
-  uint32_t w = 0x88888888u;  // all codes 0
-  if (!bad && d != 0.0f) {
-    w = 0;
+  if (bad || d == 0.0f) return 0x88888888u;  // all codes 0
+  // Nearest integers by x times 1 / d, rounded by adding 1.5 * 2^23: right wherever the remainder (which fma gives
+  // exactly) stays below d / 2; where it does not, a tie or a quotient next to one, by the division.
+  constexpr float kRound = 12582912.0f;
+  const float inv = __frcp_rn(d);
+  uint32_t w = 0;
+  float far = 0.0f;
 #pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = fmaf(x[i], inv, kRound);
+    far = fmaxf(far, fabsf(fmaf(kRound - t, d, x[i])));
+    w |= (__float_as_uint(fminf(fmaxf(t, kRound - 8.0f), kRound + 7.0f)) & 15u) << (4 * i);
+  }
+  if (!(far < 0.5f * fabsf(d))) {
+    w = 0;
+#pragma unroll 1
     for (int i = 0; i < 8; ++i) {
-      const int c = (int)fminf(fmaxf(rintf(__fdiv_rn(x[i], d)), -8.0f), 7.0f);
-      w |= (uint32_t)(c + 8) << (4 * i);
+      float v = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) v = i == j ? x[j] : v;
+      w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(v, d)), -8.0f), 7.0f) & 15u) << (4 * i);
     }
   }
-  return w;
+  return w ^ 0x88888888u;  // c + 8
 }
 
 struct Kv4Rows {  // rows [rows][kv][hd] with strides in elements
@@ -99,16 +113,17 @@ constexpr int kKv4Threads = 256;
 
 // One quad of lanes per block of a row: reads 32 floats, writes 16 bytes of
 // codes and a scale. Rows of no valid slot are skipped.
-template <bool VEC>
+// Index: 32 bits where the call's blocks fit (a 64-bit division costs as much as the packing).
+template <bool VEC, typename Index>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_store_kernel(const Kv4View c, int layer, const Kv4Rows k, const Kv4Rows v, const int *__restrict__ slots,
                      int rows) {
   const int per_row = 2 * c.kv * c.nb;  // blocks of a row: K heads, then V heads
-  const int64_t total = (int64_t)rows * per_row;
-  const int64_t i0 = ((int64_t)blockIdx.x * kKv4Threads + threadIdx.x) >> 2;
+  const Index total = (Index)rows * per_row;
+  const Index i0 = (Index)blockIdx.x * (kKv4Threads / 4) + (threadIdx.x >> 2);
   const bool inside = i0 < total;
-  const int64_t idx = inside ? i0 : total - 1;  // whole warps: kv4_pack shuffles
-  const int row = (int)(idx / per_row), in_row = (int)(idx % per_row);
+  const Index idx = inside ? i0 : total - 1;  // whole warps: kv4_pack shuffles
+  const int row = (int)(idx / per_row), in_row = (int)(idx - (Index)row * per_row);
   const bool is_v = in_row >= c.kv * c.nb;
   const int hb = is_v ? in_row - c.kv * c.nb : in_row, head = hb / c.nb, j = hb % c.nb, t = threadIdx.x & 3;
   const int slot = slots[row];
@@ -140,14 +155,14 @@ __global__ void __launch_bounds__(kKv4Threads)
 
 // The values at `slots`, k and v [rows][kv][hd]; rows of no valid slot are 0.
 // Threads as in the store.
-template <bool VEC>
+template <bool VEC, typename Index>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_load_kernel(const Kv4View c, int layer, const int *__restrict__ slots, int rows, float *__restrict__ k,
                     float *__restrict__ v) {
   const int per_row = 2 * c.kv * c.nb;
-  const int64_t idx = ((int64_t)blockIdx.x * kKv4Threads + threadIdx.x) >> 2;
-  if (idx >= (int64_t)rows * per_row) return;
-  const int row = (int)(idx / per_row), in_row = (int)(idx % per_row);
+  const Index idx = (Index)blockIdx.x * (kKv4Threads / 4) + (threadIdx.x >> 2);
+  if (idx >= (Index)rows * per_row) return;
+  const int row = (int)(idx / per_row), in_row = (int)(idx - (Index)row * per_row);
   const bool is_v = in_row >= c.kv * c.nb;
   const int hb = is_v ? in_row - c.kv * c.nb : in_row, head = hb / c.nb, j = hb % c.nb, t = threadIdx.x & 3;
   const int slot = slots[row];

@@ -653,7 +653,7 @@ struct Kv4Join {
   int ctas[2];
 };
 constexpr int kJoinRows = 8;
-constexpr int kJoinSlices = 4;
+constexpr int kJoinSlices = 2;  // blocks of 512 threads: all of the few-row kernel's are resident at once
 
 template <int NB>
 __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices) kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices) kv4_join_ker
   float top = -INFINITY, total = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (real) {
-#pragma unroll 8
+#pragma unroll 16
     for (int i = slice; i < parts; i += kJoinSlices) top = fmaxf(top, part(i)[row]);
   }
   if (e == 0) s_top[slice][r] = top;
