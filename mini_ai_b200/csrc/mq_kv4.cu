@@ -59,7 +59,7 @@ bool vector16(const void *p, int64_t ld, int64_t hs) {
 }
 
 // Whether the blocks that so many CTAs of a store or load pack count in 32 bits.
-bool fits32(int64_t ctas) { return ctas * (kKv4Threads / 4) < (int64_t)1 << 32; }
+bool fits32(int64_t ctas) { return ctas * kKv4Blocks < (int64_t)1 << 32; }
 
 int check_cache(const mq_kv4 *c, int layer) {
   if (!c) return fail(MQ_ERR_INVALID, "null cache handle");
@@ -254,7 +254,7 @@ int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64
   if (int rc = check_rows("key", k, ld_k, hs_k, c->v.kv, c->v.hd)) return rc;
   if (int rc = check_rows("value", v, ld_v, hs_v, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
-  const int64_t blocks = ((int64_t)rows * 8 * c->v.kv * c->v.nb + kKv4Threads - 1) / kKv4Threads;
+  const int64_t blocks = ((int64_t)rows * 2 * c->v.kv * c->v.nb + kKv4Blocks - 1) / kKv4Blocks;
   if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
@@ -276,7 +276,7 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
   if (int rc = check_rows("key", k, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
   if (int rc = check_rows("value", v, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
-  const int64_t blocks = ((int64_t)rows * 8 * c->v.kv * c->v.nb + kKv4Threads - 1) / kKv4Threads;
+  const int64_t blocks = ((int64_t)rows * 2 * c->v.kv * c->v.nb + kKv4Blocks - 1) / kKv4Blocks;
   if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");

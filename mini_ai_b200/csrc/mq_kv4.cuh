@@ -111,45 +111,76 @@ struct Kv4Rows {  // rows [rows][kv][hd] with strides in elements
 
 constexpr int kKv4Threads = 256;
 
-// One quad of lanes per block of a row: reads 32 floats, writes 16 bytes of
-// codes and a scale. Rows of no valid slot are skipped.
+constexpr int kKv4Each = 2;                                   // blocks a quad of lanes
+constexpr int kKv4Blocks = kKv4Threads / 4 * kKv4Each;         // blocks a CTA
+
+// A block's place: row, head and block of the head, K or V.
+struct Kv4Place {
+  int row, head, j;
+  bool v;
+};
+template <typename Index>
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4View &c, Index idx, int per_row) {
+  Kv4Place p;
+  p.row = (int)(idx / per_row);
+  const int in_row = (int)(idx - (Index)p.row * per_row), half = c.kv * c.nb;
+  p.v = in_row >= half;
+  const int hb = p.v ? in_row - half : in_row;
+  p.head = hb / c.nb, p.j = hb % c.nb;
+  return p;
+}
+// Where lane t's 8 elements of the block lie in `unit`: K one word, V two half-words 2 nb bytes apart; and its scale.
+__device__ __forceinline__ uint8_t *kv4_codes(const Kv4View &c, uint8_t *unit, const Kv4Place &p, int tok, int t) {
+  if (p.v) return unit + kv4_v_off(c.nb) + tok * 16 * c.nb + 4 * t * c.nb + 2 * p.j;
+  return unit + tok * 16 * c.nb + t * 4 * c.nb + 4 * p.j;
+}
+__device__ __forceinline__ uint16_t *kv4_scale(const Kv4View &c, uint8_t *unit, const Kv4Place &p, int tok) {
+  return reinterpret_cast<uint16_t *>(unit + (p.v ? kv4_v_scale_off(c.nb) : kv4_k_scale_off(c.nb))) + tok * c.nb + p.j;
+}
+
+// One quad of lanes per block of a row, two blocks each: reads 32 floats,
+// writes 16 bytes of codes and a scale. Rows of no valid slot are skipped.
 // Index: 32 bits where the call's blocks fit (a 64-bit division costs as much as the packing).
 template <bool VEC, typename Index>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_store_kernel(const Kv4View c, int layer, const Kv4Rows k, const Kv4Rows v, const int *__restrict__ slots,
                      int rows) {
-  const int per_row = 2 * c.kv * c.nb;  // blocks of a row: K heads, then V heads
-  const Index total = (Index)rows * per_row;
-  const Index i0 = (Index)blockIdx.x * (kKv4Threads / 4) + (threadIdx.x >> 2);
-  const bool inside = i0 < total;
-  const Index idx = inside ? i0 : total - 1;  // whole warps: kv4_pack shuffles
-  const int row = (int)(idx / per_row), in_row = (int)(idx - (Index)row * per_row);
-  const bool is_v = in_row >= c.kv * c.nb;
-  const int hb = is_v ? in_row - c.kv * c.nb : in_row, head = hb / c.nb, j = hb % c.nb, t = threadIdx.x & 3;
-  const int slot = slots[row];
-  const Kv4Rows &src = is_v ? v : k;
-  const float *p = src.p + row * src.ld + head * src.hs + 32 * j + 8 * t;
-  float x[8];
-  if (VEC) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
+  const int per_row = 2 * c.kv * c.nb, t = threadIdx.x & 3;  // blocks of a row: K heads, then V heads
+  const Index total = (Index)rows * per_row, i0 = (Index)blockIdx.x * kKv4Blocks + (threadIdx.x >> 2);
+  Kv4Place at[kKv4Each];
+  int slot[kKv4Each];
+  float x[kKv4Each][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __ldg(p + i);
+  for (int n = 0; n < kKv4Each; ++n) {
+    const Index idx = i0 + n * (kKv4Threads / 4);
+    at[n] = kv4_place(c, idx < total ? idx : total - 1, per_row);  // whole warps: kv4_pack shuffles
+    slot[n] = idx < total ? slots[at[n].row] : -1;
+    const Kv4Rows &src = at[n].v ? v : k;
+    const float *p = src.p + at[n].row * src.ld + at[n].head * src.hs + 32 * at[n].j + 8 * t;
+    if (VEC) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+      x[n][0] = a.x, x[n][1] = a.y, x[n][2] = a.z, x[n][3] = a.w;
+      x[n][4] = b.x, x[n][5] = b.y, x[n][6] = b.z, x[n][7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[n][i] = __ldg(p + i);
+    }
   }
-  uint16_t scale;
-  const uint32_t w = kv4_pack(x, scale);
-  if (!inside || slot < 0 || slot >= c.pages * c.page) return;
-  const int page_id = slot / c.page, in_page = slot % c.page, tok = in_page % kKv4Unit;
-  uint8_t *unit = kv4_unit(c, layer, page_id, head, in_page / kKv4Unit);
-  if (!is_v) {
-    *reinterpret_cast<uint32_t *>(unit + tok * 16 * c.nb + t * 4 * c.nb + 4 * j) = w;
-    if (t == 0) *reinterpret_cast<uint16_t *>(unit + kv4_k_scale_off(c.nb) + 2 * (tok * c.nb + j)) = scale;
-  } else {
-    uint8_t *vr = unit + kv4_v_off(c.nb) + tok * 16 * c.nb + 2 * j;
-    *reinterpret_cast<uint16_t *>(vr + (2 * t) * 2 * c.nb) = (uint16_t)w;
-    *reinterpret_cast<uint16_t *>(vr + (2 * t + 1) * 2 * c.nb) = (uint16_t)(w >> 16);
-    if (t == 0) *reinterpret_cast<uint16_t *>(unit + kv4_v_scale_off(c.nb) + 2 * (tok * c.nb + j)) = scale;
+#pragma unroll
+  for (int n = 0; n < kKv4Each; ++n) {
+    uint16_t scale;
+    const uint32_t w = kv4_pack(x[n], scale);
+    if (slot[n] < 0 || slot[n] >= c.pages * c.page) continue;
+    const int page_id = slot[n] / c.page, in_page = slot[n] - page_id * c.page, tok = in_page % kKv4Unit;
+    uint8_t *unit = kv4_unit(c, layer, page_id, at[n].head, in_page / kKv4Unit);
+    uint8_t *codes = kv4_codes(c, unit, at[n], tok, t);
+    if (at[n].v) {
+      *reinterpret_cast<uint16_t *>(codes) = (uint16_t)w;
+      *reinterpret_cast<uint16_t *>(codes + 2 * c.nb) = (uint16_t)(w >> 16);
+    } else {
+      *reinterpret_cast<uint32_t *>(codes) = w;
+    }
+    if (t == 0) *kv4_scale(c, unit, at[n], tok) = scale;
   }
 }
 
@@ -159,41 +190,43 @@ template <bool VEC, typename Index>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_load_kernel(const Kv4View c, int layer, const int *__restrict__ slots, int rows, float *__restrict__ k,
                     float *__restrict__ v) {
-  const int per_row = 2 * c.kv * c.nb;
-  const Index idx = (Index)blockIdx.x * (kKv4Threads / 4) + (threadIdx.x >> 2);
-  if (idx >= (Index)rows * per_row) return;
-  const int row = (int)(idx / per_row), in_row = (int)(idx - (Index)row * per_row);
-  const bool is_v = in_row >= c.kv * c.nb;
-  const int hb = is_v ? in_row - c.kv * c.nb : in_row, head = hb / c.nb, j = hb % c.nb, t = threadIdx.x & 3;
-  const int slot = slots[row];
-  float x[8];
+  const int per_row = 2 * c.kv * c.nb, t = threadIdx.x & 3;
+  const Index total = (Index)rows * per_row, i0 = (Index)blockIdx.x * kKv4Blocks + (threadIdx.x >> 2);
+  Kv4Place at[kKv4Each];
+  uint32_t w[kKv4Each];
+  float d[kKv4Each];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-  if (slot >= 0 && slot < c.pages * c.page) {
-    const int page_id = slot / c.page, in_page = slot % c.page, tok = in_page % kKv4Unit;
-    const uint8_t *unit = kv4_unit(c, layer, page_id, head, in_page / kKv4Unit);
-    uint32_t w;
-    uint16_t scale;
-    if (!is_v) {
-      w = __ldg(reinterpret_cast<const uint32_t *>(unit + tok * 16 * c.nb + t * 4 * c.nb + 4 * j));
-      scale = __ldg(reinterpret_cast<const uint16_t *>(unit + kv4_k_scale_off(c.nb) + 2 * (tok * c.nb + j)));
-    } else {
-      const uint8_t *vr = unit + kv4_v_off(c.nb) + tok * 16 * c.nb + 2 * j;
-      w = __ldg(reinterpret_cast<const uint16_t *>(vr + (2 * t) * 2 * c.nb)) |
-          (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(vr + (2 * t + 1) * 2 * c.nb)) << 16;
-      scale = __ldg(reinterpret_cast<const uint16_t *>(unit + kv4_v_scale_off(c.nb) + 2 * (tok * c.nb + j)));
-    }
-    const float d = __half2float(__ushort_as_half(scale));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = d * (float)((int)((w >> (4 * i)) & 15u) - 8);
+  for (int n = 0; n < kKv4Each; ++n) {
+    const Index idx = i0 + n * (kKv4Threads / 4);
+    if (idx >= total) continue;
+    at[n] = kv4_place(c, idx, per_row);
+    const int slot = slots[at[n].row];
+    w[n] = 0x88888888u, d[n] = 0.0f;
+    if (slot < 0 || slot >= c.pages * c.page) continue;
+    const int page_id = slot / c.page, in_page = slot - page_id * c.page, tok = in_page % kKv4Unit;
+    uint8_t *unit = kv4_unit(c, layer, page_id, at[n].head, in_page / kKv4Unit);
+    const uint8_t *codes = kv4_codes(c, unit, at[n], tok, t);
+    if (at[n].v)
+      w[n] = __ldg(reinterpret_cast<const uint16_t *>(codes)) |
+             (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(codes + 2 * c.nb)) << 16;
+    else
+      w[n] = __ldg(reinterpret_cast<const uint32_t *>(codes));
+    d[n] = __half2float(__ushort_as_half(__ldg(kv4_scale(c, unit, at[n], tok))));
   }
-  float *o = (is_v ? v : k) + ((int64_t)row * c.kv + head) * c.hd + 32 * j + 8 * t;
-  if (VEC) {
-    reinterpret_cast<float4 *>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4 *>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = x[i];
+  for (int n = 0; n < kKv4Each; ++n) {
+    if (i0 + n * (kKv4Threads / 4) >= total) continue;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = d[n] * (float)((int)((w[n] >> (4 * i)) & 15u) - 8);
+    float *o = (at[n].v ? v : k) + ((int64_t)at[n].row * c.kv + at[n].head) * c.hd + 32 * at[n].j + 8 * t;
+    if (VEC) {
+      reinterpret_cast<float4 *>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4 *>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = x[i];
+    }
   }
 }
 

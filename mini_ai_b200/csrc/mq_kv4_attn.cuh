@@ -644,9 +644,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
 }
 
 // Joins the parts of the items that their first CTA left unfinished: 8 rows of
-// one item a block, 4 elements a thread, every kJoinSlices-th part a slice. A
-// slice adds its parts in order, and the slices are added in order. The blocks
-// of the few-row kernel's CTAs come first, then `chunks` for each of the other's.
+// one item a block, 4 elements a thread, every kJoinSlices-th part a slice;
+// eight parts' loads are in flight together. A slice adds its parts in order,
+// and the slices are added in order. The blocks of the few-row kernel's CTAs
+// come first, then 16 for each of the other's.
 struct Kv4Join {
   const int4 *meta[2];
   const float *parts[2];
@@ -654,9 +655,11 @@ struct Kv4Join {
 };
 constexpr int kJoinRows = 8;
 constexpr int kJoinSlices = 2;  // blocks of 512 threads: all of the few-row kernel's are resident at once
+constexpr int kJoinBatch = 8;
 
 template <int NB>
-__global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices) kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
+__global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
+    kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
   constexpr int HD = 32 * NB, kQuads = HD / 4, kLanes = kJoinRows * kQuads;
   __shared__ float4 s_acc[kJoinSlices][kLanes];
   __shared__ float s_top[kJoinSlices][kJoinRows], s_sum[kJoinSlices][kJoinRows];
@@ -664,48 +667,58 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices) kv4_join_ker
   const int which = blockIdx.x >= j.ctas[0], row_tile = which ? 128 : kDecRowTile;
   const int at = which ? blockIdx.x - j.ctas[0] : blockIdx.x, chunks = row_tile / kJoinRows, b = at / chunks;
   const int4 *meta = (which ? j.meta[1] : j.meta[0]) + 2 * b;
+  const int4 m = meta[0];
   const int parts = meta[1].x;
   if (parts == 0) return;
-  const int4 m = meta[0];
   const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes, r = lane / kQuads, e = 4 * (lane % kQuads);
   const int row = at % chunks * kJoinRows + r, fr = m.y * row_tile + row;
   const bool real = fr < m.w;  // rows past the item's have no parts
   const int64_t stride = kv4_part_floats(row_tile, HD);
-  const float *parts0 = which ? j.parts[1] : j.parts[0];
-  auto part = [&](int i) { return parts0 + (2 * (int64_t)(b + i) + (i == 0)) * stride; };
+  const float *parts0 = (which ? j.parts[1] : j.parts[0]) + 2 * b * stride;
   float top = -INFINITY, total = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (real) {
-#pragma unroll 16
-    for (int i = slice; i < parts; i += kJoinSlices) top = fmaxf(top, part(i)[row]);
-  }
-  if (e == 0) s_top[slice][r] = top;
-  __syncthreads();
+  for (int i0 = slice; real && i0 < parts; i0 += kJoinSlices * kJoinBatch) {
+    float ref[kJoinBatch], sum[kJoinBatch];
+    float4 v[kJoinBatch];
 #pragma unroll
-  for (int i = 0; i < kJoinSlices; ++i) top = fmaxf(top, s_top[i][r]);
-  const float shift = top == -INFINITY ? 0.0f : top;
-  if (real) {
-#pragma unroll 8
-    for (int i = slice; i < parts; i += kJoinSlices) {
-      const float *p = part(i);
-      const float k = ex2(p[row] - shift);
-      const float4 v = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * HD + e);
-      total += k * p[row_tile + row];
-      acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+    for (int n = 0; n < kJoinBatch; ++n) {
+      const int i = i0 + n * kJoinSlices;
+      ref[n] = -INFINITY, sum[n] = 0.0f, v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i < parts) {
+        const float *p = parts0 + (2 * i + (i == 0)) * stride;  // the item's head is the second part of its CTA
+        ref[n] = p[row], sum[n] = p[row_tile + row];
+        v[n] = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * HD + e);
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int n = 0; n < kJoinBatch; ++n) now = fmaxf(now, ref[n]);
+    const float shift = now == -INFINITY ? 0.0f : now, old = ex2(top - shift);
+    total *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+    top = now;
+#pragma unroll
+    for (int n = 0; n < kJoinBatch; ++n) {
+      const float k = ex2(ref[n] - shift);
+      total += k * sum[n];
+      acc.x += k * v[n].x, acc.y += k * v[n].y, acc.z += k * v[n].z, acc.w += k * v[n].w;
     }
   }
-  s_acc[slice][lane] = acc;
-  if (e == 0) s_sum[slice][r] = total;
+  if (slice) s_acc[slice][lane] = acc;
+  if (e == 0) s_top[slice][r] = top, s_sum[slice][r] = total;
   __syncthreads();
   if (slice || !real) return;
+  float all = top;
+#pragma unroll
+  for (int i = 1; i < kJoinSlices; ++i) all = fmaxf(all, s_top[i][r]);
+  const float shift = all == -INFINITY ? 0.0f : all, own = ex2(top - shift);
+  total *= own, acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
 #pragma unroll
   for (int i = 1; i < kJoinSlices; ++i) {
+    const float k = ex2(s_top[i][r] - shift);
     const float4 v = s_acc[i][lane];
-    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    total += k * s_sum[i][r];
+    acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
   }
-  total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kJoinSlices; ++i) total += s_sum[i][r];
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
   float *dst =

@@ -204,7 +204,11 @@ class Kv4Cache:
         rows = slots.numel()
         at = _ints(torch, "slots", slots, self.device, rows)
         sh = _stream_on(torch, self.device, stream)
-        k, v = _empty(torch, (2, rows, self.kv_heads, self.head_dim), torch.float32, slots.device, stream).unbind(0)
+        shape = (rows, self.kv_heads, self.head_dim)
+        if stream is None:
+            k, v = slots.new_empty(shape, dtype=torch.float32), slots.new_empty(shape, dtype=torch.float32)
+        else:
+            k, v = (_empty(torch, shape, torch.float32, slots.device, stream) for _ in range(2))
         _ok(lib().mq_kv4_load(self.handle, layer, at, rows, k.data_ptr(), v.data_ptr(), sh), "Kv4Cache.load")
         return k, v
 
