@@ -166,7 +166,7 @@ int run_attention(Kv4AttnArgs a, const mq_kv4 *c, uint8_t *ws, bool many, cudaSt
   }
   if (!a.cut) return MQ_OK;
   return launch_after("join attention parts", kv4_join_kernel<NB>,
-                      dim3(j.ctas[0] + j.ctas[1] * (kPreRows / kJoinRows)), kJoinRows * 8 * NB * kJoinSlices, 0, s, a, j);
+                      dim3(j.ctas[0] + j.ctas[1] * (kPreRows / kJoinMany)), kJoinRows * 8 * NB * kJoinSlices, 0, s, a, j);
 }
 
 }  // namespace

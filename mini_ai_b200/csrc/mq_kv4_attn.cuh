@@ -643,19 +643,47 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
   }
 }
 
-// Joins the parts of the items that their first CTA left unfinished: 8 rows of
-// one item a block, 4 elements a thread, every kJoinSlices-th part a slice;
-// eight parts' loads are in flight together. A slice adds its parts in order,
-// and the slices are added in order. The blocks of the few-row kernel's CTAs
-// come first, then 16 for each of the other's.
+// Joins the parts of the items that their first CTA left unfinished. Items of
+// 8 rows, which may have many parts: one a block, 4 elements a thread, every
+// kJoinSlices-th part a slice, eight parts' loads in flight together. Items of
+// 128 rows, mostly of two parts: 64 rows a block, 4 rows a thread. Parts are
+// added in order, and slices in order. Blocks are few and large enough that all
+// are resident at once: their latency (two dependent loads) is the time.
 struct Kv4Join {
   const int4 *meta[2];
   const float *parts[2];
   int ctas[2];
 };
 constexpr int kJoinRows = 8;
-constexpr int kJoinSlices = 2;  // blocks of 512 threads: all of the few-row kernel's are resident at once
+constexpr int kJoinSlices = 2;
 constexpr int kJoinBatch = 8;
+constexpr int kJoinEach = 4;                                    // rows a thread of the large items
+constexpr int kJoinMany = kJoinRows * kJoinSlices * kJoinEach;  // rows a block of them
+
+// `parts0`: the two places of the item's first CTA; its own part is the second.
+__device__ __forceinline__ const float *kv4_part(const float *parts0, int i, int64_t stride) {
+  return parts0 + (2 * i + (i == 0)) * stride;
+}
+
+// acc and total, in units of 2^top, joined with another sum; all -inf: nothing was seen.
+__device__ __forceinline__ void kv4_add_part(float &top, float &total, float4 &acc, float ref, float sum, float4 v) {
+  const float now = fmaxf(top, ref), shift = now == -INFINITY ? 0.0f : now;
+  const float old = ex2(top - shift), k = ex2(ref - shift);
+  top = now;
+  total = total * old + k * sum;
+  acc.x = acc.x * old + k * v.x, acc.y = acc.y * old + k * v.y;
+  acc.z = acc.z * old + k * v.z, acc.w = acc.w * old + k * v.w;
+}
+
+// Row fr of the item `m` (Kv4AttnArgs::meta): acc / total to elements e..e + 3.
+__device__ __forceinline__ void kv4_write(const Kv4AttnArgs &a, int4 m, int fr, int e, float total, float4 acc) {
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+  float *dst =
+      a.out + (int64_t)(m.x + fr / a.group) * a.ld_o + (int64_t)(m.z * a.group + fr % a.group) * a.hs_o + e;
+  if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
+  else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
+}
 
 template <int NB>
 __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
@@ -664,17 +692,51 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
   __shared__ float4 s_acc[kJoinSlices][kLanes];
   __shared__ float s_top[kJoinSlices][kJoinRows], s_sum[kJoinSlices][kJoinRows];
   sm100::griddep_wait();
-  const int which = blockIdx.x >= j.ctas[0], row_tile = which ? 128 : kDecRowTile;
-  const int at = which ? blockIdx.x - j.ctas[0] : blockIdx.x, chunks = row_tile / kJoinRows, b = at / chunks;
-  const int4 *meta = (which ? j.meta[1] : j.meta[0]) + 2 * b;
-  const int4 m = meta[0];
-  const int parts = meta[1].x;
+  if ((int)blockIdx.x >= j.ctas[0]) {
+    constexpr int kRows = 128, kChunks = kRows / kJoinMany;
+    const int at = blockIdx.x - j.ctas[0], b = at / kChunks;
+    const int4 m = j.meta[1][2 * b];
+    const int parts = j.meta[1][2 * b + 1].x;
+    if (parts == 0) return;
+    constexpr int64_t kStride = kv4_part_floats(kRows, HD);
+    const float *parts0 = j.parts[1] + 2 * b * kStride;
+    const int row0 = at % kChunks * kJoinMany + threadIdx.x / kQuads, e = 4 * (threadIdx.x % kQuads);
+    float top[kJoinEach], total[kJoinEach];
+    float4 acc[kJoinEach];
+#pragma unroll
+    for (int n = 0; n < kJoinEach; ++n) top[n] = -INFINITY, total[n] = 0.0f, acc[n] = make_float4(0, 0, 0, 0);
+    for (int i = 0; i < parts; ++i) {
+      const float *p = kv4_part(parts0, i, kStride);
+      float ref[kJoinEach], sum[kJoinEach];
+      float4 v[kJoinEach];
+#pragma unroll
+      for (int n = 0; n < kJoinEach; ++n) {
+        const int row = row0 + n * (kJoinRows * kJoinSlices);
+        ref[n] = -INFINITY, sum[n] = 0.0f, v[n] = make_float4(0, 0, 0, 0);
+        if (m.y * kRows + row < m.w) {  // rows past the item's have no parts
+          ref[n] = p[row], sum[n] = p[kRows + row];
+          v[n] = *reinterpret_cast<const float4 *>(p + 2 * kRows + row * HD + e);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kJoinEach; ++n) kv4_add_part(top[n], total[n], acc[n], ref[n], sum[n], v[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < kJoinEach; ++n) {
+      const int fr = m.y * kRows + row0 + n * (kJoinRows * kJoinSlices);
+      if (fr < m.w) kv4_write(a, m, fr, e, total[n], acc[n]);
+    }
+    return;
+  }
+  const int b = blockIdx.x;
+  const int4 m = j.meta[0][2 * b];
+  const int parts = j.meta[0][2 * b + 1].x;
   if (parts == 0) return;
-  const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes, r = lane / kQuads, e = 4 * (lane % kQuads);
-  const int row = at % chunks * kJoinRows + r, fr = m.y * row_tile + row;
-  const bool real = fr < m.w;  // rows past the item's have no parts
-  const int64_t stride = kv4_part_floats(row_tile, HD);
-  const float *parts0 = (which ? j.parts[1] : j.parts[0]) + 2 * b * stride;
+  constexpr int64_t kStride = kv4_part_floats(kDecRowTile, HD);
+  const float *parts0 = j.parts[0] + 2 * b * kStride;
+  const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes, row = lane / kQuads, e = 4 * (lane % kQuads);
+  const int fr = m.y * kDecRowTile + row;
+  const bool real = fr < m.w;
   float top = -INFINITY, total = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int i0 = slice; real && i0 < parts; i0 += kJoinSlices * kJoinBatch) {
@@ -685,46 +747,21 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
       const int i = i0 + n * kJoinSlices;
       ref[n] = -INFINITY, sum[n] = 0.0f, v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (i < parts) {
-        const float *p = parts0 + (2 * i + (i == 0)) * stride;  // the item's head is the second part of its CTA
-        ref[n] = p[row], sum[n] = p[row_tile + row];
-        v[n] = *reinterpret_cast<const float4 *>(p + 2 * row_tile + row * HD + e);
+        const float *p = kv4_part(parts0, i, kStride);
+        ref[n] = p[row], sum[n] = p[kDecRowTile + row];
+        v[n] = *reinterpret_cast<const float4 *>(p + 2 * kDecRowTile + row * HD + e);
       }
     }
-    float now = top;
 #pragma unroll
-    for (int n = 0; n < kJoinBatch; ++n) now = fmaxf(now, ref[n]);
-    const float shift = now == -INFINITY ? 0.0f : now, old = ex2(top - shift);
-    total *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-    top = now;
-#pragma unroll
-    for (int n = 0; n < kJoinBatch; ++n) {
-      const float k = ex2(ref[n] - shift);
-      total += k * sum[n];
-      acc.x += k * v[n].x, acc.y += k * v[n].y, acc.z += k * v[n].z, acc.w += k * v[n].w;
-    }
+    for (int n = 0; n < kJoinBatch; ++n) kv4_add_part(top, total, acc, ref[n], sum[n], v[n]);
   }
   if (slice) s_acc[slice][lane] = acc;
-  if (e == 0) s_top[slice][r] = top, s_sum[slice][r] = total;
+  if (e == 0) s_top[slice][row] = top, s_sum[slice][row] = total;
   __syncthreads();
   if (slice || !real) return;
-  float all = top;
 #pragma unroll
-  for (int i = 1; i < kJoinSlices; ++i) all = fmaxf(all, s_top[i][r]);
-  const float shift = all == -INFINITY ? 0.0f : all, own = ex2(top - shift);
-  total *= own, acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
-#pragma unroll
-  for (int i = 1; i < kJoinSlices; ++i) {
-    const float k = ex2(s_top[i][r] - shift);
-    const float4 v = s_acc[i][lane];
-    total += k * s_sum[i][r];
-    acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
-  }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-  float *dst =
-      a.out + (int64_t)(m.x + fr / a.group) * a.ld_o + (int64_t)(m.z * a.group + fr % a.group) * a.hs_o + e;
-  if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
-  else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
+  for (int i = 1; i < kJoinSlices; ++i) kv4_add_part(top, total, acc, s_top[i][row], s_sum[i][row], s_acc[i][lane]);
+  kv4_write(a, m, fr, e, total, acc);
 }
 
 }  // namespace mq
