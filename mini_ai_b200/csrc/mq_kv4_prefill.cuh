@@ -7,18 +7,19 @@
 //   S = Qhi K^T + Qlo K^T            [128 rows, 128 tokens], fp32 in TMEM
 //   P = 2^(S f - ref) -> Phi, Plo    one thread a row and half of the columns
 //   O = Phi V + Plo V                [128 rows, hd], fp32 in TMEM
-// and the running output of a row is in its threads' registers: adding one
+// and the running output of a row is in a thread's registers: adding one
 // step's O there costs hd additions a row, keeps every tensor-core sum at 16
 // additions (they truncate), and lets a moved reference scale registers.
 // Both A operands come from TMEM, so shared memory feeds the tensor cores
 // with B alone (64 of its 128 bytes a clock).
 //
-// Warps: 0-7 softmax (a thread: one row, half of a step's tokens and of the
-// output's columns), 8-11 decode K and 12-15 V (packed units -> swizzled
-// tiles), 16 issues the MMAs, 17 the copies of the packed units, 18 walks the
-// items and hands their segments to the others through a ring.
-// S of step i + 1 is computed while the softmax of step i runs, and O of step
-// i during the softmax of step i + 1.
+// Warps: 0-7 softmax (a thread: one row, half of a step's tokens), 8-11 the
+// running output (a thread: one row), 12-15 decode K and 16-19 V (packed units
+// -> swizzled tiles), 20 issues the MMAs, 21 the copies of the packed units, 22
+// walks the items and hands their segments to the others through a ring.
+// S of step i + 1 is computed while the softmax of step i runs, O of step i
+// during the softmax of step i + 1; and an item is written out while the next
+// one's queries are read.
 //
 // Bound: the tensor cores. Twice 4 hd operations a (row, token) pair (hi and
 // lo) against 1.67 PFLOP/s.
@@ -31,15 +32,16 @@ namespace mq {
 constexpr int kPreRows = 128;    // RT
 constexpr int kPreTokens = 128;  // BN
 constexpr int kPreSoft = 256;      // softmax threads
-constexpr int kPreThreads = kPreSoft + 384;
+constexpr int kPreThreads = kPreSoft + 512;
 constexpr int kPreGroups = kPreSoft / kPreRows;      // threads of a row
 constexpr int kPreCols = kPreTokens / kPreGroups;    // of S a thread
-constexpr int kWarpK = kPreSoft / 32, kWarpV = kWarpK + 4, kWarpMma = kWarpV + 4, kWarpCopy = kWarpMma + 1,
+constexpr int kWarpOut = kPreSoft / 32, kWarpK = kWarpOut + 4, kWarpV = kWarpK + 4, kWarpMma = kWarpV + 4, kWarpCopy = kWarpMma + 1,
               kWarpWalk = kWarpMma + 2;
 constexpr int kPreRaw = 3;       // packed steps in flight
 constexpr int kPreStages = 2;    // K and V tiles
 constexpr int kPreMasks = 4;
 constexpr int kPreSegs = 4;
+constexpr int kStageRow = 80;  // bytes: 16 floats; 8 rows meet all banks once
 constexpr int kPreUnits = kPreTokens / kKv4Unit;
 constexpr uint64_t kPreDrainNs = 20000000ull;
 
@@ -64,11 +66,12 @@ struct PreSmem {
   static constexpr int kVOff = kPreStages * kK;
   static constexpr int kRawOff = kVOff + kPreStages * kV;
   static constexpr int kXchOff = kRawOff + kPreRaw * kRaw;  // floats [2 parities][groups][128 rows]
-  static constexpr int kNanOff = kXchOff + 2 * kPreGroups * kPreRows * 4;  // bytes [masks][NB][16 token groups]
-  static constexpr int kStageRow = HD / kPreGroups * 4 + 16;   // a thread's part of a row; rows 4 banks apart
-  static constexpr int kStageOff = kNanOff + kPreMasks * NB * 16;  // 16 rows a softmax warp
-  static constexpr int kBarOff = kStageOff + kPreSoft / 32 * 16 * kStageRow;
-  static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 6 + 2 * kPreSegs;
+  static constexpr int kOldOff = kXchOff + 2 * kPreGroups * kPreRows * 4;  // floats [masks][128]: a step's factor
+  static constexpr int kEndOff = kOldOff + kPreMasks * kPreRows * 4;       // floats [2 segments][sum, ref][128]
+  static constexpr int kNanOff = kEndOff + 4 * kPreRows * 4;  // bytes [masks][NB][16 token groups]
+  static constexpr int kStageOff = kNanOff + kPreMasks * NB * 16;  // 32 rows x 16 elements a warp
+  static constexpr int kBarOff = kStageOff + (kPreSoft / 32 + 4) * 32 * kStageRow;
+  static constexpr int kBars = 2 * kPreRaw + 4 * kPreStages + 12 + 2 * kPreSegs;
   static constexpr int kBytes = kBarOff + 8 * kBars + 64 + 16 * kPreSegs / 4 + kPreSegs * (int)sizeof(PreSegment);
   static constexpr int kAlloc = kBytes + 1024;  // slack for 1024-byte alignment
   static_assert(kAlloc <= 227 * 1024, "shared memory");
@@ -76,8 +79,9 @@ struct PreSmem {
 };
 
 // TMEM columns. P replaces S in place: the 16 columns of 16 tokens' scores
-// become 8 of their weights' hi parts and 8 of the lo parts.
-constexpr uint32_t kTmQ = 0;    // hi [0, hd / 2), lo [64, 64 + hd / 2)
+// become 8 of their weights' hi parts and 8 of the lo parts; Q likewise
+// replaces its own fp32 elements.
+constexpr uint32_t kTmQ = 0;    // hd
 constexpr uint32_t kTmS = 128;  // 2 x 128: even and odd steps
 constexpr uint32_t kTmO = 384;  // hd
 
@@ -110,10 +114,6 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t *r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tm_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-               : "memory");
 }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -163,8 +163,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   uint64_t *raw_full = reinterpret_cast<uint64_t *>(sm + L::kBarOff), *raw_empty = raw_full + kPreRaw;
   uint64_t *k_full = raw_empty + kPreRaw, *k_empty = k_full + kPreStages;
   uint64_t *v_full = k_empty + kPreStages, *v_empty = v_full + kPreStages;
-  uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 1,
-           *fin = o_full + 1, *seg_full = fin + 1, *seg_empty = seg_full + kPreSegs;
+  uint64_t *q_full = v_empty + kPreStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2,
+           *fin = o_full + 1, *o_free = fin + 1, *end_full = o_free + 1, *end_empty = end_full + 2,
+           *seg_full = end_empty + 2, *seg_empty = seg_full + kPreSegs;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + kPreSegs);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   uint32_t *raw_valid = tmem_slot + 2;   // [kPreRaw]: the packed units that were copied
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   volatile int *soft_kind = reinterpret_cast<volatile int *>(const_cast<uint32_t *>(nan_step) + kPreMasks);
   PreSegment *segs = reinterpret_cast<PreSegment *>(const_cast<int *>(soft_kind) + 1);
   float *xch = reinterpret_cast<float *>(sm + L::kXchOff);
+  float *olds = reinterpret_cast<float *>(sm + L::kOldOff), *ends = reinterpret_cast<float *>(sm + L::kEndOff);
   uint8_t *nan_bits = sm + L::kNanOff;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -184,10 +186,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     }
     sm100::mbar_init(q_full, kPreSoft);
     sm100::mbar_init(&s_full[0], 1), sm100::mbar_init(&s_full[1], 1);
-    sm100::mbar_init(p_full, kPreSoft);
+    // (two of each: the softmax may be a step ahead of the MMAs, and a parity tells only neighbouring phases apart)
+    sm100::mbar_init(&p_full[0], kPreSoft), sm100::mbar_init(&p_full[1], kPreSoft);
     sm100::mbar_init(o_full, 1);
     sm100::mbar_init(fin, 1);
-    for (int i = 0; i < kPreSegs; ++i) sm100::mbar_init(&seg_full[i], 1), sm100::mbar_init(&seg_empty[i], 11);
+    sm100::mbar_init(o_free, 128);
+    for (int i = 0; i < 2; ++i) sm100::mbar_init(&end_full[i], 128), sm100::mbar_init(&end_empty[i], 128);
+    for (int i = 0; i < kPreSegs; ++i) sm100::mbar_init(&seg_full[i], 1), sm100::mbar_init(&seg_empty[i], 15);
     *abort = 0;
     for (int i = 0; i < kPreMasks; ++i) nan_step[i] = ~0u;
     sm100::fence_mbar_init();
@@ -221,17 +226,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       sg.next();
     };
 
-    if (warp < kWarpK) {
+    if (warp < kWarpOut) {
       // -------------------------------------------------------- softmax
-      set_regs_up<152>();
       const int grp = warp >> 2, row = 32 * (warp & 3) + lane;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-      uint32_t o_phase = 0;
-      Ring<2> score;
-      uint8_t *stage = sm + L::kStageOff + warp * 16 * L::kStageRow;
-      uint32_t step = 0;  // of this CTA, counted by the decode warps alike
-      Ring<kPreMasks> mask, smask;  // of the output's and of the scores' step
-      int parity = 0;               // of the exchange buffers
+      uint8_t *stage = sm + L::kStageOff + warp * 32 * kStageRow;
+      Ring<2> score, end;
+      Ring<kPreMasks> mask;
+      int parity = 0;  // of the exchange buffers
       bool ok = true;
       // The values of this row's threads, by `join`.
       auto exchange = [&](float mine, auto join) {
@@ -243,8 +245,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       };
       auto larger = [](float x, float y) { return fmaxf(x, y); };
       auto plus = [](float x, float y) { return x + y; };
-      auto either = [](float x, float y) { return __uint_as_float(__float_as_uint(x) | __float_as_uint(y)); };
-      constexpr int QC = HD / kPreGroups;  // elements and output columns of a thread
+      constexpr int QC = HD / kPreGroups;  // query elements of a thread
       static_assert(kPreGroups == 2, "");
       for (;;) {
         // One warp waits for the segment and decides for all, whatever comes: they share barriers.
@@ -253,113 +254,93 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           if (lane == 0) *soft_kind = got ? segs[sg.i].kind : (int)kSegEnd;
         }
         softmax_sync();
-        const int kind = *soft_kind;
-        if (kind == kSegEnd) break;
+        if (*soft_kind == kSegEnd) break;
         const PreSegment &s = segs[sg.i];
         const int steps = s.steps, f = s.tile * kPreRows + row, qi = f / a.group;
         const bool real = f < s.flat;
         // The last token that the row sees, from the first of this thread's.
         int see = (real ? min(s.base + qi, s.len - 1) : -1) - s.t0 * kPreTokens - kPreCols * grp;
-        const bool sees = real && min(s.base + qi, s.len - 1) >= 0;
-        const int64_t out_row = s.row0 + qi, head = s.head * a.group + f % a.group;
-        uint64_t acc[QC / 2], sums = 0;  // pairs; two sums of the weights
-#pragma unroll
-        for (int i = 0; i < QC / 2; ++i) acc[i] = 0;
+        uint64_t sums = 0;  // of the weights, two
         float ref = -INFINITY;
-        uint32_t poison = 0;
         if (steps > 0) {
-          // ---- the thread's part of the row's elements, scaled so that the row's largest is in [2^14, 2^15)
-          float x[QC], mx = 0.0f;
-          const float *p = real ? a.q + out_row * a.ld_q + head * a.hs_q + grp * QC : nullptr;
-          // Read along the rows and handed out by row, 16 rows at a time.
-          float4 v[QC / 4];
+          // ---- the thread's half of the row's elements, scaled so that the row's largest is in [2^14, 2^15). They are
+          // read along the rows, handed out by row through shared memory, and kept in Q's place until the row's
+          // largest is known. (The scores of the segment before are complete, so no MMA reads Q.)
+          const bool sees = real && min(s.base + qi, s.len - 1) >= 0;
+          const float *p = real ? a.q + (int64_t)(s.row0 + qi) * a.ld_q +
+                                      (int64_t)(s.head * a.group + f % a.group) * a.hs_q + grp * QC
+                                : nullptr;
+          const uint32_t keep = lanes + kTmQ + QC * grp;
+          float4 v[QC / 16][4];
 #pragma unroll
-          for (int i = 0; i < QC / 4; ++i) {
-            const int at = 32 * (i % (QC / 8)) + lane, r = 16 * (i / (QC / 8)) + at / (QC / 4), e = at % (QC / 4);
+          for (int i = 0; i < 4; ++i) {
             const float *src = reinterpret_cast<const float *>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), r));
-            v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (src) {
-              if (a.vec_q) v[i] = *reinterpret_cast<const float4 *>(src + 4 * e);
-              else v[i] = make_float4(src[4 * e], src[4 * e + 1], src[4 * e + 2], src[4 * e + 3]);
-            }
-          }
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), 8 * i + (lane >> 2)));
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-#pragma unroll
-            for (int i = 0; i < QC / 8; ++i) {
-              const int at = 32 * i + lane;
-              *reinterpret_cast<float4 *>(stage + at / (QC / 4) * L::kStageRow + 16 * (at % (QC / 4))) =
-                  v[half * (QC / 8) + i];
-            }
-            __syncwarp();
-            if (lane >> 4 == half) {
-#pragma unroll
-              for (int i = 0; i < QC; i += 4) {
-                const float4 u = *reinterpret_cast<const float4 *>(stage + (lane & 15) * L::kStageRow + 4 * i);
-                x[i] = u.x, x[i + 1] = u.y, x[i + 2] = u.z, x[i + 3] = u.w;
+            for (int c = 0; c < QC / 16; ++c) {
+              const int e = 16 * c + 4 * (lane & 3);
+              v[c][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (src) {
+                if (a.vec_q) v[c][i] = *reinterpret_cast<const float4 *>(src + e);
+                else v[c][i] = make_float4(src[e], src[e + 1], src[e + 2], src[e + 3]);
               }
             }
-            __syncwarp();
           }
+          float mx = 0.0f;
           bool bad = false;
 #pragma unroll
-          for (int i = 0; i < QC; ++i) mx = fmaxf(mx, fabsf(x[i])), bad |= !isfinite(x[i]);
-          if (bad) mx = INFINITY;
-          mx = exchange(mx, larger);
+          for (int c = 0; c < QC / 16; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float4 *>(stage + (8 * i + (lane >> 2)) * kStageRow + 16 * (lane & 3)) = v[c][i];
+            __syncwarp();
+            uint32_t r[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 u = *reinterpret_cast<const uint4 *>(stage + lane * kStageRow + 16 * i);
+              r[4 * i] = u.x, r[4 * i + 1] = u.y, r[4 * i + 2] = u.z, r[4 * i + 3] = u.w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = __uint_as_float(r[i]);
+              mx = fmaxf(mx, fabsf(x)), bad |= !isfinite(x);
+            }
+            tm_st16(keep + 16 * c, r);
+          }
+          tm_st_wait();
+          mx = exchange(bad ? INFINITY : mx, larger);
           bad = mx == INFINITY;
           const int e = min(141 - (int)(__float_as_uint(mx) >> 23), 126);
           float up = __uint_as_float((uint32_t)(127 + e) << 23);
           if (a.scale < 0.0f) up = -up;  // f is positive: the largest S is the largest score
           // (never 0, so that f * -inf is -inf; a row that sees nothing is 0 whatever its query)
           const float scale = bad && sees ? __uint_as_float(0x7fc00000u) : fmaxf(ldexpf(fabsf(a.scale), -e), 1.2e-38f);
+#pragma unroll 1
+          for (int c = 0; c < QC / 16; ++c) {
+            uint32_t r[16], w[16];
+            tm_ld16(keep + 16 * c, r);
+            sm100::tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < QC / 8; ++c) {  // 8 elements, in the order of a decoded word
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) split_f16(x[8 * c + i] * up, x[8 * c + i + 4] * up, hi[i], lo[i]);
-            const uint32_t col = grp * (QC / 2) + 4 * c;
-            tm_st4(lanes + kTmQ + col, hi[0], hi[1], hi[2], hi[3]);
-            tm_st4(lanes + kTmQ + 64 + col, lo[0], lo[1], lo[2], lo[3]);
+            for (int i = 0; i < 8; ++i) {  // in the order of a decoded word: elements 0, 4, 1, 5, ... of every 8
+              const int x = 8 * (i >> 2) + (i & 3);
+              split_f16(__uint_as_float(r[x]) * up, __uint_as_float(r[x + 4]) * up, w[i], w[8 + i]);
+            }
+            tm_st16(keep + 16 * c, w);
           }
           tm_st_wait();
           sm100::tc_fence_before();
           sm100::mbar_arrive(q_full);
 
-          auto add_output = [&](int see) {  // O of a step
-            ok = wait(o_full, o_phase) && ok;
-            o_phase ^= 1u;
-            sm100::tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < QC; c += 16) {
-              uint32_t r[16];
-              tm_ld16(lanes + kTmO + grp * QC + c, r);
-              sm100::tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; i += 2)
-                acc[(c + i) / 2] = add_two(acc[(c + i) / 2], two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
-            }
-            // NaN values of the step entered as 0: the rows that see them are marked.
-            if (nan_step[mask.i] == step) {
-              const uint64_t *bits = reinterpret_cast<const uint64_t *>(nan_bits + mask.i * NB * 16 + 8 * grp);
-              const uint64_t mine = see < 0 ? 0 : see >= 63 ? ~0ull : (2ull << see) - 1;
-#pragma unroll
-              for (int b = 0; b < NB; ++b)
-                if (bits[2 * b] & mine) poison |= 1u << b;
-            }
-            ++step;
-            mask.next();
-          };
-
           for (int k = 0; k < steps; ++k) {
             ok = wait(&s_full[score.i], score.phase) && ok;
             const uint32_t cols = lanes + kTmS + 128 * score.i + kPreCols * grp;
+            uint64_t *done = &p_full[score.i];
             score.next();
             sm100::tc_fence_after();
-            const uint32_t units = unit_mask[smask.i] >> (4 * grp) & 15u;
-            smask.next();
-            // (Loops of 16 columns keep the instruction cache: unrolled further, the roles' code evicted itself and
-            // a step took three times as long.)
+            const uint32_t units = unit_mask[mask.i] >> (4 * grp) & 15u;
+            // (Loops of 16 and 32 columns keep the instruction cache: unrolled further, the roles' code evicted itself
+            // and a step took three times as long.)
             // Hide what the row does not see (TMEM is read and written by whole warps).
             if (__any_sync(0xffffffffu, see < 63 || units != 15u)) {
 #pragma unroll 1
@@ -392,6 +373,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               old = ex2(ref - to);
               ref = to;
             }
+            if (grp == 0) olds[mask.i * kPreRows + row] = old;
+            mask.next();
             const float shift = ref == -INFINITY ? 0.0f : ref;
             const uint64_t shifts = two(-shift, -shift), scales = two(scale, scale);
             sums = mul_two(sums, two(old, old));
@@ -411,62 +394,120 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               tm_st16(cols + c, w[0]);
               tm_st16(cols + c + 16, w[1]);
             }
-            if (k > 0) add_output(see + kPreTokens);
-            if (__any_sync(0xffffffffu, old != 1.0f)) {
-#pragma unroll
-              for (int i = 0; i < QC / 2; ++i) acc[i] = mul_two(acc[i], two(old, old));
-            }
             tm_st_wait();
             sm100::tc_fence_before();
-            sm100::mbar_arrive(p_full);
+            sm100::mbar_arrive(done);
             see -= kPreTokens;
           }
-          add_output(see + kPreTokens);
         }
-        // ---- the row's end
+        // ---- the rows' ends, for the output's warps
         const float2 halves = of_two(sums);
         const float total = exchange(halves.x + halves.y, plus);
-        poison = __float_as_uint(exchange(__uint_as_float(poison), either));
         if (threadIdx.x == 0) sm100::mbar_arrive(&seg_empty[sg.i]);  // all have read it
         sg.next();
-        const bool whole = kind == kSegWhole;
-        if (!ok) poison = ~0u;
+        if (grp == 0) {
+          ok = wait(&end_empty[end.i], end.phase ^ 1u) && ok;
+          ends[2 * end.i * kPreRows + row] = ok ? total : __uint_as_float(0x7fc00000u);
+          ends[(2 * end.i + 1) * kPreRows + row] = ref;
+          sm100::mbar_arrive(&end_full[end.i]);
+          end.next();
+        }
+      }
+    } else if (warp < kWarpK) {
+      // -------------------------------------------------------- the running output
+      set_regs_up<160>();
+      const int row = 32 * (warp & 3) + lane;
+      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+      uint8_t *stage = sm + L::kStageOff + warp * 32 * kStageRow;
+      uint32_t o_phase = 0, step = 0;  // steps of this CTA, counted by the decode warps alike
+      Ring<kPreMasks> mask;
+      Ring<2> end;
+      bool ok = true;
+      auto all_wait = [&](uint64_t *bar, uint32_t phase) { return __all_sync(0xffffffffu, wait(bar, phase)) != 0; };
+      for (; ok && seg_next(); seg_done()) {
+        const PreSegment &s = segs[sg.i];
+        const int steps = s.steps, f = s.tile * kPreRows + row, qi = f / a.group;
+        const bool real = f < s.flat;
+        int see = (real ? min(s.base + qi, s.len - 1) : -1) - s.t0 * kPreTokens;  // the last token that the row sees
+        uint64_t acc[HD / 2];  // pairs
+#pragma unroll
+        for (int i = 0; i < HD / 2; ++i) acc[i] = 0;
+        uint32_t poison = 0;
+        for (int k = 0; ok && k < steps; ++k) {
+          ok = all_wait(o_full, o_phase);
+          o_phase ^= 1u;
+          sm100::tc_fence_after();
+          const float old = olds[mask.i * kPreRows + row];
+          if (__any_sync(0xffffffffu, old != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < HD / 2; ++i) acc[i] = mul_two(acc[i], two(old, old));
+          }
+#pragma unroll
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t r[16];
+            tm_ld16(lanes + kTmO + c, r);
+            sm100::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+              acc[(c + i) / 2] = add_two(acc[(c + i) / 2], two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+          }
+          sm100::tc_fence_before();
+          sm100::mbar_arrive(o_free);
+          // NaN values of the step entered as 0: the rows that see them are marked.
+          if (nan_step[mask.i] == step) {
+            const uint64_t *bits = reinterpret_cast<const uint64_t *>(nan_bits + mask.i * NB * 16);
+            auto upto = [](int n) { return n < 0 ? 0 : n >= 63 ? ~0ull : (2ull << n) - 1; };
+            const uint64_t m0 = upto(see), m1 = upto(see - 64);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              if ((bits[2 * b] & m0) | (bits[2 * b + 1] & m1)) poison |= 1u << b;
+          }
+          ++step;
+          mask.next();
+          see -= kPreTokens;
+        }
+        ok = all_wait(&end_full[end.i], end.phase) && ok;
+        const float total = ok ? ends[2 * end.i * kPreRows + row] : __uint_as_float(0x7fc00000u);
+        const float ref = ends[(2 * end.i + 1) * kPreRows + row];
+        sm100::mbar_arrive(&end_empty[end.i]);
+        end.next();
+        const bool whole = s.kind == kSegWhole;
         float *dst = nullptr;
         float inv = 1.0f;
+        if (!ok) poison = ~0u;
         if (real && whole) {
-          dst = a.out + out_row * a.ld_o + head * a.hs_o + grp * QC;
+          dst = a.out + (int64_t)(s.row0 + qi) * a.ld_o + (int64_t)(s.head * a.group + f % a.group) * a.hs_o;
           inv = total == 0.0f ? 0.0f : 1.0f / total;
         } else if (real) {
-          float *part = a.parts + (int64_t)(2 * blockIdx.x + (kind == kSegHead)) * kv4_part_floats(kPreRows, HD);
-          dst = part + 2 * kPreRows + row * HD + grp * QC;
-          if (grp == 0) part[row] = ref, part[kPreRows + row] = total;
+          float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.kind == kSegHead)) * kv4_part_floats(kPreRows, HD);
+          dst = part + 2 * kPreRows + row * HD;
+          part[row] = ref, part[kPreRows + row] = total;
         }
         const bool vec = a.vec_o || !whole;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {  // 16 rows at a time, written along the rows
-          if (lane >> 4 == half) {
+        float *to[4];  // of the rows that this lane writes parts of
 #pragma unroll
-            for (int i = 0; i < QC; i += 4) {
-              const float2 u = of_two(mul_two(acc[i / 2], two(inv, inv)));
-              const float2 v = of_two(mul_two(acc[i / 2 + 1], two(inv, inv)));
-              float4 o = make_float4(u.x, u.y, v.x, v.y);
-              if (poison >> ((grp * QC + i) / 32) & 1u) {
-                const float n = __uint_as_float(0x7fc00000u);
-                o = make_float4(n, n, n, n);
-              }
-              *reinterpret_cast<float4 *>(stage + (lane & 15) * L::kStageRow + 4 * i) = o;
-            }
+        for (int i = 0; i < 4; ++i)
+          to[i] = reinterpret_cast<float *>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), 8 * i + (lane >> 2)));
+#pragma unroll
+        for (int c = 0; c < HD; c += 16) {
+          const float nan = __uint_as_float(0x7fc00000u);
+          const bool dead = poison >> (c / 32) & 1u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = of_two(mul_two(acc[(c + 4 * i) / 2], two(inv, inv)));
+            const float2 v = of_two(mul_two(acc[(c + 4 * i) / 2 + 1], two(inv, inv)));
+            *reinterpret_cast<float4 *>(stage + lane * kStageRow + 16 * i) =
+                dead ? make_float4(nan, nan, nan, nan) : make_float4(u.x, u.y, v.x, v.y);
           }
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < QC / 8; ++i) {
-            const int at = 32 * i + lane, r = at / (QC / 4), e = at % (QC / 4);
-            float *d = reinterpret_cast<float *>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), 16 * half + r));
-            const float4 o = *reinterpret_cast<const float4 *>(stage + r * L::kStageRow + 16 * e);
-            if (d) {
-              if (vec) *reinterpret_cast<float4 *>(d + 4 * e) = o;
-              else d[4 * e] = o.x, d[4 * e + 1] = o.y, d[4 * e + 2] = o.z, d[4 * e + 3] = o.w;
+          for (int i = 0; i < 4; ++i) {
+            const float4 o = *reinterpret_cast<const float4 *>(stage + (8 * i + (lane >> 2)) * kStageRow + 16 * (lane & 3));
+            if (to[i]) {
+              float *d = to[i] + c + 4 * (lane & 3);
+              if (vec) *reinterpret_cast<float4 *>(d) = o;
+              else d[0] = o.x, d[1] = o.y, d[2] = o.z, d[3] = o.w;
             }
           }
           __syncwarp();
@@ -481,7 +522,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       const uint32_t src0 = L::kRawOff + u0 * UB + tk * (16 * NB) + t * (4 * NB);
       const uint32_t scale0 = L::kRawOff + u0 * UB + kv4_k_scale_off(NB) + tk * (2 * NB);
       const uint32_t dst0 = L::kKOff + tk0 * 128 + ((t ^ (lane & 7)) << 4);  // even blocks; odd ones are 64 bytes away
-      set_regs_down<64>();
+      set_regs_down<56>();
       Ring<kPreRaw> raw;
       Ring<kPreStages> st;
       Ring<kPreMasks> mask;
@@ -540,7 +581,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
       const uint32_t scale0 = L::kRawOff + (m >> 1) * UB + kv4_v_scale_off(NB) + (8 * odd) * (2 * NB);
       const uint32_t dst0 = L::kVOff + (m >> 3) * L::kVPanel + 4 * g * 128;
       uint32_t step = 0;
-      set_regs_down<64>();
+      set_regs_down<56>();
       Ring<kPreRaw> raw;
       Ring<kPreStages> st;
       Ring<kPreMasks> mask;
@@ -626,8 +667,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         const uint64_t k_desc = sm100::umma_desc_sw128(sm100::smem_u32(sm + L::kKOff));
         const uint64_t v_desc = sm100::umma_desc_sw128(sm100::smem_u32(sm + L::kVOff));
         Ring<kPreStages> ks, vs;
-        uint32_t q_phase = 0, p_phase = 0;
-        int sb = 0, pb = 0;  // S buffers of the next scores and of the next output
+        uint32_t q_phase = 0, free_phase = 1;  // O is free at first
+        int sb = 0;     // S buffer of the next scores
+        Ring<2> pbuf;  // of the next output
         bool ok = true;
         auto all_wait = [&](uint64_t *bar, uint32_t parity) {
           return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs)) != 0;
@@ -648,7 +690,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               for (int part = 0; part < 2; ++part)
 #pragma unroll
                 for (int kk = 0; kk < 2 * NB; ++kk)
-                  umma_f16_ts(d, tmem + kTmQ + 64 * part + 8 * kk, desc + (kk >> 2) * (L::kPanel >> 4) + 2 * (kk & 3),
+                  umma_f16_ts(d, tmem + kTmQ + 16 * kk + 8 * part, desc + (kk >> 2) * (L::kPanel >> 4) + 2 * (kk & 3),
                               id_s, part || kk);
               sm100::umma_commit(&s_full[sb]);
               sm100::umma_commit(&k_empty[ks.i]);
@@ -661,11 +703,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           if (!(ok = scores())) break;
           for (int k = 0; k < steps; ++k) {
             if (k + 1 < steps && !(ok = scores())) break;
-            if (!(ok = all_wait(&v_full[vs.i], vs.phase) && all_wait(p_full, p_phase))) break;
-            p_phase ^= 1u;
+            if (!(ok = all_wait(&v_full[vs.i], vs.phase) && all_wait(&p_full[pbuf.i], pbuf.phase) && all_wait(o_free, free_phase)))
+              break;
+            free_phase ^= 1u;
             sm100::tc_fence_after();
             const uint64_t desc = v_desc + (uint64_t)(vs.i * (L::kV >> 4));
-            const uint32_t p = tmem + kTmS + 128 * pb;
+            const uint32_t p = tmem + kTmS + 128 * pbuf.i;
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < kPreTokens / 16; ++kk)
@@ -678,7 +721,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             }
             __syncwarp();
             vs.next();
-            pb ^= 1;
+            pbuf.next();
           }
         }
         if (elect_one()) {  // every MMA has completed before the TMEM is released
