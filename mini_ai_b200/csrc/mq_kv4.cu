@@ -120,10 +120,14 @@ size_t parts_bytes(int ctas, int row_tile, int hd) {
 int dec_ctas(int sms) { return 3 * sms; }
 
 // Flat rows (rows of a request times the query heads of a KV head) up to which
-// the few-row kernel takes a request: it runs 8 of them at a time.
+// the few-row kernel takes a request: it runs 8 of them at a time, and its time
+// grows with every 8. 16 requests of 4000 tokens, 8 KV heads of 128: 91 us
+// against the many-row kernel's 96 at 24 rows, 114 against 97 at 28.
 constexpr int kFewRows = 24;
 // Requests that cannot be longer are not cut, which spares the joining kernel.
-constexpr int kShortTokens = 512;
+// One request (8, 64) of 256 tokens: 8.7 us (9.9, 18.6) whole, 9.5 (11.2, 20.4)
+// cut; of 512 tokens: 12.0 (14.1, 28.0) whole, 9.2 (11.7, 27.2) cut.
+constexpr int kShortTokens = 256;
 bool many_rows(int group, int max_new) { return (int64_t)group * max_new > kFewRows; }
 
 void use_workspace(Kv4AttnArgs &a, uint8_t *ws, int ctas) {

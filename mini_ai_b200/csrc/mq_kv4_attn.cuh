@@ -58,10 +58,12 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return a / b;
 }
 
-// What beginning and ending an item costs, in steps of BN tokens (measured:
-// 18000 clocks against 4100 of a step of the many-row kernel).
+// What beginning and ending an item costs, in steps of BN tokens. Without it
+// the CTAs with many short items end last: a 4096-token prompt took 561 us
+// instead of 372. 4 for the many-row kernel (299 us; 3: 301, 6: 310), 1 for the
+// other (48 ragged chats 90.5 us; 2: 91.1, 4: 96.7).
 template <int RT>
-constexpr int kv4_setup() { return RT == 128 ? 4 : 2; }
+constexpr int kv4_setup() { return RT == 128 ? 4 : 1; }
 
 // Work of the first n row tiles of a request: for each its setup, then its steps. With `period` = G BN / RT row
 // tiles to a step of BN tokens, and the tokens before the request's rows

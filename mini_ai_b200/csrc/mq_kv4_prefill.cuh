@@ -271,34 +271,39 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
                                       (int64_t)(s.head * a.group + f % a.group) * a.hs_q + grp * QC
                                 : nullptr;
           const uint32_t keep = lanes + kTmQ + QC * grp;
-          float4 v[QC / 16][4];
+          const float *src[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float *src = reinterpret_cast<const float *>(
+          for (int i = 0; i < 4; ++i)
+            src[i] = reinterpret_cast<const float *>(
                 __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), 8 * i + (lane >> 2)));
+          auto load = [&](int c, float4 (&v)[4]) {
+            const int e = 16 * c + 4 * (lane & 3);
 #pragma unroll
-            for (int c = 0; c < QC / 16; ++c) {
-              const int e = 16 * c + 4 * (lane & 3);
-              v[c][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if (src) {
-                if (a.vec_q) v[c][i] = *reinterpret_cast<const float4 *>(src + e);
-                else v[c][i] = make_float4(src[e], src[e + 1], src[e + 2], src[e + 3]);
+            for (int i = 0; i < 4; ++i) {
+              v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (src[i]) {
+                if (a.vec_q) v[i] = *reinterpret_cast<const float4 *>(src[i] + e);
+                else v[i] = make_float4(src[i][e], src[i][e + 1], src[i][e + 2], src[i][e + 3]);
               }
             }
-          }
+          };
+          float4 v[4], next[4];
+          load(0, v);
           float mx = 0.0f;
           bool bad = false;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < QC / 16; ++c) {
+            if (c + 1 < QC / 16) load(c + 1, next);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<float4 *>(stage + (8 * i + (lane >> 2)) * kStageRow + 16 * (lane & 3)) = v[c][i];
+              *reinterpret_cast<float4 *>(stage + (8 * i + (lane >> 2)) * kStageRow + 16 * (lane & 3)) = v[i];
             __syncwarp();
             uint32_t r[16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint4 u = *reinterpret_cast<const uint4 *>(stage + lane * kStageRow + 16 * i);
               r[4 * i] = u.x, r[4 * i + 1] = u.y, r[4 * i + 2] = u.z, r[4 * i + 3] = u.w;
+              v[i] = next[i];
             }
             __syncwarp();
 #pragma unroll
@@ -339,8 +344,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             score.next();
             sm100::tc_fence_after();
             const uint32_t units = unit_mask[mask.i] >> (4 * grp) & 15u;
-            // (Loops of 16 and 32 columns keep the instruction cache: unrolled further, the roles' code evicted itself
-            // and a step took three times as long.)
+            // (Loops of 16 columns keep the instruction cache: unrolled further, the roles' code evicted itself and a
+            // step took up to three times as long.)
             // Hide what the row does not see (TMEM is read and written by whole warps).
             if (__any_sync(0xffffffffu, see < 63 || units != 15u)) {
 #pragma unroll 1
@@ -379,20 +384,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             const uint64_t shifts = two(-shift, -shift), scales = two(scale, scale);
             sums = mul_two(sums, two(old, old));
 #pragma unroll 1
-            for (int c = 0; c < kPreCols; c += 32) {
-              uint32_t r[32], w[2][16];
+            for (int c = 0; c < kPreCols; c += 16) {
+              uint32_t r[16], w[16];
               tm_ld16(cols + c, r);
-              tm_ld16(cols + c + 16, r + 16);
               sm100::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
+              for (int i = 0; i < 16; i += 2) {
                 const float2 z = of_two(fma_two(two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scales, shifts));
                 const float p0 = ex2(z.x), p1 = ex2(z.y);
                 sums = add_two(sums, two(p0, p1));
-                split_f16(p0, p1, w[i >> 4][(i & 15) >> 1], w[i >> 4][8 + ((i & 15) >> 1)]);
+                split_f16(p0, p1, w[i >> 1], w[8 + (i >> 1)]);
               }
-              tm_st16(cols + c, w[0]);
-              tm_st16(cols + c + 16, w[1]);
+              tm_st16(cols + c, w);
             }
             tm_st_wait();
             sm100::tc_fence_before();
@@ -536,7 +539,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
           if (threadIdx.x == kWarpK * 32) unit_mask[mask.i] = valid;
           const uint8_t *src = sm + src0 + raw.i * L::kRaw, *scale = sm + scale0 + raw.i * L::kRaw;
           uint8_t *dst = sm + dst0 + st.i * L::kK;
-#pragma unroll 2
+#pragma unroll 1
           for (int it = 0; it < 4; ++it) {
             uint32_t kw[NB], d[W];
             const uint8_t *kp = src + it * 2 * UB;
@@ -629,11 +632,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
                   }
               if (bad[0] | bad[1]) nan_step[mask.i] = step;
             }
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < (NB == 1 ? 1 : 2); ++h) {
               const int b = 2 * b2 + h;
               if (b >= NB) break;
-              if (g == 0) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)bad[h];
+              if (g == 0) nan_bits[(mask.i * NB + b) * 16 + m] = (uint8_t)(h ? bad[1] : bad[0]);
               const uint32_t sel = odd ? (h ? 0x3276u : 0x1054u) : (h ? 0x7632u : 0x5410u);
               uint32_t o[4][4];
 #pragma unroll

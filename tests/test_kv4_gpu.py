@@ -408,6 +408,33 @@ def test_long(mq, torch, heads, kv, hd, lens, news):
     assert_attention(torch, out[:-2], want, tol)
 
 
+@pytest.mark.parametrize("heads,kv,hd,lens,news", [
+    (32, 8, 64, [1500], [1400]), (32, 8, 128, [700, 900, 300], [700, 333, 300]), (40, 20, 32, [500] * 12, [400] * 12)])
+def test_many_items_a_cta(mq, torch, heads, kv, hd, lens, news):
+    """Many items follow one another in every CTA: its roles stay in step over many segments and steps."""
+    b = Batch(mq, torch, lens, kv, hd, 64, seed=15)
+    for again in range(3):
+        q, out = run_attention(torch, b, heads, news, 16, max_new=max(news))
+        if again:
+            assert torch.equal(out, first)
+        first = out
+    at = 0
+    for r, m in enumerate(news):  # all rows of a request share one product
+        group = heads // kv
+        k, v = (x.repeat_interleave(group, 1) for x in (b.hk[r], b.hv[r]))
+        qq = q[at:at + m].double()
+        s = torch.einsum("ihd,shd->his", qq, k) * hd ** -0.5
+        sees = torch.arange(lens[r], device="cuda") <= torch.arange(lens[r] - m, lens[r], device="cuda")[:, None]
+        p = torch.softmax(torch.where(sees, s, -math.inf), -1)
+        want = torch.einsum("his,shd->ihd", p, v)
+        size = torch.where(sees, torch.einsum("ihd,shd->his", qq.abs(), k.abs()), 0).amax(-1) * hd ** -0.5
+        rel = (2 * (size * (2 ** -22 + 44 * 2 ** -23) + 2 ** -21) + 256 * 2 ** -23).T
+        tol = rel[..., None] * torch.einsum("his,shd->ihd", p, v.abs())
+        tol += 2 ** -33 * p.amax(-1).T[..., None] * v.abs().sum(0)
+        assert_attention(torch, out[at:at + m], want, tol)
+        at += m
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
 def test_scales_and_sizes(mq, torch, scale):
     """Score scales of either sign, flat and one-hot softmaxes, queries and values of extreme sizes."""
