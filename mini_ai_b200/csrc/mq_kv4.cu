@@ -314,6 +314,7 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   if (rows == 0 || n_seqs == 0) return MQ_OK;
   if (int rc = check_rows("query", q, ld_q, hs_q, heads, c->v.hd)) return rc;
   if (int rc = check_rows("output", out, ld_out, hs_out, heads, c->v.hd)) return rc;
+  if (rows > 1 && ld_out < c->v.hd) return fail(MQ_ERR_INVALID, "output rows overlap (stride %lld)", (long long)ld_out);
   if (!offsets || !seq_lens || !block_tables) return fail(MQ_ERR_INVALID, "null offsets, lengths or block tables");
   const size_t need = mq_kv4_attention_workspace(c, heads, max_new);
   if (!workspace || workspace_bytes < need)

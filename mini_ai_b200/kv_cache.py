@@ -70,6 +70,12 @@ def _table(torch, t):
     return device, n, width, _ints(torch, "block_tables", t, max(device, 0), n * width)
 
 
+def _page(page_size: int) -> int:
+    if page_size > 1024:  # (a size of more bits would wrap on its way into C)
+        raise ValueError(f"page size {page_size}: a multiple of 16 up to 1024 is needed")
+    return page_size
+
+
 def _ok(rc: int, what: str) -> None:
     if rc == _lib.MQ_ERR_INVALID:
         raise ValueError(f"{what}: {_lib.last_error()}")
@@ -125,7 +131,7 @@ def PlanPages(ctx_lens, new_lens, block_tables, free_pages, n_free, page_size: i
     free = free_pages.numel()
     _ok(lib().mq_pages_plan(
         device, _ints(torch, "ctx_lens", ctx_lens, device, n), _ints(torch, "new_lens", new_lens, device, n), n,
-        page_size, tables, width, _ints(torch, "free_pages", free_pages, device, free), free,
+        _page(page_size), tables, width, _ints(torch, "free_pages", free_pages, device, free), free,
         _ints(torch, "n_free", n_free, device, 1), out._sizes[1], offsets, seq_lens, slots, positions, n_free_out,
         refused, _stream_on(torch, device, stream)), "PlanPages")
     return out
@@ -138,7 +144,7 @@ def ReleasePages(requests, seq_lens, block_tables, free_pages, n_free, page_size
     device, n, width, tables = _table(torch, block_tables)
     count, free = requests.numel(), free_pages.numel()
     _ok(lib().mq_pages_release(
-        device, _ints(torch, "requests", requests, device, count), count, n, page_size,
+        device, _ints(torch, "requests", requests, device, count), count, n, _page(page_size),
         _ints(torch, "seq_lens", seq_lens, device, n), tables, width,
         _ints(torch, "free_pages", free_pages, device, free), free, _ints(torch, "n_free", n_free, device, 1),
         _stream_on(torch, device, stream)), "ReleasePages")
@@ -154,6 +160,8 @@ class Kv4Cache:
                  stream=None):
         torch = _torch()
         self.handle = None
+        if max(layers, pages, page_size, kv_heads, head_dim) >= 1 << 31:  # would wrap on its way into C
+            raise ValueError("Kv4Cache: cache size overflow")
         need = lib().mq_kv4_bytes(layers, pages, page_size, kv_heads, head_dim)
         if not need:
             raise ValueError(f"Kv4Cache: {_lib.last_error()}")
@@ -173,6 +181,11 @@ class Kv4Cache:
         n = C.c_size_t()
         check(lib().mq_kv4_info(self.handle, None, None, None, None, None, None, C.byref(n)))
         return n.value
+
+    def _layer(self, layer: int) -> int:
+        if 0 <= layer < self.layers:
+            return layer
+        raise ValueError(f"layer {layer} of {self.layers}")
 
     def _rows(self, torch, name: str, t, rows: int | None, heads: int | None):
         """(shape, strides) of F32 `t` [rows, heads, head_dim] whose heads are contiguous."""
@@ -194,7 +207,7 @@ class Kv4Cache:
         torch = _torch()
         (rows, _, _), (ld_k, hs_k, _) = self._rows(torch, "keys", k, None, self.kv_heads)
         _, (ld_v, hs_v, _) = self._rows(torch, "values", v, rows, self.kv_heads)
-        _ok(lib().mq_kv4_store(self.handle, layer, k.data_ptr(), ld_k, hs_k, v.data_ptr(), ld_v, hs_v,
+        _ok(lib().mq_kv4_store(self.handle, self._layer(layer), k.data_ptr(), ld_k, hs_k, v.data_ptr(), ld_v, hs_v,
                                _ints(torch, "slots", slots, self.device, rows), rows,
                                _stream_on(torch, self.device, stream)), "Kv4Cache.store")
 
@@ -209,7 +222,7 @@ class Kv4Cache:
             k, v = slots.new_empty(shape, dtype=torch.float32), slots.new_empty(shape, dtype=torch.float32)
         else:
             k, v = (_empty(torch, shape, torch.float32, slots.device, stream) for _ in range(2))
-        _ok(lib().mq_kv4_load(self.handle, layer, at, rows, k.data_ptr(), v.data_ptr(), sh), "Kv4Cache.load")
+        _ok(lib().mq_kv4_load(self.handle, self._layer(layer), at, rows, k.data_ptr(), v.data_ptr(), sh), "Kv4Cache.load")
         return k, v
 
     def attention(self, layer: int, q, offsets, seq_lens, block_tables, max_new: int | None = None,
@@ -238,12 +251,12 @@ class Kv4Cache:
         (out_rows, _, _), (ld_o, hs_o, _) = self._rows(torch, "output", out, None, heads)
         if out_rows < rows:
             raise RuntimeError(f"output: shape mismatch ({out_rows} rows, {rows} of queries)")
-        if max_new is None:
+        if max_new is None or max_new > rows:
             max_new = rows
         need = lib().mq_kv4_attention_workspace(self.handle, heads, max_new)
         ws = _empty(torch, need, torch.uint8, q.device, stream)
         _ok(lib().mq_kv4_attention(
-            self.handle, layer, q.data_ptr(), ld_q, hs_q, rows, heads, _ints(torch, "offsets", offsets, device, n + 1),
+            self.handle, self._layer(layer), q.data_ptr(), ld_q, hs_q, rows, heads, _ints(torch, "offsets", offsets, device, n + 1),
             _ints(torch, "seq_lens", seq_lens, device, n), tables, n, width, max_new,
             1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(), ld_o, hs_o, ws.data_ptr(),
             need, sh), "Kv4Cache.attention")

@@ -579,7 +579,7 @@ def test_cache_past_4gib(mq, torch, news):
 def test_refusals(mq, torch):
     c = mq.Kv4Cache(2, 4, 16, 2, 64)
     x, at = torch.zeros(3, 2, 64, device="cuda"), ints(torch, [0, 1, 2])
-    for layer in (-1, 2):
+    for layer in (-1, 2, 1 << 32):
         with pytest.raises(ValueError, match="layer"):
             c.store(layer, x, x, at)
         with pytest.raises(ValueError, match="layer"):
@@ -608,6 +608,11 @@ def test_refusals(mq, torch):
             c.attention(0, q, offsets, lens, tables, scale=scale)
     with pytest.raises(ValueError):
         c.attention(0, q, offsets, lens, tables, max_new=-1)
+    assert torch.equal(c.attention(0, q, offsets, lens, tables, max_new=1 << 40), c.attention(0, q, offsets, lens, tables))
+    with pytest.raises(ValueError, match="overflow"):
+        mq.Kv4Cache(1, (1 << 32) + 4, 16, 2, 64)
+    with pytest.raises(ValueError, match="page size"):
+        mq.ReleasePages(at, lens, tables, at, at[:1], (1 << 32) + 16)
     lib, e = mq.lib(), mq._lib
     need = lib.mq_kv4_attention_workspace(c.handle, 4, 3)
     assert need > 0
@@ -619,7 +624,7 @@ def test_refusals(mq, torch):
     torch.cuda.synchronize()
     assert call() == e.MQ_OK
     for kw in (dict(rows=-1), dict(heads=0), dict(n=-1), dict(width=0), dict(q=None), dict(out=None), dict(offsets=None),
-               dict(lens=None), dict(tables=None), dict(hsq=63), dict(hso=32), dict(ldq=-1), dict(q=q.data_ptr() + 2)):
+               dict(lens=None), dict(tables=None), dict(hsq=63), dict(hso=32), dict(ldq=-1), dict(ldo=0), dict(q=q.data_ptr() + 2)):
         assert call(**kw) == e.MQ_ERR_INVALID, kw
     for kw in (dict(ws=None), dict(bytes=need - 1)):
         assert call(**kw) == e.MQ_ERR_SIZE, kw
