@@ -186,7 +186,8 @@ typedef struct mq_kv4 mq_kv4;
 size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head_dim);
 
 /* A cache of zeros on `device`. page_size: a multiple of 16 up to 1024;
- * head_dim: 32, 64, 96 or 128; pages * page_size < 2^31. `memory` is the
+ * head_dim: 32, 64, 96 or 128; kv_heads up to 65536; pages * page_size <
+ * 2^31. `memory` is the
  * caller's device memory for it (at least mq_kv4_bytes(), 16-byte aligned),
  * which must outlive the handle and is cleared on `stream`; NULL allocates
  * it, which synchronizes `stream`. */

@@ -58,8 +58,12 @@ bool vector16(const void *p, int64_t ld, int64_t hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0 && hs % 4 == 0;
 }
 
-// Whether the blocks that so many CTAs of a store or load pack count in 32 bits.
-bool fits32(int64_t ctas) { return ctas * kKv4Blocks < (int64_t)1 << 32; }
+// CTAs of a store or load: one for the rows that it holds at a time, or as many as the device takes at once.
+dim3 row_grid(const mq_kv4 *c, int rows) {
+  const int per_row = 2 * c->v.kv * c->v.nb, parts = (per_row + kKv4Quads - 1) / kKv4Quads;
+  const int64_t want = ((int64_t)rows + kv4_whole(per_row) - 1) / kv4_whole(per_row);
+  return dim3((unsigned)std::min<int64_t>(want, std::max(1, 8 * c->sms / std::min(parts, 8))), (unsigned)parts);
+}
 
 int check_cache(const mq_kv4 *c, int layer) {
   if (!c) return fail(MQ_ERR_INVALID, "null cache handle");
@@ -68,7 +72,7 @@ int check_cache(const mq_kv4 *c, int layer) {
 }
 
 int cache_shape(int layers, int pages, int page_size, int kv_heads, int head_dim, Kv4View &v, size_t &bytes) {
-  if (layers < 1 || pages < 1 || kv_heads < 1)
+  if (layers < 1 || pages < 1 || kv_heads < 1 || kv_heads > 65536)
     return fail(MQ_ERR_INVALID, "invalid cache shape: %d layers, %d pages, %d heads", layers, pages, kv_heads);
   if (!valid_page(page_size))
     return fail(MQ_ERR_INVALID, "page size %d: a multiple of %d up to 1024 is needed", page_size, kKv4Unit);
@@ -258,16 +262,12 @@ int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64
   if (int rc = check_rows("key", k, ld_k, hs_k, c->v.kv, c->v.hd)) return rc;
   if (int rc = check_rows("value", v, ld_v, hs_v, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
-  const int64_t blocks = ((int64_t)rows * 2 * c->v.kv * c->v.nb + kKv4Blocks - 1) / kKv4Blocks;
-  if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Kv4Rows kr{k, ld_k, hs_k}, vr{v, ld_v, hs_v};
-  const bool vec = vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v);
-  auto *kernel = fits32(blocks) ? (vec ? kv4_store_kernel<true, uint32_t> : kv4_store_kernel<false, uint32_t>)
-                                : (vec ? kv4_store_kernel<true, int64_t> : kv4_store_kernel<false, int64_t>);
-  kernel<<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
+  auto *kernel = vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v) ? kv4_store_kernel<true> : kv4_store_kernel<false>;
+  kernel<<<row_grid(c, rows), kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
   return launched("cache store");
 }
 
@@ -280,15 +280,11 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
   if (int rc = check_rows("key", k, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
   if (int rc = check_rows("value", v, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
-  const int64_t blocks = ((int64_t)rows * 2 * c->v.kv * c->v.nb + kKv4Blocks - 1) / kKv4Blocks;
-  if (blocks > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows are too many for one call", rows);
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool vec = vector16(k, 0, 0) && vector16(v, 0, 0);
-  auto *kernel = fits32(blocks) ? (vec ? kv4_load_kernel<true, uint32_t> : kv4_load_kernel<false, uint32_t>)
-                                : (vec ? kv4_load_kernel<true, int64_t> : kv4_load_kernel<false, int64_t>);
-  kernel<<<(unsigned)blocks, kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
+  auto *kernel = vector16(k, 0, 0) && vector16(v, 0, 0) ? kv4_load_kernel<true> : kv4_load_kernel<false>;
+  kernel<<<row_grid(c, rows), kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
   return launched("cache load");
 }
 

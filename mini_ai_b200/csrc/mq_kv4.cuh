@@ -53,55 +53,81 @@ __host__ __device__ __forceinline__ uint8_t *kv4_unit(const Kv4View &c, int laye
          (int64_t)u * kv4_unit_bytes(c.nb);
 }
 
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 // 32 elements over 4 neighbouring lanes, 8 each (lane t: elements 8t..8t+7):
-// this lane's nibbles and the block's scale.
+// this lane's nibbles and the block's scale. Its instructions bound the store of
+// many rows (8192 rows of 8 heads of 128: 26 us, 15.4 million warp instructions,
+// against 11 us of memory traffic); with the extreme's place carried along and
+// every code clamped at both ends they were 18.3 million, 28 us.
 __device__ __forceinline__ uint32_t kv4_pack(const float (&x)[8], uint16_t &scale) {
-  const int t = threadIdx.x & 3;
-  float s = x[0];
-  int at = 0;
-  bool bad = !isfinite(x[0]);
+  float hi = x[0], lo = x[0];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    bad |= !isfinite(x[i]);
-    if (fabsf(x[i]) > fabsf(s)) s = x[i], at = i;
+  for (int i = 1; i < 8; ++i) hi = max_nan(hi, x[i]), lo = min_nan(lo, x[i]);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
-  at += 8 * t;
+  float s = hi > -lo ? hi : lo;  // the element of largest |x|
+  if (__any_sync(0xffffffffu, hi == -lo)) {  // of both signs: the first one
+    int at = 32;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {  // ties go to the lower place
-    const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
-    bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
-    if (fabsf(s2) > fabsf(s) || (fabsf(s2) == fabsf(s) && at2 < at)) s = s2, at = at2;
+    for (int i = 7; i >= 0; --i)
+      if (fabsf(x[i]) == hi) at = 8 * (threadIdx.x & 3) + i;
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == (at & 7)) mine = x[i];
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
+      const float mine2 = __shfl_xor_sync(0xffffffffu, mine, o);
+      if (at2 < at) at = at2, mine = mine2;
+    }
+    if (hi == -lo) s = mine;
   }
   const float d8 = __bfloat162float(__float2bfloat16_rn(s * -0.125f));
-  bad |= fabsf(d8) > 8160.0f;
   const __half dh = __float2half_rn(d8);
   const float d = __half2float(dh);
+  const bool bad = !(fabsf(d8) <= 8160.0f);  // or not finite
   scale = bad ? (uint16_t)0x7e00u : __half_as_ushort(dh);
   if (bad || d == 0.0f) return 0x88888888u;  // all codes 0
   // Nearest integers by x times 1 / d, rounded by adding 1.5 * 2^23: right wherever the remainder (which fma gives
-  // exactly) stays below d / 2; where it does not, a tie or a quotient next to one, by the division.
+  // exactly) stays below d / 2; where it does not, a tie or a quotient next to one, by the division. So too below
+  // fp16's normal scales, where d may be far enough off for codes below -8.
   constexpr float kRound = 12582912.0f;
   const float inv = __frcp_rn(d);
-  uint32_t w = 0;
-  float far = 0.0f;
+  float far = 0.0f, sum0 = 34952.0f, sum1 = 34952.0f;  // four codes in base 16, each with 8 added
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = fmaf(x[i], inv, kRound);
-    far = fmaxf(far, fabsf(fmaf(kRound - t, d, x[i])));
-    w |= (__float_as_uint(fminf(fmaxf(t, kRound - 8.0f), kRound + 7.0f)) & 15u) << (4 * i);
+    const float minus = kRound - fmaf(x[i], inv, kRound);  // -c
+    far = fmaxf(far, fabsf(fmaf(minus, d, x[i])));
+    const float place = -(float)(1 << (4 * (i & 3))), c = fmaxf(minus, -7.0f);
+    if (i < 4) sum0 = fmaf(c, place, sum0);
+    else sum1 = fmaf(c, place, sum1);
   }
-  if (!(far < 0.5f * fabsf(d))) {
+  uint32_t w = __float_as_uint(sum0 + 8388608.0f) & 0xffffu | __float_as_uint(sum1 + 8388608.0f) << 16;
+  if (!(far < 0.5f * fabsf(d)) || fabsf(d) < 6.103515625e-5f) {
     w = 0;
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) {
       float v = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) v = i == j ? x[j] : v;
-      w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(v, d)), -8.0f), 7.0f) & 15u) << (4 * i);
+      w |= (uint32_t)((int)fminf(fmaxf(rintf(__fdiv_rn(v, d)), -8.0f), 7.0f) + 8) << (4 * i);
     }
   }
-  return w ^ 0x88888888u;  // c + 8
+  return w;
 }
 
 struct Kv4Rows {  // rows [rows][kv][hd] with strides in elements
@@ -111,121 +137,134 @@ struct Kv4Rows {  // rows [rows][kv][hd] with strides in elements
 
 constexpr int kKv4Threads = 256;
 
-constexpr int kKv4Each = 2;                                   // blocks a quad of lanes
-constexpr int kKv4Blocks = kKv4Threads / 4 * kKv4Each;         // blocks a CTA
+constexpr int kKv4Quads = kKv4Threads / 4;  // quads of lanes: blocks that a CTA packs at a time
+constexpr int kKv4Each = 2;                // rows in flight a thread (4 made the load slower: 25 -> 27 us)
 
-// A block's place: row, head and block of the head, K or V.
+// A thread's place in every row that it takes: the same head and block of K or
+// V. A CTA holds `whole` rows of `per_row` blocks at a time, or (rows of more
+// blocks than quads) its blockIdx.y-th part of one; CTAs stride over the rows,
+// so that the divisions are paid once.
 struct Kv4Place {
-  int row, head, j;
-  bool v;
+  int row;   // of those that the CTA holds
+  int head, j;
+  bool v, inside;
+  int codes;  // bytes from a token's place 0 in the unit to this lane's codes, and to the scale
+  int scale;
 };
-template <typename Index>
-__device__ __forceinline__ Kv4Place kv4_place(const Kv4View &c, Index idx, int per_row) {
+__host__ __device__ __forceinline__ int kv4_whole(int per_row) { return per_row < kKv4Quads ? kKv4Quads / per_row : 1; }
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4View &c) {
+  const int per_row = 2 * c.kv * c.nb, half = c.kv * c.nb, quad = threadIdx.x >> 2, t = threadIdx.x & 3;
   Kv4Place p;
-  p.row = (int)(idx / per_row);
-  const int in_row = (int)(idx - (Index)p.row * per_row), half = c.kv * c.nb;
+  p.row = per_row < kKv4Quads ? quad / per_row : 0;
+  int in_row = per_row < kKv4Quads ? quad % per_row : blockIdx.y * kKv4Quads + quad;
+  p.inside = in_row < per_row && p.row < kv4_whole(per_row);
+  in_row = min(in_row, per_row - 1);
   p.v = in_row >= half;
   const int hb = p.v ? in_row - half : in_row;
   p.head = hb / c.nb, p.j = hb % c.nb;
+  p.codes = p.v ? kv4_v_off(c.nb) + 4 * t * c.nb + 2 * p.j : t * 4 * c.nb + 4 * p.j;
+  p.scale = (p.v ? kv4_v_scale_off(c.nb) : kv4_k_scale_off(c.nb)) + 2 * p.j;
   return p;
 }
-// Where lane t's 8 elements of the block lie in `unit`: K one word, V two half-words 2 nb bytes apart; and its scale.
-__device__ __forceinline__ uint8_t *kv4_codes(const Kv4View &c, uint8_t *unit, const Kv4Place &p, int tok, int t) {
-  if (p.v) return unit + kv4_v_off(c.nb) + tok * 16 * c.nb + 4 * t * c.nb + 2 * p.j;
-  return unit + tok * 16 * c.nb + t * 4 * c.nb + 4 * p.j;
-}
-__device__ __forceinline__ uint16_t *kv4_scale(const Kv4View &c, uint8_t *unit, const Kv4Place &p, int tok) {
-  return reinterpret_cast<uint16_t *>(unit + (p.v ? kv4_v_scale_off(c.nb) : kv4_k_scale_off(c.nb))) + tok * c.nb + p.j;
+// The token of `slot` in the place's head: its unit, and its number there.
+__device__ __forceinline__ uint8_t *kv4_slot(const Kv4View &c, int layer, int head, int slot, int &tok) {
+  const int page_id = slot / c.page, in_page = slot - page_id * c.page;
+  tok = in_page % kKv4Unit;
+  return kv4_unit(c, layer, page_id, head, in_page / kKv4Unit);
 }
 
-// One quad of lanes per block of a row, two blocks each: reads 32 floats,
-// writes 16 bytes of codes and a scale. Rows of no valid slot are skipped.
-// Index: 32 bits where the call's blocks fit (a 64-bit division costs as much as the packing).
-template <bool VEC, typename Index>
+// One quad of lanes per block of a row: reads 32 floats, writes 16 bytes of
+// codes and a scale. Rows of no valid slot are skipped.
+template <bool VEC>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_store_kernel(const Kv4View c, int layer, const Kv4Rows k, const Kv4Rows v, const int *__restrict__ slots,
                      int rows) {
-  const int per_row = 2 * c.kv * c.nb, t = threadIdx.x & 3;  // blocks of a row: K heads, then V heads
-  const Index total = (Index)rows * per_row, i0 = (Index)blockIdx.x * kKv4Blocks + (threadIdx.x >> 2);
-  Kv4Place at[kKv4Each];
-  int slot[kKv4Each];
-  float x[kKv4Each][8];
+  const Kv4Place at = kv4_place(c);
+  const int64_t step = (int64_t)gridDim.x * kv4_whole(2 * c.kv * c.nb);
+  const Kv4Rows &src = at.v ? v : k;
+  const float *p = src.p + at.head * src.hs + 32 * at.j + 8 * (threadIdx.x & 3);
+  // Every warp goes around together (kv4_pack shuffles): the bound is on the CTA's first row.
+  for (int64_t first = (int64_t)blockIdx.x * kv4_whole(2 * c.kv * c.nb); first < rows; first += kKv4Each * step) {
+    int slot[kKv4Each];
+    float x[kKv4Each][8];
 #pragma unroll
-  for (int n = 0; n < kKv4Each; ++n) {
-    const Index idx = i0 + n * (kKv4Threads / 4);
-    at[n] = kv4_place(c, idx < total ? idx : total - 1, per_row);  // whole warps: kv4_pack shuffles
-    slot[n] = idx < total ? slots[at[n].row] : -1;
-    const Kv4Rows &src = at[n].v ? v : k;
-    const float *p = src.p + at[n].row * src.ld + at[n].head * src.hs + 32 * at[n].j + 8 * t;
-    if (VEC) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-      x[n][0] = a.x, x[n][1] = a.y, x[n][2] = a.z, x[n][3] = a.w;
-      x[n][4] = b.x, x[n][5] = b.y, x[n][6] = b.z, x[n][7] = b.w;
-    } else {
+    for (int n = 0; n < kKv4Each; ++n) {
+      const int64_t row = first + n * step + at.row;
+      const bool real = at.inside && row < rows;
+      slot[n] = real ? slots[row] : -1;
+      const float *q = p + (real ? row : 0) * src.ld;
+      if (VEC) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(q)), b = __ldg(reinterpret_cast<const float4 *>(q) + 1);
+        x[n][0] = a.x, x[n][1] = a.y, x[n][2] = a.z, x[n][3] = a.w;
+        x[n][4] = b.x, x[n][5] = b.y, x[n][6] = b.z, x[n][7] = b.w;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[n][i] = __ldg(p + i);
+        for (int i = 0; i < 8; ++i) x[n][i] = __ldg(q + i);
+      }
     }
-  }
 #pragma unroll
-  for (int n = 0; n < kKv4Each; ++n) {
-    uint16_t scale;
-    const uint32_t w = kv4_pack(x[n], scale);
-    if (slot[n] < 0 || slot[n] >= c.pages * c.page) continue;
-    const int page_id = slot[n] / c.page, in_page = slot[n] - page_id * c.page, tok = in_page % kKv4Unit;
-    uint8_t *unit = kv4_unit(c, layer, page_id, at[n].head, in_page / kKv4Unit);
-    uint8_t *codes = kv4_codes(c, unit, at[n], tok, t);
-    if (at[n].v) {
-      *reinterpret_cast<uint16_t *>(codes) = (uint16_t)w;
-      *reinterpret_cast<uint16_t *>(codes + 2 * c.nb) = (uint16_t)(w >> 16);
-    } else {
-      *reinterpret_cast<uint32_t *>(codes) = w;
+    for (int n = 0; n < kKv4Each; ++n) {
+      uint16_t scale;
+      const uint32_t w = kv4_pack(x[n], scale);
+      if (slot[n] < 0 || slot[n] >= c.pages * c.page) continue;
+      int tok;
+      uint8_t *unit = kv4_slot(c, layer, at.head, slot[n], tok);
+      uint8_t *codes = unit + at.codes + tok * 16 * c.nb;
+      if (at.v) {  // two half-words
+        *reinterpret_cast<uint16_t *>(codes) = (uint16_t)w;
+        *reinterpret_cast<uint16_t *>(codes + 2 * c.nb) = (uint16_t)(w >> 16);
+      } else {
+        *reinterpret_cast<uint32_t *>(codes) = w;
+      }
+      if ((threadIdx.x & 3) == 0) *reinterpret_cast<uint16_t *>(unit + at.scale + 2 * tok * c.nb) = scale;
     }
-    if (t == 0) *kv4_scale(c, unit, at[n], tok) = scale;
   }
 }
 
 // The values at `slots`, k and v [rows][kv][hd]; rows of no valid slot are 0.
 // Threads as in the store.
-template <bool VEC, typename Index>
+template <bool VEC>
 __global__ void __launch_bounds__(kKv4Threads)
     kv4_load_kernel(const Kv4View c, int layer, const int *__restrict__ slots, int rows, float *__restrict__ k,
                     float *__restrict__ v) {
-  const int per_row = 2 * c.kv * c.nb, t = threadIdx.x & 3;
-  const Index total = (Index)rows * per_row, i0 = (Index)blockIdx.x * kKv4Blocks + (threadIdx.x >> 2);
-  Kv4Place at[kKv4Each];
-  uint32_t w[kKv4Each];
-  float d[kKv4Each];
+  const Kv4Place at = kv4_place(c);
+  const int64_t step = (int64_t)gridDim.x * kv4_whole(2 * c.kv * c.nb);
+  float *out = (at.v ? v : k) + at.head * c.hd + 32 * at.j + 8 * (threadIdx.x & 3);
+  if (!at.inside) return;
+  for (int64_t first = (int64_t)blockIdx.x * kv4_whole(2 * c.kv * c.nb); first < rows; first += kKv4Each * step) {
+    uint32_t w[kKv4Each];
+    float d[kKv4Each];
 #pragma unroll
-  for (int n = 0; n < kKv4Each; ++n) {
-    const Index idx = i0 + n * (kKv4Threads / 4);
-    if (idx >= total) continue;
-    at[n] = kv4_place(c, idx, per_row);
-    const int slot = slots[at[n].row];
-    w[n] = 0x88888888u, d[n] = 0.0f;
-    if (slot < 0 || slot >= c.pages * c.page) continue;
-    const int page_id = slot / c.page, in_page = slot - page_id * c.page, tok = in_page % kKv4Unit;
-    uint8_t *unit = kv4_unit(c, layer, page_id, at[n].head, in_page / kKv4Unit);
-    const uint8_t *codes = kv4_codes(c, unit, at[n], tok, t);
-    if (at[n].v)
-      w[n] = __ldg(reinterpret_cast<const uint16_t *>(codes)) |
-             (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(codes + 2 * c.nb)) << 16;
-    else
-      w[n] = __ldg(reinterpret_cast<const uint32_t *>(codes));
-    d[n] = __half2float(__ushort_as_half(__ldg(kv4_scale(c, unit, at[n], tok))));
-  }
+    for (int n = 0; n < kKv4Each; ++n) {
+      const int64_t row = first + n * step + at.row;
+      const int slot = row < rows ? slots[row] : -1;
+      w[n] = 0x88888888u, d[n] = 0.0f;
+      if (slot < 0 || slot >= c.pages * c.page) continue;
+      int tok;
+      const uint8_t *unit = kv4_slot(c, layer, at.head, slot, tok), *codes = unit + at.codes + tok * 16 * c.nb;
+      if (at.v)
+        w[n] = __ldg(reinterpret_cast<const uint16_t *>(codes)) |
+               (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(codes + 2 * c.nb)) << 16;
+      else
+        w[n] = __ldg(reinterpret_cast<const uint32_t *>(codes));
+      d[n] = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t *>(unit + at.scale + 2 * tok * c.nb))));
+    }
 #pragma unroll
-  for (int n = 0; n < kKv4Each; ++n) {
-    if (i0 + n * (kKv4Threads / 4) >= total) continue;
-    float x[8];
+    for (int n = 0; n < kKv4Each; ++n) {
+      const int64_t row = first + n * step + at.row;
+      if (row >= rows) continue;
+      float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = d[n] * (float)((int)((w[n] >> (4 * i)) & 15u) - 8);
-    float *o = (at[n].v ? v : k) + ((int64_t)at[n].row * c.kv + at[n].head) * c.hd + 32 * at[n].j + 8 * t;
-    if (VEC) {
-      reinterpret_cast<float4 *>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4 *>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
+      for (int i = 0; i < 8; ++i)  // 2^23 + q, less 2^23 + 8
+        x[i] = d[n] * (__uint_as_float((w[n] >> (4 * i) & 15u) | 0x4B000000u) - 8388616.0f);
+      float *o = out + row * ((int64_t)c.kv * c.hd);
+      if (VEC) {
+        reinterpret_cast<float4 *>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4 *>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = x[i];
+        for (int i = 0; i < 8; ++i) o[i] = x[i];
+      }
     }
   }
 }
