@@ -304,8 +304,11 @@ __device__ __forceinline__ float half_at(const uint32_t (&a)[W], int j) {
 // Tokens of a unit are taken in the order that keeps shared memory free of
 // bank conflicts: column n of score tile i is token (n >> 1) + 4 (n & 1) + 8 i.
 //
-// Bound: the cache's bytes, 1152 a token of 8 heads of 128, against ~300 issue
-// slots a unit and warp for decoding and weights.
+// Bound: issue slots. A unit of 16 tokens x 8 rows x 128 elements costs 519
+// instructions (measured), most of them decoding; at 57 % of the slots that is
+// 2.4 TB/s of cache on 48 ragged chats (90 us; its bytes alone would take 33).
+// Three CTAs an SM: four had to spill (114 us). Two units a step: one took 99
+// us, four 104.
 constexpr int kDecWarps = 4;
 constexpr int kDecRowTile = 8;
 constexpr int kDecUnits = 2;   // per warp and step
