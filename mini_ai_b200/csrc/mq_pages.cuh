@@ -13,10 +13,11 @@
 //   free[n_free - 1 - (first_r + i - held_r)].
 //
 // The bytes are few (a thousand requests with 64k rows: 0.5 MB), so latency
-// bounds it: one launch, in which every CTA of one cluster computes the two
-// prefix sums itself (R loads, no exchange), waits once for the others to have
-// read the inputs that the outputs may overwrite, and writes its share of the
-// rows. 8 requests: 4.9 us in a graph; 1000 requests and 65 k rows: 14 us.
+// bounds it: one launch, in which every CTA computes the two prefix sums itself
+// (R loads, no exchange) and writes its share of the rows. Where outputs replace
+// inputs (the lengths, the stack's size) the CTAs are one cluster and wait once
+// for one another, between reading and writing. 8 requests: 4.9 us in a graph;
+// 1000 requests and 65 k rows: 12.3 us as a cluster of 8, 8.7 as 17 CTAs.
 #pragma once
 
 #include "mq_common.cuh"
@@ -26,7 +27,8 @@ namespace mq {
 
 constexpr int kPagesThreads = 1024;
 constexpr int kPagesMaxSeqs = 8192;  // shared memory: 12 bytes a request
-constexpr int kPagesCluster = 8;     // CTAs of a large batch
+constexpr int kPagesCluster = 8;     // CTAs of a large batch planned in place
+constexpr int kPagesCtas = 64;       // and otherwise, at most
 
 struct PagesArgs {
   const int *ctx, *fresh;  // tokens held and tokens brought, per request
@@ -38,7 +40,8 @@ struct PagesArgs {
   const int *n_free;
   int rows;
   int *offsets, *lens, *slots, *positions, *n_free_out, *refused;
-  bool vec;  // slots and positions are aligned to 16 bytes
+  bool vec;       // slots and positions are aligned to 16 bytes
+  bool in_place;  // seq_lens is ctx_lens, or n_free_out is n_free
 };
 
 __host__ __device__ constexpr size_t pages_smem(int n) { return (size_t)(3 * n + 1) * sizeof(int); }
@@ -66,6 +69,9 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int
   return v + (warp ? before : 0);
 }
 
+// Pages of n tokens, 0 <= n <= INT_MAX, in 32 bits (64-bit divisions were half of the kernel's time).
+__device__ __forceinline__ int pages_of(int n, int page) { return (int)(((uint32_t)n + page - 1) / (uint32_t)page); }
+
 __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesArgs a) {
   extern __shared__ int pages_sm[];
   __shared__ int64_t warp_sums[kPagesThreads / 32];
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesAr
     const int64_t end = rows_before + block_scan(max(m, 0), warp_sums, sum);
     rows_before += sum;
     const bool fits = real && c >= 0 && m >= 0 && (int64_t)c + m <= room && end <= a.rows;
-    const int more = fits ? (int)(((int64_t)c + m + a.page - 1) / a.page - ((int64_t)c + a.page - 1) / a.page) : 0;
+    const int more = fits ? pages_of(c + m, a.page) - pages_of(c, a.page) : 0;
     const int64_t upto = pages_before + block_scan(more, warp_sums, sum);
     pages_before += sum;
     if (real) {
@@ -98,8 +104,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesAr
   if (threadIdx.x == 0) off[0] = 0;
   int64_t both;  // refused requests and, below them, taken pages; the barriers order the writes of off, ctx and first
   block_scan((int64_t)refused << 40 | taken, warp_sums, both);
-  // seq_lens may be ctx_lens, and n_free_out may be n_free: every CTA has read them.
-  if (ncta > 1) sm100::cluster_sync();
+  if (ncta > 1 && a.in_place) sm100::cluster_sync();  // every CTA has read what is replaced
   if (cta == 0) {
     for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
       a.offsets[r + 1] = off[r + 1];
@@ -132,9 +137,9 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const PagesAr
       if (row >= total) continue;
       while (off[r + 1] <= row) ++r, known = -1;
       if (first[r] < 0) continue;
-      const int p = ctx[r] + (int)(row - off[r]), page = p / a.page, in = p - page * a.page;
+      const int p = ctx[r] + (int)(row - off[r]), page = (uint32_t)p / (uint32_t)a.page, in = p - page * a.page;
       if (page != known) {
-        const int held = (int)(((int64_t)ctx[r] + a.page - 1) / a.page);
+        const int held = pages_of(ctx[r], a.page);
         int *entry = a.tables + (int64_t)r * a.width + page;
         id = page < held ? *entry : a.stack[n_free - 1 - (first[r] + page - held)];
         if (page >= held && in == 0) *entry = id;  // a new page's first token is one of the new rows
