@@ -223,8 +223,8 @@ size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new);
  * sees positions 0 up to its own, at most seq_lens[r] of them:
  *   out = softmax(scale * q . k) v, query head h with KV head h / (heads / kv_heads).
  * seq_lens counts the step's own rows, which mq_kv4_store has written.
- * block_tables [n_seqs][max_pages] page ids; lengths past max_pages *
- * page_size count as that, and tokens of a page id outside the cache are not
+ * block_tables [n_seqs][max_pages] page ids, max_pages * page_size <=
+ * 2^31 - 4097; lengths past max_pages * page_size count as that, and tokens of a page id outside the cache are not
  * seen. A row that sees nothing is 0; rows past offsets[n_seqs] stay as they
  * are, and no row past `rows` is touched. max_new: the most rows that a
  * request brings, as far as the caller knows; it selects kernels and a lower

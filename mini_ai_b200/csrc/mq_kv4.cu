@@ -305,6 +305,8 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   if (heads < 1 || heads % c->v.kv)
     return fail(MQ_ERR_INVALID, "%d query heads do not share %d key/value heads evenly", heads, c->v.kv);
   if ((int64_t)rows * heads > INT_MAX) return fail(MQ_ERR_INVALID, "%d rows of %d heads are too many", rows, heads);
+  if ((int64_t)max_pages * c->v.page > INT_MAX - 4096)
+    return fail(MQ_ERR_INVALID, "%d pages a request: tokens must stay below 2^31 - 4096", max_pages);
   if (max_pages < 1 || max_new < 0) return fail(MQ_ERR_INVALID, "%d pages a request, %d new rows", max_pages, max_new);
   if (!std::isfinite(scale)) return fail(MQ_ERR_INVALID, "the score scale is not finite");
   if (rows == 0 || n_seqs == 0) return MQ_OK;

@@ -435,6 +435,21 @@ def test_many_items_a_cta(mq, torch, heads, kv, hd, lens, news):
         at += m
 
 
+@pytest.mark.parametrize("page", [16, 1024])
+def test_many_requests(mq, torch, page):
+    """More requests than a kernel has threads, most with one row, some with none or many."""
+    rng = np.random.default_rng(page)
+    n = 1700 if page == 16 else 300
+    lens = rng.integers(0, 40, n)
+    news = np.where(rng.random(n) < 0.05, np.minimum(lens, 30), np.minimum(lens, rng.integers(0, 2, n)))
+    b = Batch(mq, torch, [int(x) for x in lens], 1, 32, page, seed=page)
+    news = [int(x) for x in news]
+    q, out = run_attention(torch, b, 2, news, 1)
+    want, tol = ref_attention(torch, q[:-2], b.hk, b.hv, news, b.lens, 32 ** -0.5)
+    assert_attention(torch, out[:-2], want, tol)
+    assert (out[-2:] == 7.0).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
 def test_scales_and_sizes(mq, torch, scale):
     """Score scales of either sign, flat and one-hot softmaxes, queries and values of extreme sizes."""
@@ -624,7 +639,7 @@ def test_refusals(mq, torch):
     torch.cuda.synchronize()
     assert call() == e.MQ_OK
     for kw in (dict(rows=-1), dict(heads=0), dict(n=-1), dict(width=0), dict(q=None), dict(out=None), dict(offsets=None),
-               dict(lens=None), dict(tables=None), dict(hsq=63), dict(hso=32), dict(ldq=-1), dict(ldo=0), dict(q=q.data_ptr() + 2)):
+               dict(lens=None), dict(tables=None), dict(hsq=63), dict(hso=32), dict(ldq=-1), dict(ldo=0), dict(width=1 << 27), dict(q=q.data_ptr() + 2)):
         assert call(**kw) == e.MQ_ERR_INVALID, kw
     for kw in (dict(ws=None), dict(bytes=need - 1)):
         assert call(**kw) == e.MQ_ERR_SIZE, kw
