@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <new>
 
 #include "mq_kv4.cuh"
@@ -98,9 +99,14 @@ int launched(const char *what) {
 
 // Launched behind the previous kernel of the stream with programmatic
 // serialization: it may start early and waits where it depends on that one.
+// MQ_PDL=0 launches normally, as for the linears.
 template <typename... KArgs, typename... Args>
 int launch_after(const char *what, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s,
                  const Args &...args) {
+  static const bool on = [] {
+    const char *e = std::getenv("MQ_PDL");
+    return !e || !*e || std::atoi(e) != 0;
+  }();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -108,7 +114,7 @@ int launch_after(const char *what, void (*kernel)(KArgs...), dim3 grid, int thre
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = on;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
