@@ -369,10 +369,9 @@ int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_se
   const PagesArgs a{ctx_lens, new_lens, n_seqs, page_size, block_tables, max_pages, free_pages, n_pages,
                     n_free, rows, offsets, seq_lens, slots, positions, n_free_out, refused,
                     vector16(slots, 0, 0) && vector16(positions, 0, 0), seq_lens == ctx_lens || n_free_out == n_free};
-  const size_t smem = pages_smem(n_seqs);
-  if (smem > 48 * 1024)
-    MQ_CUDA(cudaFuncSetAttribute(pages_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)pages_smem(kPagesMaxSeqs)));
+  // (The 48 KB that need no permission count the kernel's static part too.)
+  static std::atomic<uint64_t> ready{0};
+  MQ_CUDA(allow_smem(pages_plan_kernel, (int)pages_smem(kPagesMaxSeqs), device, ready));
   cudaLaunchConfig_t cfg = {};
   // A thread for each request and for every four rows, in one CTA while that is enough: a decode step of 8
   // requests took 7.7 us with 1024 threads.
@@ -380,7 +379,7 @@ int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_se
   const int ctas = (int)std::min<int64_t>(kPagesCtas, ((int64_t)rows + 4 * kPagesThreads - 1) / (4 * kPagesThreads));
   cfg.gridDim = dim3(ctas <= 1 ? 1 : a.in_place ? kPagesCluster : ctas);
   cfg.blockDim = dim3(std::min(kPagesThreads, std::max(64, (want + 31) / 32 * 32)));
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = pages_smem(n_seqs);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -792,3 +792,29 @@ def test_other_device(mq, torch):
     with pytest.raises(RuntimeError):
         c.load(0, at.to("cuda:0"))
     assert torch.cuda.current_device() == 0
+
+
+# ------------------------------------------------------------------ limits
+def test_plan_sizes_in_a_fresh_process():
+    """Every request count plans in a process that has planned none larger (what a large plan allows its kernel stays
+    allowed): the sizes around the 48 KB of shared memory that need no permission."""
+    code = ("import numpy as np, torch, mini_ai_b200 as mq, test_kv4_gpu as t\n"
+            "for n in (4070, 4074, 4075, 4085, 4095, 4096, 4100):\n"
+            "    rng = np.random.default_rng(n)\n"
+            "    ctx, new, tables, free, n_free = t._plan_case(rng, n, 60, 3, 16)\n"
+            "    for in_place in (False, True):\n"
+            "        t._check_plan(mq, torch, ctx, new, tables, free, n_free, 16, int(new.sum()), in_place)\n"
+            "print('planned', n)\n")
+    _run_child(code, "planned 4100")
+
+
+def _run_child(code, last):
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    here = Path(__file__).resolve().parent
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here.parent), str(here), os.environ.get("PYTHONPATH", "")]))
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.splitlines()[-1:] == [last], r.stdout + r.stderr
