@@ -215,7 +215,6 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   void *base = memory;
   if (!base) e = cudaMalloc(&base, bytes);
   if (e != cudaSuccess) {
-    cudaGetLastError();  // an allocation that does not fit is no fault of later calls
     delete c;
     return cuda_fail(e, "cudaMalloc cache");
   }

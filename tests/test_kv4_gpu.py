@@ -818,3 +818,28 @@ def _run_child(code, last):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here.parent), str(here), os.environ.get("PYTHONPATH", "")]))
     r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.splitlines()[-1:] == [last], r.stdout + r.stderr
+
+
+def test_a_failed_call_leaves_no_error_behind(mq, torch):
+    """A call that could not get its memory fails alone: the calls after it do not report its error."""
+    rng = np.random.default_rng(0)
+    w = mq.CudaWeight(mq.QuantizeTensor(rng.standard_normal((128, 256)).astype(np.float32), mq.QuantType.kQ40), device=0)
+    x = torch.zeros(1, 256, device="cuda")
+    c, at = mq.Kv4Cache(1, 1, 16, 1, 32), ints(torch, [3])
+    row = torch.randn(1, 1, 32, device="cuda")
+    lens, tables, stack, n_free = ints(torch, [5]), ints(torch, [[0]]), ints(torch, [7, 7]), ints(torch, [1])
+    torch.cuda.synchronize()
+
+    def fail():  # the gate product of these rows would take 8 TiB; nothing is launched
+        rc = mq.lib().mq_linear_swiglu(w.handle, w.handle, x.data_ptr(), 1 << 20, 256, x.data_ptr(), 1 << 21, None)
+        assert rc == mq._lib.MQ_ERR_CUDA and "memory" in mq._lib.last_error()
+
+    fail()
+    c.store(0, row, -row, at)
+    fail()
+    k, v = c.load(0, at)
+    assert torch.equal(k, -v) and k.any()
+    fail()
+    mq.ReleasePages(ints(torch, [0]), lens, tables, stack, n_free, 16)
+    assert n_free.tolist() == [2] and stack.tolist() == [7, 0]
+    w.close()
