@@ -177,8 +177,8 @@ int mq_linear_noalloc(const mq_weight *w, const float *x, int m, int ldx, const 
  * A step: mq_pages_plan once, then for each layer mq_kv4_store and
  * mq_kv4_attention on the same stream. All lengths, offsets and tables are
  * int32 device arrays, read by the kernels when they run: a captured graph
- * serves every step of its buffers' sizes. No call allocates or synchronises,
- * except a creation without memory of its own and its destruction. */
+ * serves every step of its buffers' sizes. No call allocates device memory or
+ * synchronises, except a creation that is given none and its destruction. */
 typedef struct mq_kv4 mq_kv4;
 
 /* Device bytes of a cache: layers * pages * page_size * kv_heads * head_dim *
@@ -190,7 +190,10 @@ size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head
  * 2^31. `memory` is the
  * caller's device memory for it (at least mq_kv4_bytes(), 16-byte aligned),
  * which must outlive the handle and is cleared on `stream`; NULL allocates
- * it, which synchronizes `stream`. */
+ * it, which synchronizes `stream`. MQ_KV4_WAIT_NS in the environment limits
+ * each wait inside the cache's attention (nanoseconds, default 1 s); with
+ * MQ_KV4_LOSE_COPIES=1 every such wait runs out, so that a program's handling
+ * of MQ_ERR_TIMEOUT can be tried. */
 int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads, int head_dim, void *memory,
                   size_t memory_bytes, void *stream, mq_kv4 **out);
 void mq_kv4_destroy(mq_kv4 *c);
@@ -233,7 +236,11 @@ size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new);
  * enter the tensor cores as fp16 hi + lo pairs (22 bits). workspace: device
  * memory of at least mq_kv4_attention_workspace() bytes, 16-byte aligned,
  * not shared with a call that may run at the same time; its contents do not
- * matter. The summation order is fixed: equal inputs give equal bits. */
+ * matter. The summation order is fixed: equal inputs give equal bits. Every
+ * wait of the kernels is bounded: where one runs out, all rows that its CTA
+ * had still to write are NaN, and so are the cut rows that it had a part in;
+ * the device's error flag (mq_device_error_flag) is raised, and the next call
+ * returns MQ_ERR_TIMEOUT without launching anything. */
 int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
                      const int *offsets, const int *seq_lens, const int *block_tables, int n_seqs, int max_pages,
                      int max_new, float scale, float *out, int64_t ld_out, int64_t hs_out, void *workspace,

@@ -90,6 +90,17 @@ int cache_shape(int layers, int pages, int page_size, int kv_heads, int head_dim
   return MQ_OK;
 }
 
+bool env_set(const char *name) {
+  const char *e = std::getenv(name);
+  return e && *e && std::atoi(e) != 0;
+}
+
+uint64_t wait_limit() {
+  const char *e = std::getenv("MQ_KV4_WAIT_NS");
+  const unsigned long long ns = e ? std::strtoull(e, nullptr, 10) : 0;
+  return ns ? ns : kKv4WaitNs;
+}
+
 int launched(const char *what) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, what);
@@ -210,6 +221,17 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   auto *c = new (std::nothrow) mq_kv4;
   if (!c) return fail(MQ_ERR_INVALID, "out of host memory");
+  // (The flag is allocated with the device's first handle, which may be made while a stream is captured.)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const int rc = device_err_flag(device, &c->err_dev, &c->err_host);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (rc) {
+    delete c;
+    return rc;
+  }
+  c->wait_ns = wait_limit();
+  c->lost = env_set("MQ_KV4_LOSE_COPIES") ? 16 : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   void *base = memory;
@@ -324,6 +346,10 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
     return fail(MQ_ERR_SIZE, "attention workspace: %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
   if (reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(MQ_ERR_INVALID, "the attention workspace is not aligned to 16 bytes");
+  if (*(volatile int *)c->err_host) {
+    *(volatile int *)c->err_host = 0;
+    return fail(MQ_ERR_TIMEOUT, "an earlier tensor-core launch on device %d ran out of a bounded wait", c->device);
+  }
   OnDevice g(c->device);
   if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -337,6 +363,7 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   a.scale = scale * 1.44269504088896341f;
   a.vec_q = vector16(q, ld_q, hs_q);
   a.vec_o = vector16(out, ld_out, hs_out);
+  a.err = c->err_dev, a.wait_ns = c->wait_ns, a.lost = c->lost;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   const bool many = many_rows(a.group, max_new);
   switch (c->v.nb) {

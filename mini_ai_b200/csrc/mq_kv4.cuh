@@ -278,4 +278,7 @@ struct mq_kv4 {
   size_t bytes = 0;
   int sms = 0;
   void *owned = nullptr;  // the allocation, where the caller gave no memory
+  int *err_dev = nullptr, *err_host = nullptr;  // the device's bounded-wait flag
+  uint64_t wait_ns = 0;                         // limit of a kernel's waits
+  uint32_t lost = 0;                            // bytes that a copy is waited for beside its own
 };

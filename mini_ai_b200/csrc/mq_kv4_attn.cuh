@@ -37,9 +37,15 @@ struct Kv4AttnArgs {
   bool cut;                // items may be cut (and joined)
   float scale;             // times log2(e): the softmax is in powers of two
   float *parts;            // [grid][2] partial items
-  int4 *meta;              // [grid][2]: the item that a CTA leaves unfinished
+  int4 *meta;              // [grid][2]: the item that a CTA leaves unfinished; the CTAs that it is spread over, and
+                           // whether the CTA gave up (many rows)
   bool vec_q, vec_o;
+  int *err;          // raised when a wait ran out
+  uint64_t wait_ns;  // limit of a wait
+  uint32_t lost;     // bytes that a copy's barrier waits for and that never come: 0, or 16 where all waits shall run out
 };
+
+constexpr int kManyTile = 128;  // rows and tokens of a tile of the many-row kernel
 
 // ------------------------------------------------------------ division of the work
 struct Kv4Request {
@@ -63,7 +69,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 // instead of 372. 4 for the many-row kernel (299 us; 3: 301, 6: 310), 1 for the
 // other (48 ragged chats 90.5 us; 2: 91.1, 4: 96.7).
 template <int RT>
-constexpr int kv4_setup() { return RT == 128 ? 4 : 1; }
+constexpr int kv4_setup() { return RT == kManyTile ? 4 : 1; }
 
 // Work of the first n row tiles of a request: for each its setup, then its steps. With `period` = G BN / RT row
 // tiles to a step of BN tokens, and the tokens before the request's rows
@@ -110,9 +116,9 @@ struct Kv4Walk {
   int ctas;             // pieces
 };
 
-// All threads; a block-wide scan. false: no work for this CTA.
+// CTA `cta` of `grid`. All threads; a block-wide scan. false: no work for it.
 template <int RT, int BN>
-__device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
+__device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w, int cta, int grid) {
   __shared__ int64_t sums[32], s_at;
   __shared__ int s_r;
   const int per = (a.n + blockDim.x - 1) / blockDim.x;
@@ -121,10 +127,10 @@ __device__ __forceinline__ bool kv4_walk(const Kv4AttnArgs &a, Kv4Walk &w) {
   for (int r = r0; r < r1; ++r) mine += a.c.kv * kv4_request<RT, BN>(a, r).work;
   const int64_t upto = block_scan(mine, sums, w.line);
   if (w.line == 0) return false;
-  w.ctas = (int)min((int64_t)gridDim.x, w.line);
-  if ((int)blockIdx.x >= w.ctas) return false;
-  w.place = quotient(blockIdx.x * w.line, w.ctas);
-  w.left = quotient((blockIdx.x + 1) * w.line, w.ctas) - w.place;
+  w.ctas = (int)min((int64_t)grid, w.line);
+  if (cta >= w.ctas) return false;
+  w.place = quotient(cta * w.line, w.ctas);
+  w.left = quotient((cta + 1) * w.line, w.ctas) - w.place;
   if (w.place >= upto - mine && w.place < upto) {
     int64_t at = w.place - (upto - mine);
     int r = r0;
@@ -314,7 +320,8 @@ constexpr int kDecRowTile = 8;
 constexpr int kDecUnits = 2;   // per warp and step
 constexpr int kDecTokens = kDecWarps * kDecUnits * kKv4Unit;  // BN
 constexpr int kDecStages = 3;
-constexpr uint64_t kKv4WaitNs = 1000000000ull;
+constexpr uint64_t kKv4WaitNs = 1000000000ull;  // limit of a wait, unless the cache was made with another
+constexpr uint64_t kKv4DrainNs = 20000000ull;   // for what a CTA that gave up still has in flight
 
 template <int NB>
 struct DecSmem {
@@ -342,16 +349,20 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
     for (int s = 0; s < kDecStages; ++s) sm100::mbar_init(&bars[s], 1);
     sm100::fence_mbar_init();
   }
+  __shared__ int s_gone;  // a wait of this CTA ran out: all its rows from here on are NaN
+  if (threadIdx.x == 0) s_gone = 0;
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
   if (a.cut && threadIdx.x == 0) a.meta[2 * blockIdx.x + 1].x = 0;
   Kv4Walk walk;
-  if (!kv4_walk<kDecRowTile, kDecTokens>(a, walk)) return;
+  if (!kv4_walk<kDecRowTile, kDecTokens>(a, walk, blockIdx.x, gridDim.x)) return;
   __syncwarp();
 
   const int upp = a.c.page / kKv4Unit;  // units of a page
   const int64_t unit_page = a.c.page_head_bytes * a.c.kv;
   uint32_t steps_done = 0;  // of this warp, over all segments: the ring's place
+  volatile int *gave_up = &s_gone;
+  bool gone = false;
   Kv4Segment s;
   while (kv4_next<kDecRowTile, kDecTokens>(a, walk, s)) {
     // This thread's row of the tile: flat row f, and the last token that it sees.
@@ -363,7 +374,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
     const int last_max = min(s.q.base + (min((s.tile + 1) * kDecRowTile, s.q.flat) - 1) / a.group, s.q.len - 1);
     const int first_unit = s.t0 * (kDecTokens / kKv4Unit);
     const int end_unit = min(s.t1 * (kDecTokens / kKv4Unit), (last_max + kKv4Unit) / kKv4Unit);
-    const int steps = max(0, (end_unit - first_unit + kDecWarps * kDecUnits - 1) / (kDecWarps * kDecUnits));
+    const int steps = gone ? 0 : max(0, (end_unit - first_unit + kDecWarps * kDecUnits - 1) / (kDecWarps * kDecUnits));
     const int *table = a.tables + (int64_t)s.r * a.width;
     const uint8_t *slice = kv4_unit(a.c, a.layer, 0, s.head, 0);
 
@@ -438,7 +449,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
         }
         const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (kDecUnits * (k % kPer)) & kAll;
         held = (held & ~(kAll << (kDecUnits * stage))) | have << (kDecUnits * stage);
-        if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit);
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit + a.lost);
         __syncwarp();
         if (lane / kDecUnits == k % kPer && (there >> lane & 1u))
           sm100::bulk_load(ring + (stage * kDecUnits + lane % kDecUnits) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
@@ -448,8 +459,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       for (int k = 0; k < steps; ++k) {
         if (k + kDecStages - 1 < steps) fetch(k + kDecStages - 1);
         const uint32_t stage = (steps_done + k) % kDecStages;
-        if (!sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, nullptr, nullptr, kKv4WaitNs))
-          sum = __uint_as_float(0x7fc00000u);
+        if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, a.err, gave_up,
+                                                      a.wait_ns))) {
+          gone = true;
+          for (int i = k; i < min(k + kDecStages, steps); ++i)
+            sm100::mbar_wait(&bars[(steps_done + i) % kDecStages], ((steps_done + i) / kDecStages) & 1u, nullptr, nullptr,
+                             kKv4DrainNs);
+          break;
+        }
         const uint32_t have = held >> (kDecUnits * stage) & kAll;
         const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
         const uint8_t *buf = ring + stage * kDecUnits * L::kUnit;
@@ -578,7 +595,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       for (int i = 0; i < 4 * NB; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) nan |= isnan(o[i][c]);
-      if (!__any_sync(0xffffffffu, nan)) break;
+      if (gone || !__any_sync(0xffffffffu, nan)) break;
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -605,6 +622,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
       dst[0] = lo, dst[1] = hi;
     }
     __syncthreads();
+    gone = *gave_up;  // (no warp goes on before all have read it)
     const bool whole = s.t0 == 0 && s.t1 == s.whole;
     float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kDecRowTile, HD);
     for (int i = threadIdx.x; i < kDecRowTile * HD / 4; i += kDecWarps * 32) {
@@ -617,7 +635,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
         top = fmaxf(top, rw[w]);
       }
       const float shift = top == -INFINITY ? 0.0f : top;
-      float total = 0.0f;
+      float total = gone ? __uint_as_float(0x7fc00000u) : 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
@@ -690,18 +708,41 @@ __device__ __forceinline__ void kv4_write(const Kv4AttnArgs &a, int4 m, int fr, 
   else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
 }
 
+// NaN to all rows of the items that CTA `cta` of the many-row kernel had, or began. (A call, so that its registers are
+// no matter to the join.)
+template <int NB>
+__device__ __noinline__ void kv4_void(const Kv4AttnArgs &a, int cta, int grid) {
+  constexpr int HD = 32 * NB;
+  Kv4Walk w;
+  Kv4Segment s;
+  if (!kv4_walk<kManyTile, kManyTile>(a, w, cta, grid)) return;
+  while (kv4_next<kManyTile, kManyTile>(a, w, s)) {
+    if (s.t0) continue;  // begun by an earlier CTA, whose join looks at this one's state
+    for (int i = threadIdx.x; i < kManyTile * HD; i += blockDim.x) {
+      const int f = s.tile * kManyTile + i / HD;
+      if (f < s.q.flat)
+        a.out[(int64_t)(s.q.row0 + f / a.group) * a.ld_o + (int64_t)(s.head * a.group + f % a.group) * a.hs_o + i % HD] =
+            __uint_as_float(0x7fc00000u);
+    }
+  }
+}
+
 template <int NB>
 __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
-    kv4_join_kernel(const Kv4AttnArgs a, const Kv4Join j) {
+    kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a, const Kv4Join j) {
   constexpr int HD = 32 * NB, kQuads = HD / 4, kLanes = kJoinRows * kQuads;
   __shared__ float4 s_acc[kJoinSlices][kLanes];
   __shared__ float s_top[kJoinSlices][kJoinRows], s_sum[kJoinSlices][kJoinRows];
   sm100::griddep_wait();
   if ((int)blockIdx.x >= j.ctas[0]) {
-    constexpr int kRows = 128, kChunks = kRows / kJoinMany;
+    constexpr int kRows = kManyTile, kChunks = kRows / kJoinMany;
     const int at = blockIdx.x - j.ctas[0], b = at / kChunks;
-    const int4 m = j.meta[1][2 * b];
-    const int parts = j.meta[1][2 * b + 1].x;
+    const int4 m = j.meta[1][2 * b], state = j.meta[1][2 * b + 1];
+    if (state.y) {
+      if (at % kChunks == 0) kv4_void<NB>(a, b, j.ctas[1]);
+      return;
+    }
+    const int parts = state.x;
     if (parts == 0) return;
     constexpr int64_t kStride = kv4_part_floats(kRows, HD);
     const float *parts0 = j.parts[1] + 2 * b * kStride;
@@ -712,6 +753,7 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
     for (int n = 0; n < kJoinEach; ++n) top[n] = -INFINITY, total[n] = 0.0f, acc[n] = make_float4(0, 0, 0, 0);
     for (int i = 0; i < parts; ++i) {
       const float *p = kv4_part(parts0, i, kStride);
+      const bool gone = j.meta[1][2 * (b + i) + 1].y;  // the CTA gave up: its part may be anything
       float ref[kJoinEach], sum[kJoinEach];
       float4 v[kJoinEach];
 #pragma unroll
@@ -722,6 +764,7 @@ __global__ void __launch_bounds__(kJoinRows * 8 * NB * kJoinSlices)
           ref[n] = p[row], sum[n] = p[kRows + row];
           v[n] = *reinterpret_cast<const float4 *>(p + 2 * kRows + row * HD + e);
         }
+        if (gone) ref[n] = 0.0f, sum[n] = __uint_as_float(0x7fc00000u);
       }
 #pragma unroll
       for (int n = 0; n < kJoinEach; ++n) kv4_add_part(top[n], total[n], acc[n], ref[n], sum[n], v[n]);

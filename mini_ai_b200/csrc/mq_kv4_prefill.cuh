@@ -31,8 +31,8 @@
 
 namespace mq {
 
-constexpr int kPreRows = 128;    // RT
-constexpr int kPreTokens = 128;  // BN
+constexpr int kPreRows = kManyTile;    // RT
+constexpr int kPreTokens = kManyTile;  // BN
 constexpr int kPreSoft = 256;      // softmax threads
 constexpr int kPreThreads = kPreSoft + 512;
 constexpr int kPreGroups = kPreSoft / kPreRows;      // threads of a row
@@ -45,7 +45,6 @@ constexpr int kPreMasks = 4;
 constexpr int kPreSegs = 4;
 constexpr int kStageRow = 80;  // bytes: 16 floats; 8 rows meet all banks once
 constexpr int kPreUnits = kPreTokens / kKv4Unit;
-constexpr uint64_t kPreDrainNs = 20000000ull;
 
 // A segment as the roles need it.
 enum { kSegEnd = 0, kSegWhole = 1, kSegTail = 2, kSegHead = 3 };  // of an item: all, a later part, its first part
@@ -201,9 +200,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
   }
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
-  if (threadIdx.x == kWarpWalk * 32) a.meta[2 * blockIdx.x + 1].x = 0;  // the walker's
+  if (threadIdx.x == kWarpWalk * 32) a.meta[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);  // the walker's
   Kv4Walk walk;
-  const bool work = kv4_walk<kPreRows, kPreTokens>(a, walk);
+  const bool work = kv4_walk<kPreRows, kPreTokens>(a, walk, blockIdx.x, gridDim.x);
   if (work) {
     if (warp == kWarpMma) {
       sm100::tmem_alloc(tmem_slot, 512);
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Waits sleep in the barrier: polling took as many issue slots as the work.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-      return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, kKv4WaitNs);
+      return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, a.wait_ns);
     };
     Ring<kPreSegs> sg;
     // The next segment of a role's warp; false at the end. seg_done() lets the walker reuse its place.
@@ -677,7 +676,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         Ring<2> pbuf;  // of the next output
         bool ok = true;
         auto all_wait = [&](uint64_t *bar, uint32_t parity) {
-          return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, nullptr, abort, kKv4WaitNs)) != 0;
+          return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, nullptr, abort, a.wait_ns)) != 0;
         };
         for (; ok && seg_next(); seg_done()) {
           const int steps = segs[sg.i].steps;
@@ -731,7 +730,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
         if (elect_one()) {  // every MMA has completed before the TMEM is released
           sm100::umma_commit(fin);
-          sm100::mbar_wait(fin, 0u, nullptr, nullptr, kPreDrainNs);
+          if (!sm100::mbar_wait(fin, 0u, nullptr, nullptr, kKv4DrainNs)) *abort = 1;
         }
       } else if (warp == kWarpCopy) {
         // ------------------------------------------------------ copies of the packed units
@@ -754,7 +753,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             if (!ok) break;
             if (lane == 0) {
               raw_valid[raw.i] = have;
-              sm100::mbar_arrive_expect_tx(&raw_full[raw.i], __popc(have) * UB);
+              sm100::mbar_arrive_expect_tx(&raw_full[raw.i], __popc(have) * UB + a.lost);
             }
             __syncwarp();
             if (id >= 0)
@@ -766,7 +765,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
         // the last copies have landed before the CTA can exit
         for (int i = max(0, issued - kPreRaw); i < issued; ++i)
-          sm100::mbar_wait(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u, nullptr, nullptr, kPreDrainNs);
+          if (!sm100::mbar_wait(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u, nullptr, nullptr, kKv4DrainNs))
+            *abort = 1;
       } else if (warp == kWarpWalk && lane == 0) {
         // ------------------------------------------------------ the walk over the items
         Kv4Segment s;
@@ -795,6 +795,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     __syncwarp();
     sm100::tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort) {  // the roles have left the items that were still to come: the join sees to them
+      a.meta[2 * blockIdx.x + 1].y = 1;
+      atomicExch(a.err, 1);
+    }
     if (warp == kWarpMma) {
       sm100::tc_fence_after();
       sm100::tmem_dealloc(tmem, 512);

@@ -55,4 +55,7 @@ int run_linear_peer(const mq_weight *w, const float *x, int m, int64_t ldx, cons
 
 bool gemm_supported(int device);
 
+// The device's bounded-wait error flag (mq_device_error_flag), as its kernels and as the host see it.
+int device_err_flag(int device, int **dev_ptr, int **host_ptr);
+
 }  // namespace mq

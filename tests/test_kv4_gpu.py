@@ -843,3 +843,51 @@ def test_a_failed_call_leaves_no_error_behind(mq, torch):
     mq.ReleasePages(ints(torch, [0]), lens, tables, stack, n_free, 16)
     assert n_free.tolist() == [2] and stack.tolist() == [7, 0]
     w.close()
+
+
+WAITS = [  # heads, kv, head size, cached tokens, new rows: few rows whole and cut; many rows whole, cut, many items a CTA
+    (8, 2, 64, [100, 33], [1, 1], 16), (16, 2, 128, [20000, 40], [1, 1], 64), (4, 4, 32, [70] * 600, [1] * 600, 16),
+    (8, 1, 128, [2500], [600], 64), (2, 2, 96, [1500, 1400, 9], [1500, 700, 1], 64), (32, 8, 64, [1500], [1400], 64)]
+
+
+@pytest.mark.parametrize("heads,kv,hd,lens,news,page", WAITS)
+def test_waits_that_run_out(mq, torch, monkeypatch, heads, kv, hd, lens, news, page):
+    """Copies that never complete: every row is NaN, whichever CTA had it; the next call says so, once."""
+    monkeypatch.setenv("MQ_KV4_LOSE_COPIES", "1")
+    monkeypatch.setenv("MQ_KV4_WAIT_NS", "2000000")
+    b = Batch(mq, torch, lens, kv, hd, page, seed=1)
+    monkeypatch.delenv("MQ_KV4_LOSE_COPIES")
+    monkeypatch.delenv("MQ_KV4_WAIT_NS")
+    good = Batch(mq, torch, lens, kv, hd, page, seed=1)
+    q, want = run_attention(torch, good, heads, news, 2, max_new=max(news))
+    torch.cuda.synchronize()
+    launches = mq.lib().mq_kernel_launches()
+    for again in range(2):
+        _, out = run_attention(torch, b, heads, news, 2, max_new=max(news))
+        torch.cuda.synchronize()
+        assert torch.isnan(out[:-2]).all() and (out[-2:] == 7.0).all()
+        before = mq.lib().mq_kernel_launches()
+        with pytest.raises(mq.MQError, match="bounded wait") as info:
+            run_attention(torch, b if again else good, heads, news, 2, max_new=max(news))
+        assert info.value.code == mq._lib.MQ_ERR_TIMEOUT
+        assert mq.lib().mq_kernel_launches() == before > launches
+    _, out = run_attention(torch, good, heads, news, 2, max_new=max(news))
+    assert torch.equal(out, want)
+
+
+def test_wait_flag_of_the_device(mq, torch):
+    """The device's flag, raised as any tensor-core kernel raises it, fails the next attention before its launch."""
+    import ctypes as C
+
+    from cuda.bindings import runtime as rt
+
+    b = Batch(mq, torch, [50], 1, 32, 16, seed=1)
+    _, want = run_attention(torch, b, 2, [1], 1, max_new=1)
+    flag = C.c_void_p()
+    assert mq.lib().mq_device_error_flag(0, C.byref(flag)) == 0
+    assert int(rt.cudaMemset(flag.value, 1, 4)[0]) == 0
+    torch.cuda.synchronize()
+    with pytest.raises(mq.MQError) as info:
+        run_attention(torch, b, 2, [1], 1, max_new=1)
+    assert info.value.code == mq._lib.MQ_ERR_TIMEOUT
+    assert torch.equal(run_attention(torch, b, 2, [1], 1, max_new=1)[1], want)
