@@ -191,7 +191,7 @@ size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head
  * caller's device memory for it (at least mq_kv4_bytes(), 16-byte aligned),
  * which must outlive the handle and is cleared on `stream`; NULL allocates
  * it, which synchronizes `stream`. MQ_KV4_WAIT_NS in the environment limits
- * each wait inside the cache's attention (nanoseconds, default 1 s); with
+ * each wait inside the cache's attention (nanoseconds, default 1 s, at most 10 s); with
  * MQ_KV4_LOSE_COPIES=1 every such wait runs out, so that a program's handling
  * of MQ_ERR_TIMEOUT can be tried. */
 int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads, int head_dim, void *memory,

@@ -98,7 +98,7 @@ bool env_set(const char *name) {
 uint64_t wait_limit() {
   const char *e = std::getenv("MQ_KV4_WAIT_NS");
   const unsigned long long ns = e ? std::strtoull(e, nullptr, 10) : 0;
-  return ns ? ns : kKv4WaitNs;
+  return ns ? std::min<uint64_t>(ns, 10 * kKv4WaitNs) : kKv4WaitNs;  // (never without a bound)
 }
 
 int launched(const char *what) {
