@@ -292,6 +292,16 @@ __device__ __forceinline__ float half_at(const uint32_t (&a)[W], int j) {
   return __half2float(__ushort_as_half((uint16_t)(a[j >> 1] >> (j & 1 ? 16 : 0))));
 }
 
+// acc and total, in units of 2^top, joined with another sum; all -inf: nothing was seen.
+__device__ __forceinline__ void kv4_add_part(float &top, float &total, float4 &acc, float ref, float sum, float4 v) {
+  const float now = fmaxf(top, ref), shift = now == -INFINITY ? 0.0f : now;
+  const float old = ex2(top - shift), k = ex2(ref - shift);
+  top = now;
+  total = total * old + k * sum;
+  acc.x = acc.x * old + k * v.x, acc.y = acc.y * old + k * v.y;
+  acc.z = acc.z * old + k * v.z, acc.w = acc.w * old + k * v.w;
+}
+
 // ------------------------------------------------------------ few rows
 // One CTA, 4 warps, 8 flat rows an item. Every warp streams its own 16-token
 // units through a ring of bulk copies in shared memory, without a barrier to
@@ -320,6 +330,11 @@ constexpr int kDecRowTile = 8;
 constexpr int kDecUnits = 2;   // per warp and step
 constexpr int kDecTokens = kDecWarps * kDecUnits * kKv4Unit;  // BN
 constexpr int kDecStages = 3;
+// Steps that one accumulator sums, two products each: a product truncates what it adds to, by up to 2^-23 of it and
+// always towards 0, and equal weights added one by one round the same way every time. 131072 tokens a CTA put outputs
+// 1.9e-4 off in one chain. Chains are joined in F32, in the place of the item's part; CTAs
+// of up to 4096 tokens have one. 32 requests of 32768 tokens, 8 KV heads of 128: 412 us (64 steps: 409, no bound: 408).
+constexpr int kDecChain = 32;
 constexpr uint64_t kKv4WaitNs = 1000000000ull;  // limit of a wait, unless the cache was made with another
 constexpr uint64_t kKv4DrainNs = 20000000ull;   // for what a CTA that gave up still has in flight
 
@@ -350,6 +365,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
     sm100::fence_mbar_init();
   }
   __shared__ int s_gone;  // a wait of this CTA ran out: all its rows from here on are NaN
+  __shared__ float s_kept[2][2][kDecRowTile];  // of even and odd chains: references and sums
   if (threadIdx.x == 0) s_gone = 0;
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
@@ -372,9 +388,6 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
     const int last = min(s.q.base + qi, s.q.len - 1);
     const int last_min = min(s.q.base + s.tile * kDecRowTile / a.group, s.q.len - 1);
     const int last_max = min(s.q.base + (min((s.tile + 1) * kDecRowTile, s.q.flat) - 1) / a.group, s.q.len - 1);
-    const int first_unit = s.t0 * (kDecTokens / kKv4Unit);
-    const int end_unit = min(s.t1 * (kDecTokens / kKv4Unit), (last_max + kKv4Unit) / kKv4Unit);
-    const int steps = gone ? 0 : max(0, (end_unit - first_unit + kDecWarps * kDecUnits - 1) / (kDecWarps * kDecUnits));
     const int *table = a.tables + (int64_t)s.r * a.width;
     const uint8_t *slice = kv4_unit(a.c, a.layer, 0, s.head, 0);
 
@@ -421,248 +434,261 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv4_decode_kernel(const Kv4
         }
     }
 
-    float o[4 * NB][4];
-    float ref, sum;       // weights are 2^(score - ref): at most 2^15; their sum over this thread's tokens
-    uint32_t poison = 0;  // blocks of this row with a NaN value that it sees
-    // A row that does not see a token weighs it 0, which a NaN value would not
-    // respect: a segment whose output has a NaN is done again with such values
-    // set to 0 and the rows that see them marked.
-    for (int careful = 0; careful < 2; ++careful) {
+    int from = s.t0;  // of the chain
+    do {
+      const int to = min(from + kDecChain, s.t1);
+      const int first_unit = from * (kDecTokens / kKv4Unit);
+      const int end_unit = min(to * (kDecTokens / kKv4Unit), (last_max + kKv4Unit) / kKv4Unit);
+      const int steps =
+          gone ? 0 : max(0, (end_unit - first_unit + kDecWarps * kDecUnits - 1) / (kDecWarps * kDecUnits));
+      float o[4 * NB][4];
+      float ref, sum;       // weights are 2^(score - ref): at most 2^15; their sum over this thread's tokens
+      uint32_t poison = 0;  // blocks of this row with a NaN value that it sees
+      // A row that does not see a token weighs it 0, which a NaN value would not
+      // respect: a segment whose output has a NaN is done again with such values
+      // set to 0 and the rows that see them marked.
+      for (int careful = 0; careful < 2; ++careful) {
 #pragma unroll
-      for (int i = 0; i < 4 * NB; ++i)
+        for (int i = 0; i < 4 * NB; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
-      ref = -INFINITY, sum = 0.0f;
+          for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
+        ref = -INFINITY, sum = 0.0f;
 
-      // The ring: step k of this warp is units first_unit + (k * 4 + warp) * 2 + {0, 1}.
-      uint32_t held = 0;  // kDecUnits bits a stage: units that were fetched
-      // Every kPer steps each lane looks up one unit of the next kPer, and copies it when its step comes.
-      const uint8_t *unit_at = nullptr;
-      uint32_t there = 0;  // lanes whose unit is in the cache
-      auto fetch = [&](int k) {
-        if (k % kPer == 0) {
-          const int u = first_unit + ((k + lane / kDecUnits) * kDecWarps + warp) * kDecUnits + lane % kDecUnits;
-          const int id = u < end_unit ? __ldg(table + u / upp) : -1;
-          const bool in = id >= 0 && id < a.c.pages;
-          unit_at = slice + id * unit_page + (int64_t)(u % upp) * L::kUnit;
-          there = __ballot_sync(0xffffffffu, in);
-        }
-        const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (kDecUnits * (k % kPer)) & kAll;
-        held = (held & ~(kAll << (kDecUnits * stage))) | have << (kDecUnits * stage);
-        if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit + a.lost);
-        __syncwarp();
-        if (lane / kDecUnits == k % kPer && (there >> lane & 1u))
-          sm100::bulk_load(ring + (stage * kDecUnits + lane % kDecUnits) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
-      };
-      for (int k = 0; k < min(kDecStages - 1, steps); ++k) fetch(k);
-
-      for (int k = 0; k < steps; ++k) {
-        if (k + kDecStages - 1 < steps) fetch(k + kDecStages - 1);
-        const uint32_t stage = (steps_done + k) % kDecStages;
-        if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, a.err, gave_up,
-                                                      a.wait_ns))) {
-          gone = true;
-          for (int i = k; i < min(k + kDecStages, steps); ++i)
-            sm100::mbar_wait(&bars[(steps_done + i) % kDecStages], ((steps_done + i) / kDecStages) & 1u, nullptr, nullptr,
-                             kKv4DrainNs);
-          break;
-        }
-        const uint32_t have = held >> (kDecUnits * stage) & kAll;
-        const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
-        const uint8_t *buf = ring + stage * kDecUnits * L::kUnit;
-
-        // ---- scores: sc[unit][tile i][b] of token t + 4 b + 8 i
-        float sc[kDecUnits][2][2];
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kDecUnits; ++j) {
-          const uint8_t *unit = buf + j * L::kUnit;
-          if (!(have >> j & 1u)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[j][i >> 1][i & 1] = -INFINITY;
-            continue;
+        // The ring: step k of this warp is units first_unit + (k * 4 + warp) * 2 + {0, 1}.
+        uint32_t held = 0;  // kDecUnits bits a stage: units that were fetched
+        // Every kPer steps each lane looks up one unit of the next kPer, and copies it when its step comes.
+        const uint8_t *unit_at = nullptr;
+        uint32_t there = 0;  // lanes whose unit is in the cache
+        auto fetch = [&](int k) {
+          if (k % kPer == 0) {
+            const int u = first_unit + ((k + lane / kDecUnits) * kDecWarps + warp) * kDecUnits + lane % kDecUnits;
+            const int id = u < end_unit ? __ldg(table + u / upp) : -1;
+            const bool in = id >= 0 && id < a.c.pages;
+            unit_at = slice + id * unit_page + (int64_t)(u % upp) * L::kUnit;
+            there = __ballot_sync(0xffffffffu, in);
           }
+          const uint32_t stage = (steps_done + k) % kDecStages, have = there >> (kDecUnits * (k % kPer)) & kAll;
+          held = (held & ~(kAll << (kDecUnits * stage))) | have << (kDecUnits * stage);
+          if (lane == 0) sm100::mbar_arrive_expect_tx(&bars[stage], __popc(have) * L::kUnit + a.lost);
+          __syncwarp();
+          if (lane / kDecUnits == k % kPer && (there >> lane & 1u))
+            sm100::bulk_load(ring + (stage * kDecUnits + lane % kDecUnits) * L::kUnit, unit_at, L::kUnit, &bars[stage]);
+        };
+        for (int k = 0; k < min(kDecStages - 1, steps); ++k) fetch(k);
+
+        for (int k = 0; k < steps; ++k) {
+          if (k + kDecStages - 1 < steps) fetch(k + kDecStages - 1);
+          const uint32_t stage = (steps_done + k) % kDecStages;
+          if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[stage], ((steps_done + k) / kDecStages) & 1u, a.err,
+                                                        gave_up, a.wait_ns))) {
+            gone = true;  // the copies in flight land before their places are used for anything else
+            for (uint32_t i = steps_done + k; i < steps_done + min(k + kDecStages, steps); ++i)
+              sm100::mbar_wait(&bars[i % kDecStages], (i / kDecStages) & 1u, nullptr, nullptr, kKv4DrainNs);
+            break;
+          }
+          const uint32_t have = held >> (kDecUnits * stage) & kAll;
+          const int u0 = first_unit + (k * kDecWarps + warp) * kDecUnits;
+          const uint8_t *buf = ring + stage * kDecUnits * L::kUnit;
+
+          // ---- scores: sc[unit][tile i][b] of token t + 4 b + 8 i
+          float sc[kDecUnits][2][2];
+          float mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t kw[NB];
-            const uint8_t *kp = unit + ((g >> 1) + 4 * (g & 1) + 8 * i) * (16 * NB) + t * (4 * NB);
-            if constexpr (NB == 4) {
-              const uint4 v = *reinterpret_cast<const uint4 *>(kp);
-              kw[0] = v.x, kw[1] = v.y, kw[2] = v.z, kw[3] = v.w;
-            } else if constexpr (NB == 2) {
-              const uint2 v = *reinterpret_cast<const uint2 *>(kp);
-              kw[0] = v.x, kw[1] = v.y;
-            } else {
+          for (int j = 0; j < kDecUnits; ++j) {
+            const uint8_t *unit = buf + j * L::kUnit;
+            if (!(have >> j & 1u)) {
 #pragma unroll
-              for (int b = 0; b < NB; ++b) kw[b] = reinterpret_cast<const uint32_t *>(kp)[b];
+              for (int i = 0; i < 4; ++i) sc[j][i >> 1][i & 1] = -INFINITY;
+              continue;
             }
-            uint32_t d0[W], d1[W];
-            lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 8 * i) * (2 * NB), d0);
-            lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 4 + 8 * i) * (2 * NB), d1);
-            uint64_t s01 = 0;  // the two tokens' scores
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              const uint32_t w = kw[b], w8 = w >> 8;
-              mma16816(c, qa[2 * b], h2_bits(code_lo(w)), h2_bits(code_hi(w)));
-              mma16816(c, qa[2 * b + 1], h2_bits(code_lo(w8)), h2_bits(code_hi(w8)));
-              const uint64_t dd = two(half_at(d0, b), half_at(d1, b));
-              s01 = fma_two(dd, two(c[0], c[1]), s01);
-              s01 = fma_two(dd, two(c[2], c[3]), s01);
-            }
-            const float2 s2 = of_two(mul_two(s01, two(fscale, fscale)));
-            sc[j][i][0] = s2.x, sc[j][i][1] = s2.y;
-          }
-          if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_min) {  // some row's end
+            for (int i = 0; i < 2; ++i) {
+              uint32_t kw[NB];
+              const uint8_t *kp = unit + ((g >> 1) + 4 * (g & 1) + 8 * i) * (16 * NB) + t * (4 * NB);
+              if constexpr (NB == 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(kp);
+                kw[0] = v.x, kw[1] = v.y, kw[2] = v.z, kw[3] = v.w;
+              } else if constexpr (NB == 2) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+                kw[0] = v.x, kw[1] = v.y;
+              } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if ((u0 + j) * kKv4Unit + t + 4 * (i & 1) + 8 * (i >> 1) > last) sc[j][i >> 1][i & 1] = -INFINITY;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[j][i >> 1][i & 1]);
-        }
-
-        // ---- the weights' reference: moved only when a weight would pass 2^15
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const bool grow = mx > ref + 15.0f || (ref == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float to = grow ? mx - 8.0f : ref;
-          const float old = grow ? ex2(ref - to) : 1.0f;
-          ref = to;
-          sum *= old;
-#pragma unroll
-          for (int i = 0; i < 4 * NB; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[i][c] *= old;
-        }
-        const float shift = ref == -INFINITY ? 0.0f : ref;
-
-        // ---- weights and output
-#pragma unroll
-        for (int j = 0; j < kDecUnits; ++j) {
-          if (!(have >> j & 1u)) continue;
-          const uint8_t *unit = buf + j * L::kUnit;
-          float p[4];  // tokens t, t + 4, t + 8, t + 12
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = ex2(sc[j][i >> 1][i & 1] - shift), sum += p[i];
-          uint32_t pa[4];
-          split_f16(p[0], p[1], pa[0], pa[1]);
-          split_f16(p[2], p[3], pa[2], pa[3]);
-          uint32_t vw[4][W], vd[4][W];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok = t + 4 * i;
-            lds_halves<NB>(unit + kv4_v_off(NB) + tok * (16 * NB) + g * (2 * NB), vw[i]);
-            lds_halves<NB>(unit + kv4_v_scale_off(NB) + tok * (2 * NB), vd[i]);
-          }
-          const int tok0 = (u0 + j) * kKv4Unit + t;
-          if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_max) {  // tokens that no row sees may hold anything
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (tok0 + 4 * i > last_max)
-#pragma unroll
-                for (int w = 0; w < W; ++w) vd[i][w] = 0u;
-          }
-          if (careful) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int b = 0; b < NB; ++b) kw[b] = reinterpret_cast<const uint32_t *>(kp)[b];
+              }
+              uint32_t d0[W], d1[W];
+              lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 8 * i) * (2 * NB), d0);
+              lds_halves<NB>(unit + kv4_k_scale_off(NB) + (t + 4 + 8 * i) * (2 * NB), d1);
+              uint64_t s01 = 0;  // the two tokens' scores
 #pragma unroll
               for (int b = 0; b < NB; ++b) {
-                const int sh = b & 1 ? 16 : 0;
-                if ((vd[i][b >> 1] >> sh & 0x7fffu) > 0x7c00u) {
-                  if (tok0 + 4 * i <= last) poison |= 1u << b;
-                  vd[i][b >> 1] &= ~(0xffffu << sh);
-                }
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t w = kw[b], w8 = w >> 8;
+                mma16816(c, qa[2 * b], h2_bits(code_lo(w)), h2_bits(code_hi(w)));
+                mma16816(c, qa[2 * b + 1], h2_bits(code_lo(w8)), h2_bits(code_hi(w8)));
+                const uint64_t dd = two(half_at(d0, b), half_at(d1, b));
+                s01 = fma_two(dd, two(c[0], c[1]), s01);
+                s01 = fma_two(dd, two(c[2], c[3]), s01);
               }
+              const float2 s2 = of_two(mul_two(s01, two(fscale, fscale)));
+              sc[j][i][0] = s2.x, sc[j][i][1] = s2.y;
+            }
+            if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_min) {  // some row's end
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if ((u0 + j) * kKv4Unit + t + 4 * (i & 1) + 8 * (i >> 1) > last) sc[j][i >> 1][i & 1] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[j][i >> 1][i & 1]);
           }
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const uint32_t x0 = pair_halves(vw[0], vw[1], b), x1 = pair_halves(vw[2], vw[3], b);
-            const __half2 e0 = bits_h2(pair_halves(vd[0], vd[1], b)), e1 = bits_h2(pair_halves(vd[2], vd[3], b));
-            const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-            mma16816(o[4 * b], pa, h2_bits(__hmul2(code_lo(x0), e0)), h2_bits(__hmul2(code_lo(x1), e1)));
-            mma16816(o[4 * b + 1], pa, h2_bits(__hmul2(code_hi(x0), e0)), h2_bits(__hmul2(code_hi(x1), e1)));
-            mma16816(o[4 * b + 2], pa, h2_bits(__hmul2(code_lo(y0), e0)), h2_bits(__hmul2(code_lo(y1), e1)));
-            mma16816(o[4 * b + 3], pa, h2_bits(__hmul2(code_hi(y0), e0)), h2_bits(__hmul2(code_hi(y1), e1)));
-          }
-        }
-        __syncwarp();  // the stage's readers are done before lane 0 refills it
-      }
-      steps_done += steps;
-      bool nan = false;
-#pragma unroll
-      for (int i = 0; i < 4 * NB; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) nan |= isnan(o[i][c]);
-      if (gone || !__any_sync(0xffffffffu, nan)) break;
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    poison |= __shfl_xor_sync(0xffffffffu, poison, 1);
-    poison |= __shfl_xor_sync(0xffffffffu, poison, 2);
 
-    // ---- join the warps through their rings
-    float *mine = reinterpret_cast<float *>(ring);
-    if (t == 0) {
-      mine[kDecRowTile * L::kRowStride + g] = ref;
-      mine[kDecRowTile * L::kRowStride + kDecRowTile + g] = sum;
-    }
+          // ---- the weights' reference: moved only when a weight would pass 2^15
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const bool grow = mx > ref + 15.0f || (ref == -INFINITY && mx > -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float to = grow ? mx - 8.0f : ref;
+            const float old = grow ? ex2(ref - to) : 1.0f;
+            ref = to;
+            sum *= old;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {  // n8-tile i of block b, column n is element 32 b + 4 n + i
-      float4 lo = make_float4(o[4 * b][0] + o[4 * b][2], o[4 * b + 1][0] + o[4 * b + 1][2],
-                              o[4 * b + 2][0] + o[4 * b + 2][2], o[4 * b + 3][0] + o[4 * b + 3][2]);
-      float4 hi = make_float4(o[4 * b][1] + o[4 * b][3], o[4 * b + 1][1] + o[4 * b + 1][3],
-                              o[4 * b + 2][1] + o[4 * b + 2][3], o[4 * b + 3][1] + o[4 * b + 3][3]);
-      if (poison >> b & 1u) {
-        const float x = __uint_as_float(0x7fc00000u);
-        lo = hi = make_float4(x, x, x, x);
-      }
-      float4 *dst = reinterpret_cast<float4 *>(mine + g * L::kRowStride + 32 * b + 8 * t);
-      dst[0] = lo, dst[1] = hi;
-    }
-    __syncthreads();
-    gone = *gave_up;  // (no warp goes on before all have read it)
-    const bool whole = s.t0 == 0 && s.t1 == s.whole;
-    float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kDecRowTile, HD);
-    for (int i = threadIdx.x; i < kDecRowTile * HD / 4; i += kDecWarps * 32) {
-      const int row = i / (HD / 4), e = 4 * (i % (HD / 4)), fr = s.tile * kDecRowTile + row;
-      if (fr >= s.q.flat) continue;
-      float rw[kDecWarps], top = -INFINITY;
+            for (int i = 0; i < 4 * NB; ++i)
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
-        rw[w] = reinterpret_cast<const float *>(sm + w * L::kRing)[kDecRowTile * L::kRowStride + row];
-        top = fmaxf(top, rw[w]);
-      }
-      const float shift = top == -INFINITY ? 0.0f : top;
-      float total = gone ? __uint_as_float(0x7fc00000u) : 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              for (int c = 0; c < 4; ++c) o[i][c] *= old;
+          }
+          const float shift = ref == -INFINITY ? 0.0f : ref;
+
+          // ---- weights and output
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
-        const float *src = reinterpret_cast<const float *>(sm + w * L::kRing);
-        const float k = ex2(rw[w] - shift);
-        const float4 v = *reinterpret_cast<const float4 *>(src + row * L::kRowStride + e);
-        total += k * src[kDecRowTile * L::kRowStride + kDecRowTile + row];
-        acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+          for (int j = 0; j < kDecUnits; ++j) {
+            if (!(have >> j & 1u)) continue;
+            const uint8_t *unit = buf + j * L::kUnit;
+            float p[4];  // tokens t, t + 4, t + 8, t + 12
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = ex2(sc[j][i >> 1][i & 1] - shift), sum += p[i];
+            uint32_t pa[4];
+            split_f16(p[0], p[1], pa[0], pa[1]);
+            split_f16(p[2], p[3], pa[2], pa[3]);
+            uint32_t vw[4][W], vd[4][W];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int tok = t + 4 * i;
+              lds_halves<NB>(unit + kv4_v_off(NB) + tok * (16 * NB) + g * (2 * NB), vw[i]);
+              lds_halves<NB>(unit + kv4_v_scale_off(NB) + tok * (2 * NB), vd[i]);
+            }
+            const int tok0 = (u0 + j) * kKv4Unit + t;
+            if ((u0 + j) * kKv4Unit + kKv4Unit - 1 > last_max) {  // tokens that no row sees may hold anything
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (tok0 + 4 * i > last_max)
+#pragma unroll
+                  for (int w = 0; w < W; ++w) vd[i][w] = 0u;
+            }
+            if (careful) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                  const int sh = b & 1 ? 16 : 0;
+                  if ((vd[i][b >> 1] >> sh & 0x7fffu) > 0x7c00u) {
+                    if (tok0 + 4 * i <= last) poison |= 1u << b;
+                    vd[i][b >> 1] &= ~(0xffffu << sh);
+                  }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t x0 = pair_halves(vw[0], vw[1], b), x1 = pair_halves(vw[2], vw[3], b);
+              const __half2 e0 = bits_h2(pair_halves(vd[0], vd[1], b)), e1 = bits_h2(pair_halves(vd[2], vd[3], b));
+              const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+              mma16816(o[4 * b], pa, h2_bits(__hmul2(code_lo(x0), e0)), h2_bits(__hmul2(code_lo(x1), e1)));
+              mma16816(o[4 * b + 1], pa, h2_bits(__hmul2(code_hi(x0), e0)), h2_bits(__hmul2(code_hi(x1), e1)));
+              mma16816(o[4 * b + 2], pa, h2_bits(__hmul2(code_lo(y0), e0)), h2_bits(__hmul2(code_lo(y1), e1)));
+              mma16816(o[4 * b + 3], pa, h2_bits(__hmul2(code_hi(y0), e0)), h2_bits(__hmul2(code_hi(y1), e1)));
+            }
+          }
+          __syncwarp();  // the stage's readers are done before lane 0 refills it
+        }
+        steps_done += steps;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < 4 * NB; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) nan |= isnan(o[i][c]);
+        if (gone || !__any_sync(0xffffffffu, nan)) break;
       }
-      if (whole) {
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-        float *dst = a.out + (int64_t)(s.q.row0 + fr / a.group) * a.ld_o +
-                     (int64_t)(s.head * a.group + fr % a.group) * a.hs_o + e;
-        if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
-        else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
-      } else {
-        *reinterpret_cast<float4 *>(part + 2 * kDecRowTile + row * HD + e) = acc;
-        if (e == 0) part[row] = top, part[kDecRowTile + row] = total;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      poison |= __shfl_xor_sync(0xffffffffu, poison, 1);
+      poison |= __shfl_xor_sync(0xffffffffu, poison, 2);
+
+      // ---- join the warps through their rings
+      float *mine = reinterpret_cast<float *>(ring);
+      if (t == 0) {
+        mine[kDecRowTile * L::kRowStride + g] = ref;
+        mine[kDecRowTile * L::kRowStride + kDecRowTile + g] = sum;
       }
-    }
-    if (threadIdx.x == 0 && s.t0 == 0 && !whole) {  // the item goes on in the next CTAs
-      a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
-      a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
-    }
-    __syncthreads();
-    sm100::fence_proxy_async_smem();  // the rings' next writers are bulk copies
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {  // n8-tile i of block b, column n is element 32 b + 4 n + i
+        float4 lo = make_float4(o[4 * b][0] + o[4 * b][2], o[4 * b + 1][0] + o[4 * b + 1][2],
+                                o[4 * b + 2][0] + o[4 * b + 2][2], o[4 * b + 3][0] + o[4 * b + 3][2]);
+        float4 hi = make_float4(o[4 * b][1] + o[4 * b][3], o[4 * b + 1][1] + o[4 * b + 1][3],
+                                o[4 * b + 2][1] + o[4 * b + 2][3], o[4 * b + 3][1] + o[4 * b + 3][3]);
+        if (poison >> b & 1u) {
+          const float x = __uint_as_float(0x7fc00000u);
+          lo = hi = make_float4(x, x, x, x);
+        }
+        float4 *dst = reinterpret_cast<float4 *>(mine + g * L::kRowStride + 32 * b + 8 * t);
+        dst[0] = lo, dst[1] = hi;
+      }
+      __syncthreads();
+      gone = *gave_up;  // (no warp goes on before all have read it)
+      const bool done = to == s.t1, whole = s.t0 == 0 && s.t1 == s.whole;
+      float *part = a.parts + (int64_t)(2 * blockIdx.x + (s.t0 == 0)) * kv4_part_floats(kDecRowTile, HD);
+      const int now = (from - s.t0) / kDecChain & 1;
+      for (int i = threadIdx.x; i < kDecRowTile * HD / 4; i += kDecWarps * 32) {
+        const int row = i / (HD / 4), e = 4 * (i % (HD / 4)), fr = s.tile * kDecRowTile + row;
+        if (fr >= s.q.flat) continue;
+        float rw[kDecWarps], top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) {
+          rw[w] = reinterpret_cast<const float *>(sm + w * L::kRing)[kDecRowTile * L::kRowStride + row];
+          top = fmaxf(top, rw[w]);
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float total = gone ? __uint_as_float(0x7fc00000u) : 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) {
+          const float *src = reinterpret_cast<const float *>(sm + w * L::kRing);
+          const float k = ex2(rw[w] - shift);
+          const float4 v = *reinterpret_cast<const float4 *>(src + row * L::kRowStride + e);
+          total += k * src[kDecRowTile * L::kRowStride + kDecRowTile + row];
+          acc.x += k * v.x, acc.y += k * v.y, acc.z += k * v.z, acc.w += k * v.w;
+        }
+        if (from > s.t0)  // the chains before, kept where the item's part has its place
+          kv4_add_part(top, total, acc, s_kept[now ^ 1][0][row], s_kept[now ^ 1][1][row],
+                       *reinterpret_cast<const float4 *>(part + 2 * kDecRowTile + row * HD + e));
+        if (done && whole) {
+          const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+          acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+          float *dst = a.out + (int64_t)(s.q.row0 + fr / a.group) * a.ld_o +
+                       (int64_t)(s.head * a.group + fr % a.group) * a.hs_o + e;
+          if (a.vec_o) *reinterpret_cast<float4 *>(dst) = acc;
+          else dst[0] = acc.x, dst[1] = acc.y, dst[2] = acc.z, dst[3] = acc.w;
+        } else {
+          *reinterpret_cast<float4 *>(part + 2 * kDecRowTile + row * HD + e) = acc;
+          if (e == 0 && done) part[row] = top, part[kDecRowTile + row] = total;
+          if (e == 0 && !done) s_kept[now][0][row] = top, s_kept[now][1][row] = total;
+        }
+      }
+      if (threadIdx.x == 0 && s.t0 == 0 && !whole && done) {  // the item goes on in the next CTAs
+        a.meta[2 * blockIdx.x] = make_int4(s.q.row0, s.tile, s.head, s.q.flat);
+        a.meta[2 * blockIdx.x + 1].x = kv4_spread(walk, walk.place - s.t1 + s.whole);
+      }
+      __syncthreads();
+      sm100::fence_proxy_async_smem();  // the rings' next writers are bulk copies
+      from = to;
+    } while (from < s.t1);
   }
 }
 
@@ -686,16 +712,6 @@ constexpr int kJoinMany = kJoinRows * kJoinSlices * kJoinEach;  // rows a block 
 // `parts0`: the two places of the item's first CTA; its own part is the second.
 __device__ __forceinline__ const float *kv4_part(const float *parts0, int i, int64_t stride) {
   return parts0 + (2 * i + (i == 0)) * stride;
-}
-
-// acc and total, in units of 2^top, joined with another sum; all -inf: nothing was seen.
-__device__ __forceinline__ void kv4_add_part(float &top, float &total, float4 &acc, float ref, float sum, float4 v) {
-  const float now = fmaxf(top, ref), shift = now == -INFINITY ? 0.0f : now;
-  const float old = ex2(top - shift), k = ex2(ref - shift);
-  top = now;
-  total = total * old + k * sum;
-  acc.x = acc.x * old + k * v.x, acc.y = acc.y * old + k * v.y;
-  acc.z = acc.z * old + k * v.z, acc.w = acc.w * old + k * v.w;
 }
 
 // Row fr of the item `m` (Kv4AttnArgs::meta): acc / total to elements e..e + 3.

@@ -891,3 +891,56 @@ def test_wait_flag_of_the_device(mq, torch):
         run_attention(torch, b, 2, [1], 1, max_new=1)
     assert info.value.code == mq._lib.MQ_ERR_TIMEOUT
     assert torch.equal(run_attention(torch, b, 2, [1], 1, max_new=1)[1], want)
+
+
+def _shared(mq, torch, n, length, kv, hd, k, v):
+    """n requests over the same `length` cached tokens: (cache, tables)."""
+    page = 1024
+    pages = -(-length // page)
+    c = mq.Kv4Cache(1, pages, page, kv, hd)
+    c.store(0, k, v, torch.arange(length, dtype=torch.int32, device="cuda"))
+    return c, torch.arange(pages, dtype=torch.int32, device="cuda").expand(n, pages).contiguous()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_long_sums_of_values(mq, torch, hd):
+    """Every CTA of the few-row kernel has 131072 tokens of its own and values of one sign: the sums' roundings must not
+    add up. One item a CTA; all requests share the pages."""
+    length, heads = 131072, 8
+    n = 3 * torch.cuda.get_device_properties(0).multi_processor_count
+    g = torch.Generator().manual_seed(hd)
+    k, v = torch.randn(length, 1, hd, generator=g) * 2, 1 + 0.1 * torch.randn(length, 1, hd, generator=g)
+    c, tables = _shared(mq, torch, n, length, 1, hd, k.cuda(), v.cuda())
+    q = torch.randn(n, heads, hd, generator=g).cuda()
+    scale = 0.05 / hd
+    out = c.attention(0, q, ints(torch, np.arange(n + 1)), ints(torch, [length] * n), tables, max_new=1, scale=scale)
+    hk, hv = (torch.from_numpy(ref_blocks_fast(torch, x)).cuda()[:, 0] for x in (k, v))
+    for r in range(0, n, 37):
+        qq = q[r:r + 37].double()
+        p = torch.softmax(qq @ hk.T * scale, -1)
+        size = (qq.abs() @ hk.abs().T).amax(-1) * scale
+        rel = 2 * (size * (2 ** -22 + 44 * 2 ** -23) + 2 ** -21) + 256 * 2 ** -23
+        tol = rel[..., None] * (p @ hv.abs()) + 2 ** -33 * p.amax(-1)[..., None] * hv.abs().sum(0)
+        assert_attention(torch, out[r:r + 37], p @ hv, tol)
+
+
+@pytest.mark.parametrize("new", [1])
+def test_long_sums_of_weights(mq, torch, new):
+    """A few strong tokens, and behind them thousands of equal weights whose 24 bits fall between the sum's: added one by
+    one, each 4096 of them round the sum up by 5.4e-5 of it. All values are 1, so every output is 1. One item a CTA.
+
+    Both sums are of the same weights p, which enter the one over values as hi + lo, off by 2^-22 of it. Few rows: a
+    thread adds 256 weights and a product 64 units between two that are kept, and 32 of these; many rows: 32 and 16
+    additions a step, 128 steps. Tensor cores' additions are off by 2^-23, others by 2^-24 of the sum:
+    (4 + 256 + 32 + 2 * 64 + 32 + 8) and (4 + 32 + 128 + 2 * 16 + 128 + 8) * 2^-24, 8 for the joins and the quotient."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    length, n, heads = (65536, 3 * sms, 8) if new == 1 else (16384, sms // 2, 4)
+    hd, bits = 32, 3.997  # the weights' logarithm below the strong tokens'
+    k, v = torch.zeros(length, 1, hd, device="cuda"), torch.ones(length, 1, hd, device="cuda")
+    k[[0, 32, 64, 96]] = 1.0  # for each of the few-row kernel's warps
+    c, tables = _shared(mq, torch, n, length, 1, hd, k, v)
+    q = torch.ones(n * new, heads, hd, device="cuda")
+    out = c.attention(0, q, ints(torch, np.arange(n + 1) * new), ints(torch, [length] * n), tables, max_new=new,
+                      scale=bits * math.log(2) / hd)
+    off = float((out.double() - 1).abs().max())
+    assert off <= (460 if new == 1 else 332) * 2 ** -24, off
