@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
             mask.next();
             const float shift = ref == -INFINITY ? 0.0f : ref;
             const uint64_t shifts = two(-shift, -shift), scales = two(scale, scale);
-            sums = mul_two(sums, two(old, old));
+            uint64_t here = 0;  // the weights of the step (thousands of equal ones, added one by one, round one way)
 #pragma unroll 1
             for (int c = 0; c < kPreCols; c += 16) {
               uint32_t r[16], w[16];
@@ -393,11 +393,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
               for (int i = 0; i < 16; i += 2) {
                 const float2 z = of_two(fma_two(two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scales, shifts));
                 const float p0 = ex2(z.x), p1 = ex2(z.y);
-                sums = add_two(sums, two(p0, p1));
+                here = add_two(here, two(p0, p1));
                 split_f16(p0, p1, w[i >> 1], w[8 + (i >> 1)]);
               }
               tm_st16(cols + c, w);
             }
+            sums = fma_two(sums, two(old, old), here);
             tm_st_wait();
             sm100::tc_fence_before();
             sm100::mbar_arrive(done);

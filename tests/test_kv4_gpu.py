@@ -924,7 +924,7 @@ def test_long_sums_of_values(mq, torch, hd):
         assert_attention(torch, out[r:r + 37], p @ hv, tol)
 
 
-@pytest.mark.parametrize("new", [1])
+@pytest.mark.parametrize("new", [1, 64])
 def test_long_sums_of_weights(mq, torch, new):
     """A few strong tokens, and behind them thousands of equal weights whose 24 bits fall between the sum's: added one by
     one, each 4096 of them round the sum up by 5.4e-5 of it. All values are 1, so every output is 1. One item a CTA.
