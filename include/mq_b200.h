@@ -231,8 +231,8 @@ size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new);
  * seen. A row that sees nothing is 0; rows past offsets[n_seqs] stay as they
  * are, and no row past `rows` is touched. max_new: the most rows that a
  * request brings, as far as the caller knows; it selects kernels and a lower
- * or higher value costs time only. q and out as in mq_kv4_store; out may be q
- * only if it has q's strides. F32 softmax and sums; q and the softmax weights
+ * or higher value costs time only. q and out as in mq_kv4_store, no two heads
+ * of out sharing memory; out may be q only if it has q's strides. F32 softmax and sums; q and the softmax weights
  * enter the tensor cores as fp16 hi + lo pairs (22 bits). workspace: device
  * memory of at least mq_kv4_attention_workspace() bytes, 16-byte aligned,
  * not shared with a call that may run at the same time; its contents do not

@@ -55,6 +55,19 @@ int check_rows(const char *what, const float *p, int64_t ld, int64_t hs, int hea
   return MQ_OK;
 }
 
+// Whether heads of hd elements at i * ld + h * hs (hs >= hd) share memory.
+bool heads_overlap(int rows, int64_t ld, int heads, int64_t hs, int hd) {
+  using wide = __int128;
+  if (rows < 2) return false;
+  if (ld < hd) return true;
+  if (heads < 2 || ld >= (wide)(heads - 1) * hs + hd || hs >= (wide)(rows - 1) * ld + hd) return false;
+  for (int h = 1; h < heads; ++h) {  // rows between heads: the two rows on either side of each head's distance
+    const wide at = (wide)h * hs, i = at / ld;
+    if ((i < rows && at - i * ld < hd) || (i + 1 < rows && (i + 1) * ld - at < hd)) return true;
+  }
+  return false;
+}
+
 bool vector16(const void *p, int64_t ld, int64_t hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0 && hs % 4 == 0;
 }
@@ -339,7 +352,8 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   if (rows == 0 || n_seqs == 0) return MQ_OK;
   if (int rc = check_rows("query", q, ld_q, hs_q, heads, c->v.hd)) return rc;
   if (int rc = check_rows("output", out, ld_out, hs_out, heads, c->v.hd)) return rc;
-  if (rows > 1 && ld_out < c->v.hd) return fail(MQ_ERR_INVALID, "output rows overlap (stride %lld)", (long long)ld_out);
+  if (heads_overlap(rows, ld_out, heads, hs_out, c->v.hd))
+    return fail(MQ_ERR_INVALID, "heads of the output overlap (strides %lld, %lld)", (long long)ld_out, (long long)hs_out);
   if (!offsets || !seq_lens || !block_tables) return fail(MQ_ERR_INVALID, "null offsets, lengths or block tables");
   const size_t need = mq_kv4_attention_workspace(c, heads, max_new);
   if (!workspace || workspace_bytes < need)

@@ -944,3 +944,29 @@ def test_long_sums_of_weights(mq, torch, new):
                       scale=bits * math.log(2) / hd)
     off = float((out.double() - 1).abs().max())
     assert off <= (460 if new == 1 else 332) * 2 ** -24, off
+
+
+def test_output_layouts(mq, torch):
+    """Outputs whose heads share memory are refused; every layout in which they do not is written."""
+    b = Batch(mq, torch, [40, 30], 2, 64, 16, seed=2)
+    for rows, heads in ((2, 4), (6, 4), (2, 2)):
+        news = [rows // 2] * 2
+        q, want = run_attention(torch, b, heads, news, 1, spare=0)
+        offsets, lens = ints(torch, [0, news[0], rows]), ints(torch, b.lens)
+        memory = torch.empty(200 * 64, device="cuda")
+        taken = 0
+        for ld in (0, 32, 64, 96, 128, 129, 192, 255, 256, 320, 448, 512):
+            for hs in (64, 65, 96, 128, 192, 384, 512):
+                at = [i * ld + h * hs for i in range(rows) for h in range(heads)]
+                apart = all(abs(x - y) >= 64 for n, x in enumerate(at) for y in at[:n])
+                out = memory.as_strided((rows, heads, 64), (ld, hs, 1))
+                if apart:
+                    memory.fill_(7.0)
+                    b.cache.attention(0, q, offsets, lens, b.tables, out=out)
+                    assert torch.equal(out, want), (ld, hs)
+                    assert int((memory == 7.0).sum()) == memory.numel() - want.numel()
+                    taken += 1
+                else:
+                    with pytest.raises(ValueError, match="overlap"):
+                        b.cache.attention(0, q, offsets, lens, b.tables, out=out)
+        assert taken > 5
