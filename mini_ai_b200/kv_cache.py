@@ -86,21 +86,31 @@ class PagePlan:
     """What ``PlanPages`` writes: row offsets ``[n + 1]`` and lengths ``[n]`` of the requests, slots and
     positions ``[rows]`` (-1 behind the last request), the free pages left and the requests refused ``[1]``.
 
-    The tensors are checked here once and stay the plan's for its life.
+    The tensors are checked here once and stay the plan's for its life: they cannot be replaced.
     """
 
     __slots__ = ("offsets", "seq_lens", "slots", "positions", "n_free", "refused", "device", "_sizes", "_addresses")
 
     def __init__(self, offsets, seq_lens, slots, positions, n_free, refused):
         torch = _torch()
-        self.offsets, self.seq_lens, self.slots = offsets, seq_lens, slots
-        self.positions, self.n_free, self.refused = positions, n_free, refused
-        self.device = max(offsets.get_device(), 0)
+        device = max(offsets.get_device(), 0)
         n, rows = seq_lens.numel(), slots.numel()
-        self._sizes = (n, rows)
-        self._addresses = tuple(_ints(torch, name, t, self.device, size) for name, t, size in (
-            ("offsets", offsets, n + 1), ("seq_lens", seq_lens, n), ("slots", slots, rows),
-            ("positions", positions, rows), ("n_free", n_free, 1), ("refused", refused, 1)))
+        tensors = (("offsets", offsets, n + 1), ("seq_lens", seq_lens, n), ("slots", slots, rows),
+                   ("positions", positions, rows), ("n_free", n_free, 1), ("refused", refused, 1))
+        addresses = tuple(_ints(torch, name, t, device, size) for name, t, size in tensors)
+        for name, t, _ in tensors:
+            object.__setattr__(self, name, t)
+        for name, value in (("device", device), ("_sizes", (n, rows)), ("_addresses", addresses)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"PagePlan.{name} stays what the plan was made with")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"PagePlan.{name} stays what the plan was made with")
+
+    def __reduce__(self):  # a copy has its own tensors' addresses
+        return PagePlan, (self.offsets, self.seq_lens, self.slots, self.positions, self.n_free, self.refused)
 
     @classmethod
     def empty(cls, n_seqs: int, rows: int, device: int = 0, seq_lens=None, n_free=None, stream=None) -> "PagePlan":

@@ -93,3 +93,50 @@ def test_python_refuses_host_tensors(mq):
         mq.PlanPages(i, i, i, i, i[:1], 16, rows=4)
     with pytest.raises(RuntimeError, match="int32 tensor on cuda"):
         mq.ReleasePages(i, i, tables, i, i[:1], 16)
+
+
+class _Ints:
+    """An int32 tensor on cuda:0, as far as the argument checks look at it."""
+
+    def __init__(self, n, device=0, at=0x1000):
+        import torch
+
+        self.dtype, self.device, self.shape, self._n, self._device, self._at = torch.int32, "cuda:0", (n,), n, device, at
+
+    def get_device(self):
+        return self._device
+
+    def numel(self):
+        return self._n
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return self._at
+
+
+def test_a_plan_keeps_its_tensors(mq):
+    """The plan's addresses are taken once, so its tensors can be neither replaced nor dropped."""
+    plan = mq.PagePlan(_Ints(3), _Ints(2), _Ints(8), _Ints(8), _Ints(1), _Ints(1))
+    for name in ("offsets", "seq_lens", "slots", "positions", "n_free", "refused", "device"):
+        held = getattr(plan, name)
+        with pytest.raises(AttributeError, match="PagePlan"):
+            setattr(plan, name, _Ints(8))
+        with pytest.raises(AttributeError, match="PagePlan"):
+            delattr(plan, name)
+        assert getattr(plan, name) is held
+
+
+def test_a_copied_plan_has_its_own_addresses(mq):
+    import copy
+
+    plan = mq.PagePlan(_Ints(3), _Ints(2), _Ints(8), _Ints(8), _Ints(1), _Ints(1))
+    same = copy.copy(plan)
+    assert same.slots is plan.slots and same._addresses == plan._addresses
+    moved = [copy.copy(t) for t in (plan.offsets, plan.seq_lens, plan.slots, plan.positions, plan.n_free, plan.refused)]
+    for i, t in enumerate(moved):
+        t._at += 0x100 * (i + 1)
+    memo = {id(a): b for a, b in zip((plan.offsets, plan.seq_lens, plan.slots, plan.positions, plan.n_free, plan.refused), moved)}
+    other = copy.deepcopy(plan, memo)
+    assert other.slots is moved[2] and other._addresses == tuple(t._at for t in moved)
