@@ -52,12 +52,17 @@ def _empty(torch, shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _ints(torch, name: str, t, device: int, n: int) -> int:
+_MOST = 1 << 31  # counts are 32-bit in C: those that would wrap on their way there are refused here
+
+
+def _ints(torch, name: str, t, device: int, n: int, most: int = _MOST) -> int:
     """The address of `n` contiguous int32 values on `device`."""
-    if t.dtype is torch.int32 and t.get_device() == device and t.numel() == n and t.is_contiguous():
+    if t.dtype is torch.int32 and t.get_device() == device and t.numel() == n < most and t.is_contiguous():
         return t.data_ptr()
     if t.dtype is not torch.int32 or t.get_device() != device:
         raise RuntimeError(f"{name}: an int32 tensor on cuda:{device} is needed, not {t.dtype} on {t.device}")
+    if n >= most:
+        raise RuntimeError(f"{name}: shape mismatch ({n} values: they must stay below 2^31)")
     raise RuntimeError(f"{name}: shape mismatch ({n} contiguous values are needed, not {tuple(t.shape)})")
 
 
@@ -67,11 +72,13 @@ def _table(torch, t):
         raise RuntimeError("block_tables: shape mismatch ([requests, pages] is needed)")
     device = t.get_device()
     n, width = t.shape
-    return device, n, width, _ints(torch, "block_tables", t, max(device, 0), n * width)
+    if max(n, width) >= _MOST:
+        raise RuntimeError("block_tables: shape mismatch (requests and pages must stay below 2^31)")
+    return device, n, width, _ints(torch, "block_tables", t, max(device, 0), n * width, n * width + 1)
 
 
 def _page(page_size: int) -> int:
-    if page_size > 1024:  # (a size of more bits would wrap on its way into C)
+    if not 0 < page_size <= 1024:  # (a size of more bits would wrap on its way into C)
         raise ValueError(f"page size {page_size}: a multiple of 16 up to 1024 is needed")
     return page_size
 
@@ -170,7 +177,8 @@ class Kv4Cache:
                  stream=None):
         torch = _torch()
         self.handle = None
-        if max(layers, pages, page_size, kv_heads, head_dim) >= 1 << 31:  # would wrap on its way into C
+        sizes = (layers, pages, page_size, kv_heads, head_dim)
+        if max(sizes) >= _MOST or min(sizes) < -_MOST:
             raise ValueError("Kv4Cache: cache size overflow")
         need = lib().mq_kv4_bytes(layers, pages, page_size, kv_heads, head_dim)
         if not need:
@@ -202,7 +210,7 @@ class Kv4Cache:
         shape = t.shape
         if (t.dtype is torch.float32 and t.get_device() == self.device and len(shape) == 3
                 and shape[2] == self.head_dim and (heads is None or shape[1] == heads)
-                and (rows is None or shape[0] == rows)):
+                and (rows is None or shape[0] == rows) and shape[0] < _MOST and shape[1] < _MOST):
             strides = t.stride()
             if strides[2] == 1:
                 return shape, strides
@@ -263,6 +271,8 @@ class Kv4Cache:
             raise RuntimeError(f"output: shape mismatch ({out_rows} rows, {rows} of queries)")
         if max_new is None or max_new > rows:
             max_new = rows
+        elif max_new < 0:
+            max_new = -1  # (refused, however many bits it has)
         need = lib().mq_kv4_attention_workspace(self.handle, heads, max_new)
         ws = _empty(torch, need, torch.uint8, q.device, stream)
         _ok(lib().mq_kv4_attention(

@@ -140,3 +140,66 @@ def test_a_copied_plan_has_its_own_addresses(mq):
     memo = {id(a): b for a, b in zip((plan.offsets, plan.seq_lens, plan.slots, plan.positions, plan.n_free, plan.refused), moved)}
     other = copy.deepcopy(plan, memo)
     assert other.slots is moved[2] and other._addresses == tuple(t._at for t in moved)
+
+
+class _Table(_Ints):
+    def __init__(self, n, width):
+        super().__init__(n * width)
+        self.shape = (n, width)
+
+    def dim(self):
+        return 2
+
+
+class _Rows:
+    """F32 rows on cuda:0, all at one address."""
+
+    def __init__(self, rows, heads, hd):
+        import torch
+
+        self.dtype, self.device, self.shape = torch.float32, "cuda:0", (rows, heads, hd)
+
+    def get_device(self):
+        return 0
+
+    def stride(self):
+        return 0, self.shape[2], 1
+
+    def data_ptr(self):
+        return 0x1000
+
+
+def test_python_refuses_sizes_that_would_wrap(mq):
+    """Counts are 32-bit in C: larger ones are refused, not taken modulo 2^32."""
+    one, big = _Ints(1), (1 << 32) + 1
+    for n in (1 << 31, big):
+        with pytest.raises(RuntimeError, match="shape"):
+            mq.PagePlan(_Ints(2), one, _Ints(n), _Ints(n), one, one)
+        with pytest.raises(RuntimeError, match="shape"):
+            mq.ReleasePages(_Ints(n), one, _Table(1, 2), one, one, 16)
+        with pytest.raises(RuntimeError, match="shape"):
+            mq.ReleasePages(one, one, _Table(1, 2), _Ints(n), one, 16)
+        with pytest.raises(RuntimeError, match="shape"):
+            mq.ReleasePages(one, one, _Table(1, n), one, one, 16)
+    plan = mq.PagePlan(_Ints(2), one, _Ints(8), _Ints(8), one, one)
+    for page in (-(1 << 32) + 16, -(1 << 31) - 16, -16, 0):
+        with pytest.raises(ValueError, match="page size"):
+            mq.PlanPages(one, one, _Table(1, 2), one, one, page, out=plan, stream=_Stream())
+    with pytest.raises(ValueError, match="overflow"):
+        mq.Kv4Cache(1, -(1 << 32) + 4, 16, 2, 64)
+    cache = object.__new__(mq.Kv4Cache)
+    cache.handle, cache.device, cache.layers, cache.kv_heads, cache.head_dim = None, 0, 1, 1, 32
+    for n in (1 << 31, big):
+        with pytest.raises(RuntimeError, match="shape"):
+            cache.store(0, _Rows(n, 1, 32), _Rows(n, 1, 32), _Ints(n), stream=_Stream())
+        with pytest.raises(RuntimeError, match="shape"):
+            cache.attention(0, _Rows(n, 1, 32), _Ints(2), one, _Table(1, 2), out=_Rows(n, 1, 32), stream=_Stream())
+        with pytest.raises(RuntimeError, match="shape"):
+            cache.load(0, _Ints(n), stream=_Stream())
+
+
+class _Stream:
+    cuda_stream = 0
+
+    class device:
+        index = 0
