@@ -255,10 +255,13 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
  * seq_lens [n_seqs] = ctx + new (may be ctx_lens); slots and positions
  * [rows], -1 behind the last request; *n_free_out (may be n_free).
  * A request is refused when a length is negative, when ctx + new passes
- * max_pages * page_size, when its rows pass `rows`, or when it needs pages
- * and it and the requests before it need more than *n_free: its table,
- * length and the stack stay as they were, and its rows get slot -1.
- * *refused counts them. */
+ * max_pages * page_size, when its rows (or, where it brings none, the rows
+ * before it) pass `rows`, or when it needs pages and it and the requests
+ * before it need more than *n_free: its table, length and the stack stay as
+ * they were, and its rows get slot -1. *refused counts them. The rows of a
+ * refused request keep their place in offsets, and mq_kv4_attention, which
+ * knows only lengths, takes them for the request's last cached tokens: finite
+ * values that mean nothing. Tell them by their slots or positions of -1. */
 int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_seqs, int page_size, int *block_tables,
                   int max_pages, const int *free_pages, int n_pages, const int *n_free, int rows, int *offsets,
                   int *seq_lens, int *slots, int *positions, int *n_free_out, int *refused, void *stream);

@@ -134,7 +134,8 @@ def PlanPages(ctx_lens, new_lens, block_tables, free_pages, n_free, page_size: i
     """Gives the requests the pages that their new rows need and maps the rows to slots (mq_pages_plan).
 
     ``block_tables`` ``[n, max_pages]`` is updated in place. ``rows`` is the capacity of the row arrays; with
-    ``out`` (whose ``seq_lens`` may be ``ctx_lens`` and whose ``n_free`` may be ``n_free``) it is theirs.
+    ``out`` (whose ``seq_lens`` may be ``ctx_lens`` and whose ``n_free`` may be ``n_free``) it is theirs. What the
+    attention answers for the rows of a refused request means nothing; their slots and positions are -1.
     """
     torch = _torch()
     if out is None and rows is None:

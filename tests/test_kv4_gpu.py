@@ -970,3 +970,29 @@ def test_output_layouts(mq, torch):
                     with pytest.raises(ValueError, match="overlap"):
                         b.cache.attention(0, q, offsets, lens, b.tables, out=out)
         assert taken > 5
+
+
+@pytest.mark.parametrize("new", [2, 40])
+def test_rows_of_a_refused_request(mq, torch, new):
+    """The plan leaves a refused request's length as it was, so the attention takes its rows for its last cached ones (and
+    for none where it has fewer): finite rows that mean nothing. The other requests' rows are as ever."""
+    lens = [70, 50, 0, 33]
+    b = Batch(mq, torch, lens, 2, 64, 16, seed=4, poison=False, extra=12)
+    used = set(b.tables.flatten().tolist())
+    free = ints(torch, [p for p in range(b.cache.pages) if p not in used])
+    tables = torch.cat([b.tables, torch.full((4, 4), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
+    need = -(-(70 + new) // 16) - 5
+    news = [new, new, new, 0]  # pages for the first request only
+    plan = mq.PlanPages(ints(torch, lens), ints(torch, news), tables, free, ints(torch, [need]), 16, rows=3 * new + 3)
+    assert plan.refused.tolist() == [1 if new == 2 else 2]
+    served = [70 + new, 52 if new == 2 else 50, 0, 33]
+    assert plan.seq_lens.tolist() == served and plan.n_free.tolist() == [0]
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(3 * new + 3, h, 64, generator=g).cuda() for h in (4, 2, 2))
+    b.cache.store(0, k, v, plan.slots)
+    out = b.cache.attention(0, q, plan.offsets, plan.seq_lens, tables, max_new=new)
+    hk, hv = ([torch.cat([h, torch.from_numpy(ref_blocks_fast(torch, z[r * new:(r + 1) * new].cpu())).cuda()])
+               if served[r] > lens[r] else h for r, h in enumerate(held)] for held, z in ((b.hk, k), (b.hv, v)))
+    want, tol = ref_attention(torch, q[:3 * new], hk, hv, news, served, 64 ** -0.5)
+    assert_attention(torch, out[:3 * new], want, tol)
+    assert not out[2 * new:].any()
