@@ -996,3 +996,22 @@ def test_rows_of_a_refused_request(mq, torch, new):
     want, tol = ref_attention(torch, q[:3 * new], hk, hv, news, served, 64 ** -0.5)
     assert_attention(torch, out[:3 * new], want, tol)
     assert not out[2 * new:].any()
+
+
+def test_scores_keep_the_low_parts(mq, torch):
+    """Scores of 16 whose last bits are sums of the queries' lo parts: seven sums of just below 2^-19, the step of 32-bit
+    numbers there, which one addition each to the score would lose. All operands are exact as hi + lo. What may be lost
+    is a step where the score reaches 16, and one where it is rounded: 2 * 2^-19 of a score, half of that times the scale
+    of the output, tanh of half the scores' difference. (2^-20 for weights, sums and quotient.)"""
+    c = mq.Kv4Cache(1, 1, 16, 1, 128)
+    k, v = torch.ones(2, 1, 128, device="cuda"), torch.ones(2, 1, 128, device="cuda")
+    k[1, :, :112] = 0.0
+    v[1] = -1.0
+    c.store(0, k, v, ints(torch, [0, 1]))
+    q = torch.ones(1, 32, 128, device="cuda")
+    q[..., :112] = 2 ** -12 * (1 + 2 ** -11 * (1 - 2 ** -6))
+    scale = 64 * math.log(2)
+    out = c.attention(0, q, ints(torch, [0, 1]), ints(torch, [2]), ints(torch, [[0]]), max_new=1, scale=scale)
+    want = math.tanh(float(q[0, 0, :112].double().sum()) * scale / 2)
+    off = float((out.double() - want).abs().max())
+    assert off <= 2 ** -19 * scale + 2 ** -20, off
