@@ -33,7 +33,6 @@ int fail(int code, const char *fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char *what) {
-  cudaGetLastError();  // reported here: a later call that looks for its own launch's error must not find it
   return fail(MQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

@@ -34,10 +34,16 @@ struct OnDevice {
   }
 };
 
+// An error that is reported is not left behind for the calls that look for their own with cudaGetLastError.
+int report(cudaError_t e, const char *what) {
+  cudaGetLastError();
+  return cuda_fail(e, what);
+}
+
 int check_device(int device) {
   int count = 0;
   const cudaError_t e = cudaGetDeviceCount(&count);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDeviceCount");
+  if (e != cudaSuccess) return report(e, "cudaGetDeviceCount");
   if (device < 0 || device >= count) return fail(MQ_ERR_INVALID, "CUDA device id %d out of range", device);
   if (!gemm_supported(device)) return fail(MQ_ERR_UNSUPPORTED, "the kernels need an sm_100 device (device %d)", device);
   return MQ_OK;
@@ -114,37 +120,41 @@ uint64_t wait_limit() {
   return ns ? std::min<uint64_t>(ns, 10 * kKv4WaitNs) : kKv4WaitNs;  // (never without a bound)
 }
 
-int launched(const char *what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, what);
-  count_launch();
-  return MQ_OK;
-}
-
-// Launched behind the previous kernel of the stream with programmatic
-// serialization: it may start early and waits where it depends on that one.
-// MQ_PDL=0 launches normally, as for the linears.
+// The launch's own status decides: an error that an earlier call of the thread left behind is none of this one's.
 template <typename... KArgs, typename... Args>
-int launch_after(const char *what, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s,
-                 const Args &...args) {
-  static const bool on = [] {
-    const char *e = std::getenv("MQ_PDL");
-    return !e || !*e || std::atoi(e) != 0;
-  }();
+int launch(const char *what, cudaLaunchAttribute attr, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
+           cudaStream_t s, const Args &...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = on;
-  cfg.attrs = attr;
+  cfg.attrs = &attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) return cuda_fail(e, what);
+  if (e != cudaSuccess) return report(e, what);
   count_launch();
   return MQ_OK;
+}
+
+// Launched behind the previous kernel of the stream with programmatic
+// serialization, where that is allowed: it may start early and waits where it
+// depends on that one.
+cudaLaunchAttribute early(bool allowed) {
+  cudaLaunchAttribute a = {};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = allowed;
+  return a;
+}
+
+// MQ_PDL=0 launches normally, as for the linears.
+template <typename... KArgs, typename... Args>
+int launch_after(const char *what, void (*kernel)(KArgs...), const Args &...args) {
+  static const bool on = [] {
+    const char *e = std::getenv("MQ_PDL");
+    return !e || !*e || std::atoi(e) != 0;
+  }();
+  return launch(what, early(on), kernel, args...);
 }
 
 // A kernel's workspace: its CTAs' notes on unfinished items, then the parts.
@@ -171,18 +181,19 @@ void use_workspace(Kv4AttnArgs &a, uint8_t *ws, int ctas) {
 
 // Lets `kernel` use `bytes` of shared memory on `device`; once per device.
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t> &ready) {
+int allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t> &ready) {
   const uint64_t bit = 1ull << (device & 63);
-  if (device < 64 && (ready.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  if (device < 64 && (ready.load(std::memory_order_relaxed) & bit)) return MQ_OK;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && device < 64) ready.fetch_or(bit, std::memory_order_relaxed);
-  return e;
+  if (e != cudaSuccess) return report(e, "cudaFuncSetAttribute");
+  if (device < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  return MQ_OK;
 }
 
 template <int NB>
 int run_attention(Kv4AttnArgs a, const mq_kv4 *c, uint8_t *ws, bool many, cudaStream_t s) {
   static std::atomic<uint64_t> dec_ready{0}, pre_ready{0};
-  MQ_CUDA(allow_smem(kv4_decode_kernel<NB>, DecSmem<NB>::kBytes, c->device, dec_ready));
+  if (int rc = allow_smem(kv4_decode_kernel<NB>, DecSmem<NB>::kBytes, c->device, dec_ready)) return rc;
   Kv4Join j{};
   j.ctas[0] = dec_ctas(c->sms);
   use_workspace(a, ws, j.ctas[0]);
@@ -193,7 +204,7 @@ int run_attention(Kv4AttnArgs a, const mq_kv4 *c, uint8_t *ws, bool many, cudaSt
                             DecSmem<NB>::kBytes, s, a))
     return rc;
   if (many) {
-    MQ_CUDA(allow_smem(kv4_prefill_kernel<NB>, PreSmem<NB>::kAlloc, c->device, pre_ready));
+    if (int rc = allow_smem(kv4_prefill_kernel<NB>, PreSmem<NB>::kAlloc, c->device, pre_ready)) return rc;
     j.ctas[1] = c->sms;
     use_workspace(a, ws + parts_bytes(j.ctas[0], kDecRowTile, a.c.hd), j.ctas[1]);
     a.min_rows = kFewRows + 1, a.max_rows = INT_MAX;
@@ -231,7 +242,7 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   if (reinterpret_cast<uintptr_t>(memory) % 16) return fail(MQ_ERR_INVALID, "cache memory is not aligned to 16 bytes");
   if (int rc = check_device(device)) return rc;
   OnDevice g(device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
   auto *c = new (std::nothrow) mq_kv4;
   if (!c) return fail(MQ_ERR_INVALID, "out of host memory");
   // (The flag is allocated with the device's first handle, which may be made while a stream is captured.)
@@ -240,6 +251,7 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   const int rc = device_err_flag(device, &c->err_dev, &c->err_host);
   cudaThreadExchangeStreamCaptureMode(&mode);
   if (rc) {
+    cudaGetLastError();
     delete c;
     return rc;
   }
@@ -251,14 +263,14 @@ int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads
   if (!base) e = cudaMalloc(&base, bytes);
   if (e != cudaSuccess) {
     delete c;
-    return cuda_fail(e, "cudaMalloc cache");
+    return report(e, "cudaMalloc cache");
   }
   e = cudaMemsetAsync(base, 0, bytes, s);
   if (e == cudaSuccess && !memory) e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) {
     if (!memory) cudaFree(base);
     delete c;
-    return cuda_fail(e, "clear cache");
+    return report(e, "clear cache");
   }
   v.base = static_cast<uint8_t *>(base);
   c->device = device;
@@ -303,12 +315,12 @@ int mq_kv4_store(const mq_kv4 *c, int layer, const float *k, int64_t ld_k, int64
   if (int rc = check_rows("value", v, ld_v, hs_v, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
   OnDevice g(c->device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Kv4Rows kr{k, ld_k, hs_k}, vr{v, ld_v, hs_v};
   auto *kernel = vector16(k, ld_k, hs_k) && vector16(v, ld_v, hs_v) ? kv4_store_kernel<true> : kv4_store_kernel<false>;
-  kernel<<<row_grid(c, rows), kKv4Threads, 0, s>>>(c->v, layer, kr, vr, slots, rows);
-  return launched("cache store");
+  return launch("cache store", early(false), kernel, row_grid(c, rows), kKv4Threads, 0, s, c->v, layer, kr, vr, slots,
+                rows);
 }
 
 int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k, float *v, void *stream) {
@@ -321,11 +333,11 @@ int mq_kv4_load(const mq_kv4 *c, int layer, const int *slots, int rows, float *k
   if (int rc = check_rows("value", v, ld, c->v.hd, c->v.kv, c->v.hd)) return rc;
   if (!slots) return fail(MQ_ERR_INVALID, "null slot map");
   OnDevice g(c->device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto *kernel = vector16(k, 0, 0) && vector16(v, 0, 0) ? kv4_load_kernel<true> : kv4_load_kernel<false>;
-  kernel<<<row_grid(c, rows), kKv4Threads, 0, s>>>(c->v, layer, slots, rows, k, v);
-  return launched("cache load");
+  return launch("cache load", early(false), kernel, row_grid(c, rows), kKv4Threads, 0, s, c->v, layer, slots, rows, k,
+                v);
 }
 
 size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new) {
@@ -353,7 +365,8 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
   if (int rc = check_rows("query", q, ld_q, hs_q, heads, c->v.hd)) return rc;
   if (int rc = check_rows("output", out, ld_out, hs_out, heads, c->v.hd)) return rc;
   if (heads_overlap(rows, ld_out, heads, hs_out, c->v.hd))
-    return fail(MQ_ERR_INVALID, "heads of the output overlap (strides %lld, %lld)", (long long)ld_out, (long long)hs_out);
+    return fail(MQ_ERR_INVALID, "heads of the output overlap (strides %lld, %lld)", (long long)ld_out,
+                (long long)hs_out);
   if (!offsets || !seq_lens || !block_tables) return fail(MQ_ERR_INVALID, "null offsets, lengths or block tables");
   const size_t need = mq_kv4_attention_workspace(c, heads, max_new);
   if (!workspace || workspace_bytes < need)
@@ -365,7 +378,7 @@ int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, i
     return fail(MQ_ERR_TIMEOUT, "an earlier tensor-core launch on device %d ran out of a bounded wait", c->device);
   }
   OnDevice g(c->device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Kv4AttnArgs a{};
   a.c = c->v;
@@ -405,32 +418,26 @@ int mq_pages_plan(int device, const int *ctx_lens, const int *new_lens, int n_se
   if (seq_lens == new_lens && n_seqs) return fail(MQ_ERR_INVALID, "the lengths may not replace the new row counts");
   if (int rc = check_device(device)) return rc;
   OnDevice g(device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
   const PagesArgs a{ctx_lens, new_lens, n_seqs, page_size, block_tables, max_pages, free_pages, n_pages,
                     n_free, rows, offsets, seq_lens, slots, positions, n_free_out, refused,
                     vector16(slots, 0, 0) && vector16(positions, 0, 0), seq_lens == ctx_lens || n_free_out == n_free};
   // (The 48 KB that need no permission count the kernel's static part too.)
   static std::atomic<uint64_t> ready{0};
-  MQ_CUDA(allow_smem(pages_plan_kernel, (int)pages_smem(kPagesMaxSeqs), device, ready));
-  cudaLaunchConfig_t cfg = {};
+  if (int rc = allow_smem(pages_plan_kernel, (int)pages_smem(kPagesMaxSeqs), device, ready)) return rc;
   // A thread for each request and for every four rows, in one CTA while that is enough: a decode step of 8
   // requests took 7.7 us with 1024 threads.
   const int want = std::max(n_seqs, rows / 4);
   const int ctas = (int)std::min<int64_t>(kPagesCtas, ((int64_t)rows + 4 * kPagesThreads - 1) / (4 * kPagesThreads));
-  cfg.gridDim = dim3(ctas <= 1 ? 1 : a.in_place ? kPagesCluster : ctas);
-  cfg.blockDim = dim3(std::min(kPagesThreads, std::max(64, (want + 31) / 32 * 32)));
-  cfg.dynamicSmemBytes = pages_smem(n_seqs);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.in_place ? cfg.gridDim.x : 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  MQ_CUDA(cudaLaunchKernelEx(&cfg, pages_plan_kernel, a));
-  count_launch();
-  return MQ_OK;
+  const dim3 grid(ctas <= 1 ? 1 : a.in_place ? kPagesCluster : ctas);
+  cudaLaunchAttribute cluster = {};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = a.in_place ? grid.x : 1;
+  cluster.val.clusterDim.y = 1;
+  cluster.val.clusterDim.z = 1;
+  return launch("plan pages", cluster, pages_plan_kernel, grid,
+                std::min(kPagesThreads, std::max(64, (want + 31) / 32 * 32)), pages_smem(n_seqs),
+                static_cast<cudaStream_t>(stream), a);
 }
 
 int mq_pages_release(int device, const int *requests, int n, int n_seqs, int page_size, int *seq_lens,
@@ -446,10 +453,10 @@ int mq_pages_release(int device, const int *requests, int n, int n_seqs, int pag
     return fail(MQ_ERR_INVALID, "null pointer");
   if (int rc = check_device(device)) return rc;
   OnDevice g(device);
-  if (g.err != cudaSuccess) return cuda_fail(g.err, "cudaSetDevice");
-  pages_release_kernel<<<1, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      requests, n, n_seqs, page_size, seq_lens, block_tables, max_pages, free_pages, n_pages, n_free);
-  return launched("release pages");
+  if (g.err != cudaSuccess) return report(g.err, "cudaSetDevice");
+  return launch("release pages", early(false), pages_release_kernel, dim3(1), kPagesThreads, 0,
+                static_cast<cudaStream_t>(stream), requests, n, n_seqs, page_size, seq_lens, block_tables, max_pages,
+                free_pages, n_pages, n_free);
 }
 
 }  // extern "C"
