@@ -169,7 +169,7 @@ int mq_linear_noalloc(const mq_weight *w, const float *x, int m, int ldx, const 
  * value row are a Q4_0 block, c * d with c in [-8, 7]: for the block's first
  * element s of largest |x|, d = fp16(bf16(s / -8)), and c = x / d rounded to
  * nearest even and clamped. (d has 8 significant bits, so that every c * d is
- * an fp16 number.) A block with a non-finite element, or whose |d| would pass
+ * an fp16 number; mq_quantize keeps 11, so its blocks hold other values.) A block with a non-finite element, or whose |d| would pass
  * 8160, is stored as NaN, and attention that sees it answers NaN. 4.5 bits an
  * element. No counterpart in the reference, whose forward keeps one
  * max_seq_len F32 cache per context (src/forward.cc).

@@ -8,7 +8,9 @@
 // Rounding d to bf16's 8 significant bits is the one liberty taken with the
 // Q4_0 block: c has at most 3 bits beside its power of two, so that every
 // c * d is an fp16 number exactly, and one fp16 tensor-core operand holds the
-// cache without error. It costs at most 2^-9 of d, against a step of d. x / d
+// cache without error. It costs at most 2^-8 of d, against a step of d (and
+// 2^-25 more below 2^-14, where fp16's numbers stand 2^-24 apart), and it makes
+// values differ from those of a Q4_0 block with its full fp16 scale. x / d
 // is a true division: fp32 then gives the nearest code of the real quotient,
 // since d * (k + 1/2) is an fp32 number and no x beside it divides to k + 1/2.
 // A block with a non-finite element, or whose |d| passes 8160 (8 d would pass
@@ -65,10 +67,12 @@ __device__ __forceinline__ float min_nan(float x, float y) {
 }
 
 // 32 elements over 4 neighbouring lanes, 8 each (lane t: elements 8t..8t+7):
-// this lane's nibbles and the block's scale. Its instructions bound the store of
-// many rows (8192 rows of 8 heads of 128: 26 us, 15.4 million warp instructions,
-// against 11 us of memory traffic); with the extreme's place carried along and
-// every code clamped at both ends they were 18.3 million, 28 us.
+// this lane's nibbles and the block's scale. Its instructions are about half of
+// the time of a store of many rows (8192 rows of 8 heads of 128: 26 us, 15.4
+// million warp instructions, 13 us of issue slots, against 11 us of memory
+// traffic); the rest is the latency of slots, rows and codes one after another.
+// With the extreme's place carried along and every code clamped at both ends
+// they were 18.3 million, 28 us.
 __device__ __forceinline__ uint32_t kv4_pack(const float (&x)[8], uint16_t &scale) {
   float hi = x[0], lo = x[0];
 #pragma unroll

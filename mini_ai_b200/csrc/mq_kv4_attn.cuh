@@ -66,8 +66,8 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 // What beginning and ending an item costs, in steps of BN tokens. Without it
 // the CTAs with many short items end last: a 4096-token prompt took 561 us
-// instead of 372. 4 for the many-row kernel (299 us; 3: 301, 6: 310), 1 for the
-// other (48 ragged chats 90.5 us; 2: 91.1, 4: 96.7).
+// instead of 372. 4 for the many-row kernel (299 us with the queries in L2; 3:
+// 301, 6: 310), 1 for the other (48 ragged chats 90.5 us; 2: 91.1, 4: 96.7).
 template <int RT>
 constexpr int kv4_setup() { return RT == kManyTile ? 4 : 1; }
 
@@ -320,11 +320,12 @@ __device__ __forceinline__ void kv4_add_part(float &top, float &total, float4 &a
 // Tokens of a unit are taken in the order that keeps shared memory free of
 // bank conflicts: column n of score tile i is token (n >> 1) + 4 (n & 1) + 8 i.
 //
-// Bound: issue slots. A unit of 16 tokens x 8 rows x 128 elements costs 519
-// instructions (measured), most of them decoding; at 57 % of the slots that is
-// 2.4 TB/s of cache on 48 ragged chats (90 us; its bytes alone would take 33).
-// Three CTAs an SM: four had to spill (114 us). Two units a step: one took 99
-// us, four 104.
+// Bound: latency of dependent instructions. A unit of 16 tokens x 8 rows x 128
+// elements costs 524 instructions (measured), most of them decoding; 12 warps an
+// SM (168 registers a thread) issue in 57 % of the slots, and that is 2.4 TB/s
+// of cache on 48 ragged chats (89 us; the slots alone would take 43, the bytes
+// 33). Three CTAs an SM: four had to spill (114 us). Two units a step: one took
+// 99 us, four 104.
 constexpr int kDecWarps = 4;
 constexpr int kDecRowTile = 8;
 constexpr int kDecUnits = 2;   // per warp and step

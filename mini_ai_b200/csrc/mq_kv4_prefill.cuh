@@ -7,13 +7,13 @@
 //   S = Qhi K^T + Qlo K^T            [128 rows, 128 tokens], fp32 in TMEM
 //   P = 2^(S f - ref) -> Phi, Plo    one thread a row and half of the columns
 //   O = Phi V + Plo V                [128 rows, hd], fp32 in TMEM
-// (all lo products before the hi ones: an addition truncates the sum that it
-// makes, so the small terms go where the sums are small. With them last,
-// scores lost up to 8 more steps of 2^-23 and outputs were 1.06e-6 off instead
-// of 0.47e-6, four chunks of 300-700 rows),
 // and the running output of a row is in a thread's registers: adding one
 // step's O there costs hd additions a row, keeps every tensor-core sum at 16
 // additions (they truncate), and lets a moved reference scale registers.
+// All lo products come before the hi ones: an addition truncates the sum that it
+// makes, so the small terms go where sums are small. With them last, scores lost
+// up to 8 more steps of 2^-23, and the outputs of four chunks of 300-700 rows
+// were 1.07e-6 off instead of 0.47e-6.
 // Both A operands come from TMEM, so shared memory feeds the tensor cores
 // with B alone (64 of its 128 bytes a clock).
 //
@@ -27,8 +27,12 @@
 //
 // Bound: the tensor cores' 2048 clocks a step (twice 4 hd operations a (row,
 // token) pair), and nearly as much the softmax chain of a step, which is longer
-// by a quarter. Measured: a 4096-token prompt of 32 heads of 128 in 299 us, 0.92
-// PFLOP/s of MMAs. With the running output in the softmax warps, 372.
+// by a quarter. Measured: a 4096-token prompt of 32 heads of 128 in 334 us, 0.82
+// PFLOP/s of MMAs, where every pass has new queries, and 307 us with the queries
+// in L2 (there 372 with the running output in the softmax warps).
+//
+// A wait that runs out makes the CTA's roles leave, whatever they have before
+// them; the join then writes NaN for all that the CTA had (kv4_void).
 #pragma once
 
 #include "mq_kv4_attn.cuh"

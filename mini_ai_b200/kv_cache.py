@@ -251,7 +251,8 @@ class Kv4Cache:
         ``offsets`` ``[n + 1]`` and ``seq_lens`` ``[n]`` as ``PlanPages`` gives them, ``block_tables``
         ``[n, max_pages]``. ``max_new`` is the most rows that a request brings (None: unknown). Rows past
         ``offsets[n]`` of ``out`` stay as they are; without ``out`` they are 0. ``scale`` defaults to
-        1 / sqrt(head_dim).
+        1 / sqrt(head_dim). ``MQError`` (``MQ_ERR_TIMEOUT``): a wait of an earlier launch on the device ran out, and
+        rows of its output are NaN.
         """
         torch = _torch()
         device = self.device
