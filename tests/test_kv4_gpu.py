@@ -820,29 +820,46 @@ def _run_child(code, last):
     assert r.returncode == 0 and r.stdout.splitlines()[-1:] == [last], r.stdout + r.stderr
 
 
-def test_a_failed_call_leaves_no_error_behind(mq, torch):
-    """A call that could not get its memory fails alone: the calls after it do not report its error."""
-    rng = np.random.default_rng(0)
-    w = mq.CudaWeight(mq.QuantizeTensor(rng.standard_normal((128, 256)).astype(np.float32), mq.QuantType.kQ40), device=0)
-    x = torch.zeros(1, 256, device="cuda")
-    c, at = mq.Kv4Cache(1, 1, 16, 1, 32), ints(torch, [3])
-    row = torch.randn(1, 1, 32, device="cuda")
-    lens, tables, stack, n_free = ints(torch, [5]), ints(torch, [[0]]), ints(torch, [7, 7]), ints(torch, [1])
-    torch.cuda.synchronize()
+def test_errors_of_earlier_calls():
+    """A call reports its own errors only: not that of a product before it that could not get its memory. (In a process
+    of its own, which takes the error that the product leaves behind with it.)"""
+    _run_child(EARLIER_ERRORS, "done")
 
-    def fail():  # the gate product of these rows would take 8 TiB; nothing is launched
-        rc = mq.lib().mq_linear_swiglu(w.handle, w.handle, x.data_ptr(), 1 << 20, 256, x.data_ptr(), 1 << 21, None)
-        assert rc == mq._lib.MQ_ERR_CUDA and "memory" in mq._lib.last_error()
 
-    fail()
-    c.store(0, row, -row, at)
-    fail()
-    k, v = c.load(0, at)
-    assert torch.equal(k, -v) and k.any()
-    fail()
-    mq.ReleasePages(ints(torch, [0]), lens, tables, stack, n_free, 16)
-    assert n_free.tolist() == [2] and stack.tolist() == [7, 0]
-    w.close()
+EARLIER_ERRORS = """
+import numpy as np, torch, mini_ai_b200 as mq
+from test_kv4_gpu import ints
+rng = np.random.default_rng(0)
+w = mq.CudaWeight(mq.QuantizeTensor(rng.standard_normal((128, 256)).astype(np.float32), mq.QuantType.kQ40), device=0)
+x = torch.zeros(1, 256, device="cuda")
+c, at = mq.Kv4Cache(1, 1, 16, 1, 32), ints(torch, [3])
+row = torch.randn(1, 1, 32, device="cuda")
+lens, tables, stack, n_free = ints(torch, [5]), ints(torch, [[0]]), ints(torch, [7, 7]), ints(torch, [1])
+torch.cuda.synchronize()
+
+
+def fail():  # the gate product of these rows would take 8 TiB; nothing is launched
+    rc = mq.lib().mq_linear_swiglu(w.handle, w.handle, x.data_ptr(), 1 << 20, 256, x.data_ptr(), 1 << 21, None)
+    assert rc == mq._lib.MQ_ERR_CUDA and "memory" in mq._lib.last_error()
+
+
+fail()
+c.store(0, row, -row, at)
+fail()
+k, v = c.load(0, at)
+assert torch.equal(k, -v) and k.any()
+fail()
+mq.ReleasePages(ints(torch, [0]), lens, tables, stack, n_free, 16)
+assert n_free.tolist() == [2] and stack.tolist() == [7, 0]
+fail()
+q = torch.randn(1, 32, 32, device="cuda")
+for max_new in (0, 1):
+    c.attention(0, q, ints(torch, [0, 1]), ints(torch, [4]), tables, max_new=max_new)
+plan = mq.PlanPages(lens, ints(torch, [1]), tables, stack, n_free, 16, rows=1)
+assert plan.refused.tolist() == [0]
+w.close()
+print("done")
+"""
 
 
 WAITS = [  # heads, kv, head size, cached tokens, new rows: few rows whole and cut; many rows whole, cut, many items a CTA
