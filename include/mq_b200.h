@@ -168,11 +168,12 @@ int mq_linear_noalloc(const mq_weight *w, const float *x, int m, int ldx, const 
  * request; page ids are shared by the layers. Every 32 elements of a key or
  * value row are a Q4_0 block, c * d with c in [-8, 7]: for the block's first
  * element s of largest |x|, d = fp16(bf16(s / -8)), and c = x / d rounded to
- * nearest even and clamped. (d has 8 significant bits, so that every c * d is
- * an fp16 number; mq_quantize keeps 11, so its blocks hold other values.) A block with a non-finite element, or whose |d| would pass
- * 8160, is stored as NaN, and attention that sees it answers NaN. 4.5 bits an
- * element. No counterpart in the reference, whose forward keeps one
- * max_seq_len F32 cache per context (src/forward.cc).
+ * nearest even and clamped. (d has 8 significant bits, so that every c * d
+ * is an fp16 number; mq_quantize keeps 11, so its blocks hold other values.)
+ * A block with a non-finite element, or whose |d| would pass 8160, is stored
+ * as NaN, and attention that sees it answers NaN. 4.5 bits an element. No
+ * counterpart in the reference, whose forward keeps one max_seq_len F32
+ * cache per context (src/forward.cc).
  *
  * A step: mq_pages_plan once, then for each layer mq_kv4_store and
  * mq_kv4_attention on the same stream. All lengths, offsets and tables are
@@ -187,13 +188,13 @@ size_t mq_kv4_bytes(int layers, int pages, int page_size, int kv_heads, int head
 
 /* A cache of zeros on `device`. page_size: a multiple of 16 up to 1024;
  * head_dim: 32, 64, 96 or 128; kv_heads up to 65536; pages * page_size <
- * 2^31. `memory` is the
- * caller's device memory for it (at least mq_kv4_bytes(), 16-byte aligned),
- * which must outlive the handle and is cleared on `stream`; NULL allocates
- * it, which synchronizes `stream`. MQ_KV4_WAIT_NS in the environment limits
- * each wait inside the cache's attention (nanoseconds, default 1 s, at most 10 s); with
- * MQ_KV4_LOSE_COPIES=1 every such wait runs out, so that a program's handling
- * of MQ_ERR_TIMEOUT can be tried. */
+ * 2^31. `memory` is the caller's device memory for it (at least
+ * mq_kv4_bytes(), 16-byte aligned), which must outlive the handle and is
+ * cleared on `stream`; NULL allocates it, which synchronizes `stream`.
+ * MQ_KV4_WAIT_NS in the environment limits each wait inside the cache's
+ * attention (nanoseconds, default 1 s, at most 10 s); with
+ * MQ_KV4_LOSE_COPIES=1 every such wait runs out, so that a program's
+ * handling of MQ_ERR_TIMEOUT can be tried. */
 int mq_kv4_create(int device, int layers, int pages, int page_size, int kv_heads, int head_dim, void *memory,
                   size_t memory_bytes, void *stream, mq_kv4 **out);
 void mq_kv4_destroy(mq_kv4 *c);
@@ -226,21 +227,22 @@ size_t mq_kv4_attention_workspace(const mq_kv4 *c, int heads, int max_new);
  * sees positions 0 up to its own, at most seq_lens[r] of them:
  *   out = softmax(scale * q . k) v, query head h with KV head h / (heads / kv_heads).
  * seq_lens counts the step's own rows, which mq_kv4_store has written.
- * block_tables [n_seqs][max_pages] page ids, max_pages * page_size <=
- * 2^31 - 4097; lengths past max_pages * page_size count as that, and tokens of a page id outside the cache are not
- * seen. A row that sees nothing is 0; rows past offsets[n_seqs] stay as they
- * are, and no row past `rows` is touched. max_new: the most rows that a
- * request brings, as far as the caller knows; it selects kernels and a lower
- * or higher value costs time only. q and out as in mq_kv4_store, no two heads
- * of out sharing memory; out may be q only if it has q's strides. F32 softmax and sums; q and the softmax weights
+ * block_tables [n_seqs][max_pages] page ids, max_pages * page_size <= 2^31 -
+ * 4097; lengths past max_pages * page_size count as that, and tokens of a
+ * page id outside the cache are not seen. A row that sees nothing is 0; rows
+ * past offsets[n_seqs] stay as they are, and no row past `rows` is touched.
+ * max_new: the most rows that a request brings, as far as the caller knows;
+ * it selects kernels and a lower or higher value costs time only. q and out
+ * as in mq_kv4_store, no two heads of out sharing memory; out may be q only
+ * if it has q's strides. F32 softmax and sums; q and the softmax weights
  * enter the tensor cores as fp16 hi + lo pairs (22 bits). workspace: device
  * memory of at least mq_kv4_attention_workspace() bytes, 16-byte aligned,
  * not shared with a call that may run at the same time; its contents do not
  * matter. The summation order is fixed: equal inputs give equal bits. Every
  * wait of the kernels is bounded: where one runs out, all rows that its CTA
  * had still to write are NaN, and so are the cut rows that it had a part in;
- * the device's error flag (mq_device_error_flag) is raised, and the next call
- * returns MQ_ERR_TIMEOUT without launching anything. */
+ * the device's error flag (mq_device_error_flag) is raised, and the next
+ * call returns MQ_ERR_TIMEOUT without launching anything. */
 int mq_kv4_attention(const mq_kv4 *c, int layer, const float *q, int64_t ld_q, int64_t hs_q, int rows, int heads,
                      const int *offsets, const int *seq_lens, const int *block_tables, int n_seqs, int max_pages,
                      int max_new, float scale, float *out, int64_t ld_out, int64_t hs_out, void *workspace,

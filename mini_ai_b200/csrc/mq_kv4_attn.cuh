@@ -331,10 +331,12 @@ constexpr int kDecRowTile = 8;
 constexpr int kDecUnits = 2;   // per warp and step
 constexpr int kDecTokens = kDecWarps * kDecUnits * kKv4Unit;  // BN
 constexpr int kDecStages = 3;
-// Steps that one accumulator sums, two products each: a product truncates what it adds to, by up to 2^-23 of it and
-// always towards 0, and equal weights added one by one round the same way every time. 131072 tokens a CTA put outputs
-// 1.9e-4 off in one chain. Chains are joined in F32, in the place of the item's part; CTAs
-// of up to 4096 tokens have one. 32 requests of 32768 tokens, 8 KV heads of 128: 412 us (64 steps: 409, no bound: 408).
+// Steps that one accumulator sums, two products each: a product truncates what
+// it adds to, by up to 2^-23 of it and always towards 0, and equal weights added
+// one by one round the same way every time (131072 tokens a CTA put outputs
+// 1.9e-4 off in one chain). Chains are joined in F32, in the place of the item's
+// part; up to 4096 tokens are one. 32 requests of 32768 tokens, 8 KV heads of
+// 128: 412 us (64 steps: 409, no bound: 408).
 constexpr int kDecChain = 32;
 constexpr uint64_t kKv4WaitNs = 1000000000ull;  // limit of a wait, unless the cache was made with another
 constexpr uint64_t kKv4DrainNs = 20000000ull;   // for what a CTA that gave up still has in flight

@@ -224,6 +224,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       return sm100::mbar_wait_sleep(bar, parity, nullptr, abort, a.wait_ns);
     };
+    // What is still in flight at the end. (Looked at once more when the time is up: it may have passed while another
+    // process had the device.)
+    auto drain = [&](uint64_t *bar, uint32_t parity) {
+      if (!sm100::mbar_wait(bar, parity, nullptr, nullptr, kKv4DrainNs) && !sm100::mbar_try_wait(bar, parity)) *abort = 1;
+    };
     Ring<kPreSegs> sg;
     // The next segment of a role's warp; false at the end. seg_done() lets the walker reuse its place.
     auto seg_next = [&]() {
@@ -739,7 +744,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
         if (elect_one()) {  // every MMA has completed before the TMEM is released
           sm100::umma_commit(fin);
-          if (!sm100::mbar_wait(fin, 0u, nullptr, nullptr, kKv4DrainNs)) *abort = 1;
+          drain(fin, 0u);
         }
       } else if (warp == kWarpCopy) {
         // ------------------------------------------------------ copies of the packed units
@@ -774,8 +779,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const Kv4At
         }
         // the last copies have landed before the CTA can exit
         for (int i = max(0, issued - kPreRaw); i < issued; ++i)
-          if (!sm100::mbar_wait(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u, nullptr, nullptr, kKv4DrainNs))
-            *abort = 1;
+          drain(&raw_full[i % kPreRaw], (uint32_t)(i / kPreRaw) & 1u);
       } else if (warp == kWarpWalk && lane == 0) {
         // ------------------------------------------------------ the walk over the items
         Kv4Segment s;
